@@ -414,6 +414,88 @@ ORT_CUDA_API int ort_cuda_rotary_embedding(ort_cuda_session* s, const float* X,
                                            int64_t seq, int64_t heads, int64_t head_size,
                                            int64_t rotary_dim, float* Y, int flags);
 
+/* ---- paged KV cache ----------------------------------------------------
+ * The cache of many sequences of different lengths, as the com.microsoft
+ * PagedAttention operator lays it out: pages of page_size tokens, each
+ * [page_size, kv_num_heads, head_size], found through a block table.  No
+ * counterpart in the reference, whose cache is one dense past per call
+ * (lib/src/onnx_ops.dart:1507-1650).
+ *
+ * A call carries `num_tokens` packed tokens: sequence b holds tokens
+ * [cu_seqlens[b], cu_seqlens[b + 1]) at positions past_lens[b],
+ * past_lens[b] + 1, ...; position p of it is row p % page_size of page
+ * block_table[b * max_pages + p / page_size].  Tokens behind the last
+ * sequence (from cu_seqlens[batch] on) are padding: nothing of them is read
+ * into the cache and their output rows are left as they were.  A sequence
+ * may have no tokens.
+ *
+ * The structure lives on the host; every pointer in it is a device pointer.
+ * Lengths and pages are read on the device when the kernels run, so a
+ * recorded call follows what the caller writes there between replays.  What
+ * does not fit (cu_seqlens that fall or pass num_tokens, a negative
+ * past_lens, more tokens than max_pages * page_size, a page outside
+ * [0, num_pages), ...) is never followed: the sequence, or the keys of the
+ * page, are left out, and the next synchronising call returns
+ * ORT_CUDA_ERR_INVALID_ARG. */
+#define ORT_CUDA_CACHE_F32 0
+#define ORT_CUDA_CACHE_F16 1
+#define ORT_CUDA_CACHE_BF16 2
+typedef struct ort_cuda_paged_cache {
+  void* key;                  /* [num_pages, page_size, kv_num_heads, head_size]   */
+  void* value;                /* the same; both 16-byte aligned                    */
+  const int32_t* block_table; /* [batch, max_pages]                                */
+  const int32_t* cu_seqlens;  /* [batch + 1]                                       */
+  const int32_t* past_lens;   /* [batch]: tokens in the cache before this call     */
+  int64_t num_pages, page_size, max_pages, batch, head_size;
+  int32_t kv_num_heads;
+  int32_t type;               /* ORT_CUDA_CACHE_*: the element type of the pages   */
+} ort_cuda_paged_cache;
+
+/* Appends this call's keys and values to the cache, with RoPE of the keys
+ * (and, when Q is given, of the queries) on the way: key row = R(position) .
+ * K, value row = V, each rounded once to the cache's type; Q_out = R(position)
+ * . Q in fp32.  K and V are [num_tokens, kv_num_heads * head_size] fp32 with
+ * rows k_stride and v_stride floats apart (slices of a fused projection's
+ * output need no copy), Q [num_tokens, num_heads * head_size] with row stride
+ * q_stride, or NULL with Q_out NULL; Q_out is contiguous and may be Q itself
+ * when q_stride is its row length.  cos/sin caches [max_pos, rotary_half] as
+ * for ort_cuda_group_query_attention (ORT_CUDA_ROTARY_INTERLEAVED for (2i, 2i + 1)
+ * pairs; a position >= max_pos is not rotated but left out, and reported as
+ * above), or both NULL: no rotation.  The rows of one call must be distinct
+ * (no page listed twice within the written range).  head_size a multiple of 8
+ * up to 128.  Device pointers only; stream-ordered. */
+ORT_CUDA_API int ort_cuda_paged_kv_append(ort_cuda_session* s, const ort_cuda_paged_cache* cache,
+                                          const float* Q, int64_t q_stride, const float* K,
+                                          int64_t k_stride, const float* V, int64_t v_stride,
+                                          int64_t num_tokens, int num_heads,
+                                          const float* cos_cache, const float* sin_cache,
+                                          int64_t rotary_half, int64_t max_pos, float* Q_out,
+                                          int flags);
+
+/* Attention of this call's queries over the cache that already holds their
+ * keys and values (ort_cuda_paged_kv_append first).  The query at position p
+ * of its sequence sees keys j <= p of that sequence and, with window > 0,
+ * only j > p - window (window keys, its own among them; <= 0: all).  Scores
+ * are scale * q.k (scale <= 0: 1/sqrt(head_size)) and, with softcap > 0,
+ * softcap * tanh(score / softcap).  Q [num_tokens, num_heads * head_size] fp32
+ * with row stride q_stride; out [num_tokens, num_heads * head_size] fp32,
+ * contiguous.  Query head h reads KV head h / (num_heads / kv_num_heads).
+ *   max_seq     bound of the tokens of any one sequence of the call (a
+ *               sequence with more is left out and reported)
+ *   shared_len  > 0: the first shared_len positions of every sequence hold
+ *               the same tokens, and are read through the first row of the
+ *               block table, once for the whole batch; every past_lens[b]
+ *               of a sequence with tokens must be at least shared_len
+ * fp32 results whatever the cache's type: products, softmax statistics and
+ * sums keep 22 bits or more.  Device pointers only; stream-ordered.  A call
+ * uses a workspace of its stream (or of the graph being captured), so calls
+ * on different streams may run at the same time. */
+ORT_CUDA_API int ort_cuda_paged_attention(ort_cuda_session* s, const ort_cuda_paged_cache* cache,
+                                          const float* Q, int64_t q_stride, int64_t num_tokens,
+                                          int64_t max_seq, int num_heads, double scale,
+                                          double softcap, int64_t window, int64_t shared_len,
+                                          float* out, int flags);
+
 /* TopK (opTopK, lib/src/onnx_ops.dart:2261-2303) over the last axis of X,
  * a [rows x cols] fp32 matrix with row stride ldx: values[r][0..k) and
  * indices[r][0..k) (int64) in the reference's order -- value descending

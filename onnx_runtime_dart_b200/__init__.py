@@ -6,7 +6,7 @@ build (build.py) and a Python mirror of the reference's operator interface
 (session.py) used by the tests and the benchmark.
 """
 from ._lib import StateError, UnsupportedError  # noqa: F401
-from .session import (CudaSession, DeviceTensor, default_session, op_gemm,  # noqa: F401
-                      op_matmul, op_matmul_nbits)
+from .session import (CudaSession, DeviceTensor, PagedKVCache, default_session,  # noqa: F401
+                      op_gemm, op_matmul, op_matmul_nbits)
 
 __version__ = "0.1.0"

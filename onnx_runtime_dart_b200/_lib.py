@@ -52,13 +52,24 @@ ROTARY_INTERLEAVED = 0x200
 ROTARY_BHSD = 0x400
 TOPK_SMALLEST = 0x800
 FUSE_DROP_PARTS = 0x1  # ort_cuda_fuse_nbits flags
+CACHE_F32, CACHE_F16, CACHE_BF16 = 0, 1, 2  # ort_cuda_paged_cache element types
 
-# Every symbol include/ort_cuda.h declares, with (restype, argtypes).
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f = ctypes.c_float
 _cp = ctypes.c_char_p
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """ort_cuda_paged_cache."""
+    _fields_ = [("key", _vp), ("value", _vp), ("block_table", _vp), ("cu_seqlens", _vp),
+                ("past_lens", _vp), ("num_pages", _i64), ("page_size", _i64),
+                ("max_pages", _i64), ("batch", _i64), ("head_size", _i64),
+                ("kv_num_heads", ctypes.c_int32), ("type", ctypes.c_int32)]
+
+
+# Every symbol include/ort_cuda.h declares, with (restype, argtypes).
 SIGNATURES = {
     "ort_cuda_last_error": (ctypes.c_char_p, []),
     "ort_cuda_version": (ctypes.c_char_p, []),
@@ -104,6 +115,10 @@ SIGNATURES = {
                                    _i64, ctypes.c_double, _vp, _int]),
     "ort_cuda_rotary_embedding": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _i64, _i64, _i64, _i64,
                                          _i64, _i64, _i64, _vp, _int]),
+    "ort_cuda_paged_kv_append": (_int, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _int,
+                                        _vp, _vp, _i64, _i64, _vp, _int]),
+    "ort_cuda_paged_attention": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, ctypes.c_double,
+                                        ctypes.c_double, _i64, _i64, _vp, _int]),
     "ort_cuda_graph_begin": (_int, [_vp]),
     "ort_cuda_graph_end": (_int, [_vp, ctypes.POINTER(_int)]),
     "ort_cuda_graph_launch": (_int, [_vp, _int]),

@@ -31,6 +31,20 @@ int cuda_fail(cudaError_t e, const char* what);
     if (!(cond)) return ::ortc::fail((code), (msg));     \
   } while (0)
 
+// Makes the session's device current for the call and restores the caller's.
+struct DeviceGuard {
+  int prev = -1;
+  explicit DeviceGuard(int dev) {
+    cudaGetDevice(&prev);
+    if (prev != dev) cudaSetDevice(dev);
+  }
+  ~DeviceGuard() {
+    int cur = -1;
+    cudaGetDevice(&cur);
+    if (prev >= 0 && cur != prev) cudaSetDevice(prev);
+  }
+};
+
 // ---- weights -------------------------------------------------------------
 enum WeightKind { W_NBITS = 1, W_DENSE = 2, W_INT8 = 3, W_GROUP = 4 };
 constexpr int kMaxSegs = 4;  // weights in one fused group (ort_cuda_fuse_nbits)
@@ -120,6 +134,10 @@ __host__ __device__ __forceinline__ uint32_t nbits_zp(const uint8_t* zp, int64_t
 }  // namespace ortc
 
 struct ort_cuda_profile;  // per-op-type device times (csrc/profile.cu)
+namespace ortc {
+struct PagedScratch;  // workspaces of the paged attention (csrc/paged.cu)
+void paged_free(ort_cuda_session* s);
+}
 
 struct ort_cuda_session {
   int device = 0;
@@ -153,6 +171,8 @@ struct ort_cuda_session {
   // to zero by every call) then partials
   void* attnscratch = nullptr;
   size_t attn_bytes = 0;
+  // paged attention: one workspace per stream or captured graph
+  ortc::PagedScratch* paged = nullptr;
   // N-sharded sessions: peer-memory exchange of Y (csrc/p2p.cu).  xbuf holds
   // a 256-byte flag area (8 peer flags, epoch counter, CTA counter) then two
   // halves of xcap floats; xpeer[r] is rank r's xbuf mapped into this

@@ -1,0 +1,395 @@
+// The paged KV cache: C entry points (include/ort_cuda.h), the workspaces of
+// its attention, and the append kernel.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <map>
+#include <memory>
+#include <mutex>
+#include <utility>
+#include <vector>
+
+#include <cuda_bf16.h>
+
+#include "paged.cuh"
+
+namespace ortc {
+
+// ---- workspaces ----------------------------------------------------------------
+// A call's workspace belongs to the stream it is launched on, or to the graph
+// being captured on that stream: calls on two streams, and two captured graphs
+// replayed at once, never share one.  A graph's workspace is handed back when
+// the graph and everything instantiated from it are gone (a CUDA user object),
+// and is reused by later captures.  The first kTicketBytes are zero between calls.
+constexpr size_t kTicketBytes = 4096;
+
+struct PagedScratch {
+  struct Buf {
+    void* p = nullptr;
+    size_t bytes = 0;
+  };
+  struct Pool {  // outlives the session while a graph still holds a workspace
+    std::mutex m;
+    std::vector<Buf> idle;
+  };
+  std::shared_ptr<Pool> pool = std::make_shared<Pool>();
+  std::vector<void*> all;
+  std::map<cudaStream_t, Buf> streams;
+  unsigned long long capture = 0;  // the capture `captured` belongs to
+  std::map<cudaStream_t, Buf> captured;
+};
+
+namespace {
+
+struct GraphHold {
+  std::shared_ptr<PagedScratch::Pool> pool;
+  PagedScratch::Buf buf;
+};
+
+void CUDART_CB release_hold(void* p) {
+  auto* h = static_cast<GraphHold*>(p);
+  {
+    std::lock_guard<std::mutex> lock(h->pool->m);
+    h->pool->idle.push_back(h->buf);
+  }
+  delete h;
+}
+
+// A new zeroed workspace, also while a stream is being captured.
+int new_buf(PagedScratch* w, size_t bytes, PagedScratch::Buf* out) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  ORTC_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+  PagedScratch::Buf b;
+  cudaStream_t st = nullptr;
+  cudaError_t e = cudaMalloc(&b.p, bytes);
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(b.p, 0, kTicketBytes, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (st) cudaStreamDestroy(st);
+  if (e != cudaSuccess && b.p) cudaFree(b.p);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return cuda_fail(e, "paged attention workspace");
+  b.bytes = bytes;
+  w->all.push_back(b.p);
+  *out = b;
+  return ORT_CUDA_OK;
+}
+
+int paged_scratch(ort_cuda_session* s, size_t bytes, void** out) {
+  *out = nullptr;
+  if (bytes == 0) return ORT_CUDA_OK;
+  if (!s->paged) s->paged = new PagedScratch();
+  PagedScratch* w = s->paged;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  cudaGraph_t graph = nullptr;
+  ORTC_CUDA(cudaStreamGetCaptureInfo_v2(s->stream, &status, &id, &graph, nullptr, nullptr));
+  if (status == cudaStreamCaptureStatusNone) {
+    PagedScratch::Buf& b = w->streams[s->stream];
+    if (bytes > b.bytes) {
+      if (b.p) {
+        ORTC_CUDA(cudaStreamSynchronize(s->stream));
+        ORTC_CUDA(cudaFree(b.p));
+        w->all.erase(std::find(w->all.begin(), w->all.end(), b.p));
+        b = PagedScratch::Buf();
+      }
+      const int rc = new_buf(w, bytes, &b);
+      if (rc) return rc;
+    }
+    *out = b.p;
+    return ORT_CUDA_OK;
+  }
+  ORTC_CHECK(status == cudaStreamCaptureStatusActive, ORT_CUDA_ERR_CUDA,
+             "paged attention: the stream's capture was invalidated");
+  if (w->capture != id) {
+    w->captured.clear();
+    w->capture = id;
+  }
+  PagedScratch::Buf& b = w->captured[s->stream];
+  if (bytes > b.bytes) {
+    PagedScratch::Buf got;
+    {
+      std::lock_guard<std::mutex> lock(w->pool->m);
+      auto& idle = w->pool->idle;
+      for (size_t i = 0; i < idle.size(); i++)
+        if (idle[i].bytes >= bytes) {
+          got = idle[i];
+          idle.erase(idle.begin() + i);
+          break;
+        }
+    }
+    if (!got.p) {
+      const int rc = new_buf(w, bytes, &got);
+      if (rc) return rc;
+    }
+    auto* hold = new GraphHold{w->pool, got};
+    cudaUserObject_t obj = nullptr;
+    cudaError_t e = cudaUserObjectCreate(&obj, hold, release_hold, 1, cudaUserObjectNoDestructorSync);
+    if (e != cudaSuccess) {
+      release_hold(hold);
+      return cuda_fail(e, "cudaUserObjectCreate");
+    }
+    e = cudaGraphRetainUserObject(graph, obj, 1, cudaGraphUserObjectMove);
+    if (e != cudaSuccess) {
+      cudaUserObjectRelease(obj, 1);
+      return cuda_fail(e, "cudaGraphRetainUserObject");
+    }
+    b = got;
+  }
+  *out = b.p;
+  return ORT_CUDA_OK;
+}
+
+}  // namespace
+
+void paged_free(ort_cuda_session* s) {
+  if (!s->paged) return;
+  for (void* p : s->paged->all) cudaFree(p);
+  delete s->paged;
+  s->paged = nullptr;
+}
+
+// ---- append ----------------------------------------------------------------------
+namespace {
+
+struct AppendArgs {
+  PagedView c;
+  const float* q = nullptr;
+  const float* k = nullptr;
+  const float* v = nullptr;
+  int64_t q_stride = 0, k_stride = 0, v_stride = 0;
+  float* q_out = nullptr;
+  int heads = 0;  // query heads, 0 without Q
+  const float* cos = nullptr;
+  const float* sin = nullptr;
+  int half = 0, interleaved = 0;
+  int64_t max_pos = 0;
+};
+
+template <typename T>
+__device__ __forceinline__ T to_cache(double x);
+template <>
+__device__ __forceinline__ float to_cache<float>(double x) {
+  return (float)x;
+}
+template <>
+__device__ __forceinline__ __half to_cache<__half>(double x) {
+  return __double2half(x);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 to_cache<__nv_bfloat16>(double x) {
+  return __double2bfloat16(x);
+}
+
+// One CTA per token: every feature of the token's query, key and value heads.
+template <typename T>
+__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
+  const PagedView& c = a.c;
+  const int t = blockIdx.x;
+  if (t == 0)  // sequences that no token of the call reaches are checked too
+    for (int b = threadIdx.x; b < c.batch; b += blockDim.x) paged_seq(c, b, INT_MAX, 0);
+  __shared__ int s_b, s_pos;
+  __shared__ int64_t s_off;
+  if (threadIdx.x < 32) {
+    const int b = paged_find(c, t);
+    if (threadIdx.x == 0) {
+      s_b = -1;
+      const PagedSeq s = b < c.batch ? paged_seq(c, b, INT_MAX, 0) : PagedSeq{0, 0, 0};
+      if (t >= s.row0 && t < s.row0 + s.count) {
+        const int pos = s.past + t - s.row0;
+        if (a.half && pos >= a.max_pos) {
+          record_error(c.err, KERR_PAGED_POSITION);
+        } else {
+          s_b = b;
+          s_pos = pos;
+          s_off = paged_row(c, b, pos);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (s_b < 0) return;
+  const int pos = s_pos, D = c.D, half = a.half;
+  const int64_t off = s_off;
+  const float* cs = a.cos + (int64_t)pos * half;
+  const float* sn = a.sin + (int64_t)pos * half;
+  const int per = D - half;  // pairs, then the features behind them
+  const int n = (a.heads + 2 * c.kv_heads) * per;
+  for (int e = threadIdx.x; e < n; e += blockDim.x) {
+    int h = e / per;
+    const int i = e - h * per;
+    const bool pair = i < half;
+    const int a0 = pair ? (a.interleaved ? 2 * i : i) : i + half;
+    const int a1 = pair ? (a.interleaved ? 2 * i + 1 : i + half) : a0;
+    if (h < a.heads) {
+      const float* src = a.q + t * a.q_stride + (int64_t)h * D;
+      float* dst = a.q_out + ((int64_t)t * a.heads + h) * D;
+      const double x0 = src[a0], x1 = src[a1];
+      if (pair) {
+        dst[a0] = (float)(x0 * cs[i] - x1 * sn[i]);
+        dst[a1] = (float)(x1 * cs[i] + x0 * sn[i]);
+      } else {
+        dst[a0] = (float)x0;
+      }
+      continue;
+    }
+    if (off < 0) continue;
+    h -= a.heads;
+    const bool is_v = h >= c.kv_heads;
+    if (is_v) h -= c.kv_heads;
+    const float* src =
+        (is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride) + (int64_t)h * D;
+    T* dst = static_cast<T*>(is_v ? c.value : c.key) + off + (int64_t)h * D;
+    const double x0 = src[a0], x1 = src[a1];
+    if (pair && !is_v) {
+      dst[a0] = to_cache<T>(x0 * cs[i] - x1 * sn[i]);
+      dst[a1] = to_cache<T>(x1 * cs[i] + x0 * sn[i]);
+    } else {
+      dst[a0] = to_cache<T>(x0);
+      if (pair) dst[a1] = to_cache<T>(x1);
+    }
+  }
+}
+
+int launch_append(const AppendArgs& a, cudaStream_t st, int64_t* launches) {
+  switch (a.c.type) {
+    case ORT_CUDA_CACHE_F32:
+      append_kernel<float><<<a.c.num_tokens, 256, 0, st>>>(a);
+      break;
+    case ORT_CUDA_CACHE_F16:
+      append_kernel<__half><<<a.c.num_tokens, 256, 0, st>>>(a);
+      break;
+    default:
+      append_kernel<__nv_bfloat16><<<a.c.num_tokens, 256, 0, st>>>(a);
+  }
+  ORTC_CUDA(cudaGetLastError());
+  (*launches)++;
+  return ORT_CUDA_OK;
+}
+
+// Checks what the host can see of a cache and fills the kernels' view.
+int paged_view(ort_cuda_session* s, const ort_cuda_paged_cache* c, int64_t num_tokens, int flags,
+               PagedView* v) {
+  ORTC_CHECK(s && c, ORT_CUDA_ERR_INVALID_ARG, "NULL argument");
+  ORTC_CHECK((flags & ORT_CUDA_HOST_IO) == 0, ORT_CUDA_ERR_INVALID_ARG,
+             "the paged KV cache takes device tensors");
+  ORTC_CHECK(c->type == ORT_CUDA_CACHE_F32 || c->type == ORT_CUDA_CACHE_F16 ||
+                 c->type == ORT_CUDA_CACHE_BF16,
+             ORT_CUDA_ERR_UNSUPPORTED, "paged KV cache: unknown element type");
+  ORTC_CHECK(c->batch >= 0 && c->num_pages >= 0 && c->page_size >= 1 && c->max_pages >= 0 &&
+                 c->kv_num_heads >= 1 && c->head_size >= 1 && num_tokens >= 0,
+             ORT_CUDA_ERR_INVALID_ARG,
+             "paged KV cache: need page_size, kv_num_heads, head_size >= 1 and sizes >= 0");
+  ORTC_CHECK(c->head_size % 8 == 0 && c->head_size <= 128, ORT_CUDA_ERR_UNSUPPORTED,
+             "paged KV cache: head sizes are multiples of 8 up to 128");
+  ORTC_CHECK(c->num_pages <= INT_MAX && c->page_size <= INT_MAX && c->max_pages <= INT_MAX &&
+                 c->batch < INT_MAX && num_tokens <= INT_MAX / 2 &&
+                 (int64_t)c->kv_num_heads * c->head_size <= INT_MAX / c->page_size &&
+                 c->max_pages <= (int64_t)(INT_MAX / 2) / c->page_size,
+             ORT_CUDA_ERR_INVALID_ARG, "paged KV cache: sizes too large");
+  if (num_tokens == 0 || c->batch == 0) return ORT_CUDA_OK;
+  ORTC_CHECK(c->key && c->value && c->block_table && c->cu_seqlens && c->past_lens,
+             ORT_CUDA_ERR_INVALID_ARG, "NULL argument");
+  ORTC_CHECK(((uintptr_t)c->key & 15) == 0 && ((uintptr_t)c->value & 15) == 0,
+             ORT_CUDA_ERR_INVALID_ARG, "paged KV cache: key and value must be 16-byte aligned");
+  v->key = c->key, v->value = c->value;
+  v->table = c->block_table, v->cu = c->cu_seqlens, v->past = c->past_lens;
+  v->kv_heads = c->kv_num_heads, v->D = (int)c->head_size, v->type = c->type;
+  v->row_elems = v->kv_heads * v->D;
+  v->page_elems = c->page_size * v->row_elems;
+  v->num_pages = (int)c->num_pages, v->page_size = (int)c->page_size;
+  v->max_pages = (int)c->max_pages, v->batch = (int)c->batch;
+  v->num_tokens = (int)num_tokens;
+  v->err = s->err_dev;
+  return ORT_CUDA_OK;
+}
+
+}  // namespace
+}  // namespace ortc
+
+using namespace ortc;
+
+extern "C" {
+
+ORT_CUDA_API int ort_cuda_paged_kv_append(ort_cuda_session* s, const ort_cuda_paged_cache* cache,
+                                          const float* Q, int64_t q_stride, const float* K,
+                                          int64_t k_stride, const float* V, int64_t v_stride,
+                                          int64_t num_tokens, int num_heads,
+                                          const float* cos_cache, const float* sin_cache,
+                                          int64_t rotary_half, int64_t max_pos, float* Q_out,
+                                          int flags) try {
+  AppendArgs a;
+  int rc = paged_view(s, cache, num_tokens, flags, &a.c);
+  if (rc) return rc;
+  const int64_t D = cache->head_size, row = cache->kv_num_heads * D;
+  ORTC_CHECK((Q == nullptr) == (Q_out == nullptr), ORT_CUDA_ERR_INVALID_ARG,
+             "paged append: give both Q and Q_out or neither");
+  ORTC_CHECK(!Q || (num_heads >= 1 && num_heads % cache->kv_num_heads == 0 &&
+                    num_heads <= INT_MAX / D && q_stride >= num_heads * D),
+             ORT_CUDA_ERR_INVALID_ARG,
+             "paged append: need num_heads a multiple of kv_num_heads and q_stride >= its row");
+  ORTC_CHECK(Q != Q_out || !Q || q_stride == num_heads * D, ORT_CUDA_ERR_INVALID_ARG,
+             "paged append: Q_out may be Q only when Q is contiguous");
+  ORTC_CHECK(k_stride >= row && v_stride >= row, ORT_CUDA_ERR_INVALID_ARG,
+             "paged append: k_stride and v_stride must be at least a row");
+  ORTC_CHECK((cos_cache == nullptr) == (sin_cache == nullptr), ORT_CUDA_ERR_INVALID_ARG,
+             "paged append: give both cos and sin caches or neither");
+  ORTC_CHECK(!cos_cache || (rotary_half >= 1 && 2 * rotary_half <= D && max_pos >= 1),
+             ORT_CUDA_ERR_INVALID_ARG,
+             "paged append: rotary needs cos/sin caches of rotary_half <= head_size / 2 values");
+  if (num_tokens == 0 || cache->batch == 0) return ORT_CUDA_OK;
+  ORTC_CHECK(K && V, ORT_CUDA_ERR_INVALID_ARG, "NULL argument");
+  a.q = Q, a.q_out = Q_out, a.q_stride = q_stride, a.heads = Q ? num_heads : 0;
+  a.k = K, a.k_stride = k_stride, a.v = V, a.v_stride = v_stride;
+  if (cos_cache) {
+    a.cos = cos_cache, a.sin = sin_cache, a.half = (int)rotary_half, a.max_pos = max_pos;
+    a.interleaved = (flags & ORT_CUDA_ROTARY_INTERLEAVED) ? 1 : 0;
+  }
+  DeviceGuard guard(s->device);
+  OpTimer timer(s, "PagedKVAppend");
+  return launch_append(a, s->stream, &s->launches);
+} catch (const std::exception& e) {
+  return fail(ORT_CUDA_ERR_OOM, std::string("paged append: ") + e.what());
+}
+
+ORT_CUDA_API int ort_cuda_paged_attention(ort_cuda_session* s, const ort_cuda_paged_cache* cache,
+                                          const float* Q, int64_t q_stride, int64_t num_tokens,
+                                          int64_t max_seq, int num_heads, double scale,
+                                          double softcap, int64_t window, int64_t shared_len,
+                                          float* out, int flags) try {
+  PagedAttnArgs a;
+  int rc = paged_view(s, cache, num_tokens, flags, &a.c);
+  if (rc) return rc;
+  const int64_t D = cache->head_size;
+  ORTC_CHECK(num_heads >= 1 && num_heads % cache->kv_num_heads == 0 && num_heads <= INT_MAX / D &&
+                 q_stride >= num_heads * D,
+             ORT_CUDA_ERR_INVALID_ARG,
+             "paged attention: need num_heads a multiple of kv_num_heads and q_stride >= its row");
+  ORTC_CHECK(max_seq >= 0 && shared_len >= 0, ORT_CUDA_ERR_INVALID_ARG,
+             "paged attention: need max_seq, shared_len >= 0");
+  ORTC_CHECK(shared_len <= cache->max_pages * cache->page_size, ORT_CUDA_ERR_INVALID_ARG,
+             "paged attention: shared_len exceeds max_pages * page_size");
+  ORTC_CHECK(std::isfinite(scale) && std::isfinite(softcap), ORT_CUDA_ERR_INVALID_ARG,
+             "paged attention: scale and softcap must be finite");
+  if (num_tokens == 0 || cache->batch == 0) return ORT_CUDA_OK;
+  ORTC_CHECK(Q && out, ORT_CUDA_ERR_INVALID_ARG, "NULL argument");
+  ORTC_CHECK(num_tokens * num_heads <= INT_MAX, ORT_CUDA_ERR_INVALID_ARG,
+             "paged attention: sizes too large");
+  a.q = Q, a.q_stride = q_stride, a.out = out;
+  a.heads = num_heads, a.group = num_heads / cache->kv_num_heads;
+  a.max_seq = (int)std::min<int64_t>(max_seq, num_tokens);
+  a.shared = (int)shared_len;
+  a.window = window > 0 && window < INT_MAX ? (int)window : 0;
+  a.scale = (float)(scale > 0 ? scale : 1.0 / std::sqrt((double)D));
+  a.softcap = softcap > 0 ? (float)softcap : 0.0f;
+  DeviceGuard guard(s->device);
+  OpTimer timer(s, "PagedAttention");
+  void* scratch = nullptr;
+  rc = paged_scratch(s, paged_attention_scratch(a, s->sm_count), &scratch);
+  if (rc) return rc;
+  return launch_paged_attention(a, scratch, s->sm_count, s->stream, &s->launches);
+} catch (const std::exception& e) {
+  return fail(ORT_CUDA_ERR_OOM, std::string("paged attention: ") + e.what());
+}
+
+}  // extern "C"

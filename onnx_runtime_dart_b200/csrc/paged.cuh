@@ -1,0 +1,84 @@
+// Internal declarations of the paged KV cache (csrc/paged.cu: entry points,
+// workspaces, append; csrc/paged_attn.cu: attention).
+#pragma once
+
+#include "common.cuh"
+#include "ptx.cuh"
+
+namespace ortc {
+
+// The cache and the batch of one call, as the kernels see them.
+struct PagedView {
+  void* key = nullptr;
+  void* value = nullptr;
+  const int32_t* table = nullptr;
+  const int32_t* cu = nullptr;
+  const int32_t* past = nullptr;
+  int64_t page_elems = 0;  // elements of a page: page_size * kv_heads * D
+  int row_elems = 0;       // elements of a token's row: kv_heads * D
+  int num_pages = 0, page_size = 0, max_pages = 0, batch = 0;
+  int kv_heads = 0, D = 0, type = 0;
+  int num_tokens = 0;
+  int* err = nullptr;  // host-mapped error word
+};
+
+// Sequence b of a call: its first token, its token count and its past; no
+// tokens when its lengths do not fit (see fits).
+struct PagedSeq {
+  int row0, count, past;
+};
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedView& v, int b, int max_seq, int shared) {
+  const int c0 = v.cu[b], c1 = v.cu[b + 1], past = v.past[b];
+  PagedSeq s = {c0, c1 - c0, past};
+  if (c0 >= 0 && c1 == c0) {  // no tokens: nothing to check
+    s.count = 0;
+    return s;
+  }
+  const bool fits = c0 >= 0 && c0 < c1 && (b == 0 || c0 >= v.cu[b - 1]) && c1 <= v.num_tokens && c1 - c0 <= max_seq && past >= 0 &&
+                    past >= shared &&
+                    (int64_t)past + (c1 - c0) <= (int64_t)v.max_pages * v.page_size;
+  if (!fits) {
+    record_error(v.err, KERR_PAGED_LENGTH);
+    s.count = 0;
+  }
+  return s;
+}
+
+// The sequence that token t belongs to: the first that ends behind t, `batch`
+// when there is none.  Whole warp; the lengths of 32 sequences a step.
+__device__ __forceinline__ int paged_find(const PagedView& v, int t) {
+  const int lane = threadIdx.x & 31;
+  for (int b0 = 0; b0 < v.batch; b0 += 32) {
+    const unsigned m = __ballot_sync(0xffffffffu, b0 + lane < v.batch && v.cu[b0 + lane + 1] > t);
+    if (m) return b0 + __ffs(m) - 1;
+  }
+  return v.batch;
+}
+
+// Offset in elements of position `pos` of sequence b (KV head 0) in the key
+// and value pages, -1 when its page is outside the cache.
+__device__ __forceinline__ int64_t paged_row(const PagedView& v, int b, int pos) {
+  const int pg = pos / v.page_size;
+  const int page = __ldg(v.table + (int64_t)b * v.max_pages + pg);
+  if (page < 0 || page >= v.num_pages) {
+    record_error(v.err, KERR_PAGED_PAGE);
+    return -1;
+  }
+  return page * v.page_elems + (int64_t)(pos - pg * v.page_size) * v.row_elems;
+}
+
+struct PagedAttnArgs {
+  PagedView c;
+  const float* q = nullptr;
+  int64_t q_stride = 0;
+  float* out = nullptr;
+  int heads = 0, group = 1, max_seq = 0, shared = 0;
+  int window = 0;  // 0: no window
+  float scale = 1.0f, softcap = 0.0f;
+};
+size_t paged_attention_scratch(const PagedAttnArgs& a, int sm_count);
+int launch_paged_attention(const PagedAttnArgs& a, void* scratch, int sm_count, cudaStream_t st,
+                           int64_t* launches);
+
+}  // namespace ortc

@@ -15,6 +15,10 @@ enum KernelError : int {
   KERR_WAIT_MMA = 3,    // tensor-core commit never arrived
   KERR_WAIT_DRAIN = 4,  // in-flight copies did not land before exit
   KERR_WAIT_PEER = 5,   // a peer GPU's ready flag did not arrive
+  // device-side lengths and pages that do not fit (csrc/paged.cu)
+  KERR_PAGED_LENGTH = 16,
+  KERR_PAGED_PAGE = 17,
+  KERR_PAGED_POSITION = 18,
 };
 
 // Upper bound of any single wait (ns of %globaltimer).  Every legitimate

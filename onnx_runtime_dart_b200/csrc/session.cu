@@ -23,6 +23,7 @@
 
 #include "common.cuh"
 #include "nccl_dl.cuh"
+#include "ptx.cuh"
 
 namespace ortc {
 
@@ -104,19 +105,6 @@ int ensure_kscratch(ort_cuda_session* s, size_t bytes) {
 
 namespace {
 
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    cudaGetDevice(&prev);
-    if (prev != dev) cudaSetDevice(dev);
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    cudaGetDevice(&cur);
-    if (prev >= 0 && cur != prev) cudaSetDevice(prev);
-  }
-};
-
 bool is_pinned_host(const void* p) {
   cudaPointerAttributes at;
   if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
@@ -184,6 +172,20 @@ int check_kernel_error(ort_cuda_session* s) {
   if (!e || *e == 0) return ORT_CUDA_OK;
   const int code = *e;
   *e = 0;
+  switch (code) {
+    case KERR_PAGED_LENGTH:
+      return fail(ORT_CUDA_ERR_INVALID_ARG,
+                  "paged KV cache: cu_seqlens and past_lens do not fit num_tokens, max_seq, "
+                  "shared_len or max_pages * page_size; the sequence was left out");
+    case KERR_PAGED_PAGE:
+      return fail(ORT_CUDA_ERR_INVALID_ARG,
+                  "paged KV cache: block_table names a page outside [0, num_pages); its tokens "
+                  "were left out");
+    case KERR_PAGED_POSITION:
+      return fail(ORT_CUDA_ERR_INVALID_ARG,
+                  "paged KV cache: a position is outside the cos/sin caches; its token was left "
+                  "out");
+  }
   return fail(ORT_CUDA_ERR_TIMEOUT,
               "a kernel wait exceeded its bound (code " + std::to_string(code) +
                   "); the kernel stopped and returned");
@@ -444,6 +446,7 @@ ORT_CUDA_API int ort_cuda_close(ort_cuda_session* s) {
   if (s->argscratch) cudaFree(s->argscratch);
   if (s->dqscratch) cudaFree(s->dqscratch);
   if (s->attnscratch) cudaFree(s->attnscratch);
+  paged_free(s);
   if (s->pinned) cudaFreeHost(s->pinned);
   if (s->err_host) cudaFreeHost(s->err_host);
   for (auto& kv : s->graphs) cudaGraphExecDestroy(kv.second.exec);

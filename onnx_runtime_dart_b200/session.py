@@ -83,6 +83,69 @@ class DeviceTensor:
 Tensorish = Union[np.ndarray, DeviceTensor]
 
 
+class PagedKVCache:
+    """A paged KV cache and the batch that a call works on (ort_cuda_paged_cache):
+    torch CUDA tensors ``key`` / ``value`` [num_pages, page_size, kv_heads,
+    head] (float32, float16 or bfloat16), and int32 ``block_table`` [batch,
+    max_pages], ``cu_seqlens`` [batch + 1], ``past_lens`` [batch].  The tensors
+    are used in place and read when the kernels run: a serving loop writes new
+    lengths and pages into them and keeps the object."""
+
+    def __init__(self, key, value, block_table, cu_seqlens, past_lens):
+        import torch
+        types = {torch.float32: _lib.CACHE_F32, torch.float16: _lib.CACHE_F16,
+                 torch.bfloat16: _lib.CACHE_BF16}
+        for name, t in (("key", key), ("value", value), ("block_table", block_table),
+                        ("cu_seqlens", cu_seqlens), ("past_lens", past_lens)):
+            if not isinstance(t, torch.Tensor) or not t.is_cuda or not t.is_contiguous():
+                raise ValueError(f"PagedKVCache: {name} must be a contiguous CUDA tensor")
+            if t.device != key.device:
+                raise ValueError(f"PagedKVCache: {name} is on {t.device}, key on {key.device}")
+        if key.dtype not in types:
+            raise UnsupportedError(f"PagedKVCache: pages of type {key.dtype}")
+        if key.ndim != 4 or value.shape != key.shape or value.dtype != key.dtype:
+            raise ValueError("PagedKVCache: key and value must be [num_pages, page_size, "
+                             "kv_heads, head] of one type")
+        for name, t in (("block_table", block_table), ("cu_seqlens", cu_seqlens),
+                        ("past_lens", past_lens)):
+            if t.dtype != torch.int32:
+                raise ValueError(f"PagedKVCache: {name} must be int32")
+        batch = int(past_lens.shape[0]) if past_lens.ndim == 1 else -1
+        if batch < 0 or tuple(cu_seqlens.shape) != (batch + 1,) or block_table.ndim != 2 or \
+                int(block_table.shape[0]) != batch:
+            raise ValueError("PagedKVCache: need block_table [batch, max_pages], cu_seqlens "
+                             "[batch + 1] and past_lens [batch]")
+        self.key, self.value = key, value
+        self.block_table, self.cu_seqlens, self.past_lens = block_table, cu_seqlens, past_lens
+        self.batch, self.device = batch, key.device
+        self.kv_heads, self.head_size = int(key.shape[2]), int(key.shape[3])
+        self.struct = _lib.PagedCacheStruct(
+            key.data_ptr(), value.data_ptr(), block_table.data_ptr(), cu_seqlens.data_ptr(),
+            past_lens.data_ptr(), key.shape[0], key.shape[1], block_table.shape[1], batch,
+            self.head_size, self.kv_heads, types[key.dtype])
+        self.ref = ctypes.addressof(self.struct)
+
+    def rows(self, name: str, x, width: int):
+        """(tensor, row stride) of a float32 activation of `width` features a
+        token: rows may lie apart (a slice of a fused projection's output),
+        anything else is made contiguous."""
+        if x.device != self.device or not x.is_floating_point():
+            raise ValueError(f"{name} must be a float tensor on {self.device}")
+        if x.ndim < 2 or x.numel() != x.shape[0] * width:
+            raise ValueError(f"{name} must be [tokens, {width}] (or [tokens, heads, "
+                             f"{self.head_size}]), got {tuple(x.shape)}")
+        if x.element_size() != 4:
+            x = x.float()
+        if x.is_contiguous():
+            return x, width
+        if x.ndim == 2 and x.stride(1) == 1 and x.stride(0) >= width:
+            return x, x.stride(0)
+        if x.ndim == 3 and x.stride(2) == 1 and x.stride(1) == x.shape[2] and \
+                x.stride(0) >= width:
+            return x, x.stride(0)
+        return x.contiguous(), width
+
+
 class CudaSession:
     """One GPU (or one rank of an N-sharded group) running the hot ops.
 
@@ -107,6 +170,7 @@ class CudaSession:
         # initializer name -> ("nbits" | "dense", K, N)
         self.weights: Dict[str, tuple] = {}
         self._explicit_stream = False  # set_stream() chose the launch stream
+        self._stream_ptr: Optional[int] = None
         self._followed: Optional[int] = None
 
     @staticmethod
@@ -138,6 +202,7 @@ class CudaSession:
         stream (torch's default stream), passed as cudaStreamLegacy; None
         restores the session's own stream."""
         self._explicit_stream = stream_ptr is not None
+        self._stream_ptr = stream_ptr
         self._followed = None
         self._set_stream_raw(stream_ptr)
 
@@ -156,7 +221,7 @@ class CudaSession:
         if self._explicit_stream:
             return
         import torch
-        cur = torch.cuda.current_stream().cuda_stream
+        cur = torch.cuda.current_stream(self.device).cuda_stream
         if cur != self._followed:
             self._set_stream_raw(cur)
             self._followed = cur
@@ -581,6 +646,100 @@ class CudaSession:
             "ort_cuda_group_query_attention")
         return out, pk, pv
 
+    # -- paged KV cache ------------------------------------------------------
+    def _paged_stream(self, cache: "PagedKVCache"):
+        """Where a paged call runs: on torch's current stream, or, after
+        set_stream(), with that stream current for torch too, so that what the
+        call allocates and converts belongs to it."""
+        import contextlib
+        import torch
+        if cache.device.index != self.device:
+            raise ValueError(f"PagedKVCache is on {cache.device}, the session on cuda:"
+                             f"{self.device}")
+        if not self._explicit_stream:
+            self._follow_torch_stream()
+            return contextlib.nullcontext()
+        if self._stream_ptr in (0, 1):
+            return torch.cuda.stream(torch.cuda.default_stream(cache.device))
+        return torch.cuda.stream(torch.cuda.ExternalStream(self._stream_ptr, cache.device))
+
+    @staticmethod
+    def _paged_out(name: str, out, like):
+        """The fp32 output of a paged call: `out` checked, or a new tensor."""
+        if out is None:
+            import torch
+            return torch.empty(like.shape, dtype=torch.float32, device=like.device)
+        if out.shape != like.shape or out.element_size() != 4 or not out.is_floating_point() or \
+                out.device != like.device or not out.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float32 tensor like the queries")
+        return out
+
+    def paged_kv_append(self, cache: "PagedKVCache", k, v, q=None, num_heads: int = 0,
+                        cos_cache=None, sin_cache=None, rotary_interleaved: bool = False,
+                        q_out=None):
+        """Appends the keys and values [tokens, kv_heads * head] of this call to
+        the paged cache (ort_cuda_paged_kv_append), with RoPE of the keys and of
+        the queries ``q`` when cos/sin caches are given.  Returns the rotated
+        queries (``q_out``, which may be ``q`` itself), or None without ``q``."""
+        width = cache.kv_heads * cache.head_size
+        with self._paged_stream(cache):
+            k, ks = cache.rows("k", k, width)
+            v, vs = cache.rows("v", v, width)
+            n = int(k.shape[0])
+            if int(v.shape[0]) != n or (q is not None and int(q.shape[0]) != n):
+                raise ValueError("paged_kv_append: q, k and v need the same number of tokens")
+            qp = qs = op = 0
+            if q is not None:
+                rows, qs = cache.rows("q", q, num_heads * cache.head_size)
+                if q_out is q and rows is not q:
+                    raise ValueError("paged_kv_append: only contiguous float32 queries are "
+                                     "rotated in place")
+                q_out = self._paged_out("q_out", q_out, rows)
+                qp, op = rows.data_ptr(), q_out.data_ptr()
+            elif q_out is not None:
+                raise ValueError("paged_kv_append: q_out without q")
+            cp = sp = half = max_pos = 0
+            if (cos_cache is None) != (sin_cache is None):
+                raise ValueError("paged_kv_append: give both cos and sin caches or neither")
+            if cos_cache is not None:
+                for t in (cos_cache, sin_cache):
+                    if t.device != cache.device or t.element_size() != 4 or \
+                            not t.is_floating_point() or not t.is_contiguous() or t.ndim != 2 or \
+                            t.shape != cos_cache.shape:
+                        raise ValueError("paged_kv_append: cos/sin caches must be contiguous "
+                                         "float32 [max_pos, rotary_half] CUDA tensors")
+                cp, sp = cos_cache.data_ptr(), sin_cache.data_ptr()
+                max_pos, half = cos_cache.shape
+            rc = _lib.load().ort_cuda_paged_kv_append(
+                self.handle, cache.ref, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, n, num_heads,
+                cp, sp, half, max_pos, op, _lib.ROTARY_INTERLEAVED if rotary_interleaved else 0)
+        if rc:
+            check(rc, "ort_cuda_paged_kv_append")
+        return q_out
+
+    def paged_attention(self, cache: "PagedKVCache", q, num_heads: int, *,
+                        max_seq: Optional[int] = None, scale: Optional[float] = None,
+                        softcap: float = 0.0, local_window_size: int = -1, shared_len: int = 0,
+                        out=None):
+        """Attention of the queries [tokens, num_heads * head] over the paged
+        cache that already holds their keys (ort_cuda_paged_attention): causal,
+        optionally over the last ``local_window_size`` keys, scores optionally
+        capped by ``softcap * tanh(score / softcap)``.  ``max_seq`` bounds the
+        tokens of any one sequence (default: the tokens of the call);
+        ``shared_len``: that many first positions are the same in every
+        sequence and are read once, through the block table's first row."""
+        with self._paged_stream(cache):
+            q, qs = cache.rows("q", q, num_heads * cache.head_size)
+            out = self._paged_out("out", out, q)
+            n = int(q.shape[0])
+            rc = _lib.load().ort_cuda_paged_attention(
+                self.handle, cache.ref, q.data_ptr(), qs, n, n if max_seq is None else max_seq,
+                num_heads, 0.0 if scale is None else scale, softcap, local_window_size,
+                shared_len, out.data_ptr(), 0)
+        if rc:
+            check(rc, "ort_cuda_paged_attention")
+        return out
+
     def multi_head_attention(self, q, k, v, num_heads: int, scale=None, attention_bias=None):
         """MultiHeadAttention (opMultiHeadAttention, lib/src/onnx_ops.dart:
         1656-1725) over already-projected [batch, seq, hidden] Q/K/V."""
@@ -871,6 +1030,25 @@ class CudaSession:
                 rotary_interleaved=bool(attrs.get("rotary_interleaved", 0)),
                 cos_cache=opt(7), sin_cache=opt(8), past_key=opt(3), past_value=opt(4),
                 attention_bias=opt(10)))
+        if op == "PagedAttention":  # com.microsoft; no counterpart in the reference
+            names = ins + [""] * (10 - len(ins))
+            k, v, kc, vc, cu, past, table, cos, sin = (values[x] if x else None
+                                                       for x in names[1:10])
+            heads, kv = attrs["num_heads"], attrs["kv_num_heads"]
+            if k is None:  # q, k and v side by side
+                D = int(a.shape[-1]) // (heads + 2 * kv)
+                a, k, v = a.split([heads * D, kv * D, kv * D], dim=-1)
+            rotary = bool(attrs.get("do_rotary", 0))
+            cache = PagedKVCache(kc, vc, table, cu, past)
+            q = self.paged_kv_append(cache, k, v, q=a if rotary else None, num_heads=heads,
+                                     cos_cache=cos if rotary else None,
+                                     sin_cache=sin if rotary else None,
+                                     rotary_interleaved=bool(attrs.get("rotary_interleaved", 0)))
+            out = self.paged_attention(cache, q if rotary else a, heads,
+                                       scale=attrs.get("scale"),
+                                       softcap=attrs.get("softcap", 0.0),
+                                       local_window_size=attrs.get("local_window_size", -1))
+            return [out, kc, vc]
         if op == "MultiHeadAttention":  # onnx_graph.dart:994-1000
             bias = values.get(ins[5]) if len(ins) > 5 and ins[5] else None
             return [self.multi_head_attention(a, values[ins[1]], values[ins[2]],
@@ -945,5 +1123,5 @@ def op_matmul(a: np.ndarray, b: np.ndarray, mode: str = "exact") -> np.ndarray:
     return s.matmul_batched(a, b, flags=fl)
 
 
-__all__ = ["CudaSession", "DeviceTensor", "UnsupportedError", "StateError", "op_matmul_nbits",
+__all__ = ["CudaSession", "DeviceTensor", "PagedKVCache", "UnsupportedError", "StateError", "op_matmul_nbits",
            "op_gemm", "op_matmul", "default_session"]
