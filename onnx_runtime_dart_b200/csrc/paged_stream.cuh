@@ -1,0 +1,866 @@
+// Attention over the paged KV cache for few query rows per sequence and KV
+// head (decode steps, drafted tokens, a batch over a shared prefix): a stream
+// over the keys.
+//
+// One CTA per SM.  A segment is (sequence, tile of R query rows, KV head); its
+// keys are cut into tiles of 8 warps x KW keys, and the tiles of all segments,
+// in order, are cut into equal runs, one per CTA, whatever the
+// sequences' lengths are (read on the device; every CTA finds its run from a
+// scan over the batch).  Each warp owns KW keys of every tile with a ring of
+// its own in shared memory, filled by cp.async some tiles ahead, across
+// segment borders, and its own running maximum and sum (no CTA barrier inside
+// a segment); the warps' states are joined at a segment's end.  A segment that
+// lies in several CTAs' runs is joined by the last of them (a ticket), in run
+// order, so results do not depend on timing.
+//
+// The products run on mma.sync (rows as M = 16, so tcgen05's M = 128 would be
+// empty for the most part; the bound is the key stream).  They keep fp32
+// results from 16-bit operands by splitting the fp32 side, q and the softmax
+// weights p, into parts of the cache's type whose products are exact in fp32:
+// fp16 hi + lo (22 bits; q scaled by a power of two per row, p by 2^15, so
+// that the low part keeps its bits), bf16 hi + mid + lo (24 bits).  fp32 pages
+// take tf32 with both sides split in two (hi.hi + lo.hi + hi.lo).  Up to 8
+// rows, a row's hi and lo parts are rows r and r + 8 of one MMA, so the split
+// costs nothing.
+//
+// Operand layouts avoid shuffles and transposes: the feature order of q.k is
+// free, so a lane's 16-byte chunk of a key row serves as its B operand of two
+// MMAs; the score accumulator is, after exp2, the A operand of p.v; and a
+// lane's 16-byte chunks of the value rows 2c, 2c + 1, 2c + 8, 2c + 9 give,
+// with byte permutes, its B operand of eight MMAs.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "paged.cuh"
+
+namespace ortc {
+
+// floor(x / d) for 0 <= x < 2^31.
+struct FastDiv {
+  uint32_t mul = 0, shift = 0;  // mul 0: a power of two
+  __host__ void set(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) s++;
+    if ((1ull << s) == d) {
+      mul = 0, shift = s;
+    } else {  // ceil(2^(31 + s) / d) < 2^32: exact for 31-bit x
+      mul = (uint32_t)(((1ull << (31 + s)) + d - 1) / d);
+      shift = s - 1;
+    }
+  }
+  __device__ __forceinline__ int div(int x) const {
+    return mul ? (int)(__umulhi((uint32_t)x, mul) >> shift) : x >> shift;
+  }
+};
+
+struct StreamArgs {
+  PagedAttnArgs a;
+  FastDiv page_div;
+  int q_vec = 0;       // float4 loads of q rows
+  int prefix = 0;      // 1: rows of all tokens over keys [0, shared) of row 0's pages
+  int max_rows = 0;    // sequences with more query rows per KV head are not this kernel's
+  float t_scale = 0;   // scale (softcap: scale / softcap)
+  float t_mul = 0;     // log2(e) (softcap: softcap * log2(e))
+  unsigned* tickets = nullptr;  // one per CTA, zero between calls
+  float* part_ml = nullptr;     // [2 * grid][R][2]
+  float* part_o = nullptr;      // [2 * grid][R][DP]
+  // prefix results per (token, head): maximum and sum, unnormalised output
+  float* pre_ml = nullptr;
+  float* pre_o = nullptr;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1,
+                                          __half) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1,
+                                          __nv_bfloat16) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_1688(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t tf32_rna(float x) {
+  uint32_t y;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
+  return y;
+}
+
+// The parts of a pair of fp32 values in the cache's 16-bit type: PARTS words,
+// each rounded to nearest from what the ones before it left.
+template <typename T>
+struct Split;
+template <>
+struct Split<__half> {
+  static constexpr int PARTS = 2;
+  static __device__ __forceinline__ void pair(float x, float y, uint32_t (&w)[2]) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    w[0] = *reinterpret_cast<const uint32_t*>(&h);
+    w[1] = *reinterpret_cast<const uint32_t*>(&l);
+  }
+};
+template <>
+struct Split<__nv_bfloat16> {
+  static constexpr int PARTS = 3;
+  static __device__ __forceinline__ void pair(float x, float y, uint32_t (&w)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+      const float2 f = __bfloat1622float2(h);
+      x -= f.x, y -= f.y;
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+};
+template <>
+struct Split<float> {
+  static constexpr int PARTS = 2;
+  static __device__ __forceinline__ void one(float x, uint32_t (&w)[2]) {
+    w[0] = tf32_rna(x);
+    w[1] = tf32_rna(x - __uint_as_float(w[0]));
+  }
+};
+
+template <typename T, int DP, int R>
+struct StreamCfg {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int KW = F32 ? 8 : 16;           // keys of a warp per tile
+  static constexpr int TK = 8 * KW;                 // keys of a tile
+  static constexpr int CHP = DP * (int)sizeof(T) / 16;  // 16-byte chunks of a padded row
+  static constexpr int ROWB = DP * (int)sizeof(T);
+  static constexpr int WSTAGE = 2 * KW * ROWB;      // a warp's stage: K rows, V rows
+  static constexpr int NS = 3 * 8192 / WSTAGE;      // 24 KB of ring per warp
+  static constexpr int KS = F32 ? DP / 8 : DP / 16; // k-steps of q.k
+  // q operands: R = 8 packs two parts into the 16 rows of an MMA
+  static constexpr int QP = R == 8 ? (Split<T>::PARTS + 1) / 2 : Split<T>::PARTS;
+  static constexpr int QB = QP * KS * 512;
+  static constexpr int RING = 8 * NS * WSTAGE;
+  static constexpr int JOIN = 8 * 8 * 64 * 4;       // [warp][8 rows][64 features]
+  static constexpr int SMEM = RING + QB + JOIN + 8 * R * 8;  // + (max, sum) per warp and row
+};
+
+// Where a CTA is in the list of tiles: tile `tile` of segment (b, rt, g).
+struct StreamPos {
+  int b, rt, g, tile;
+  int row0, count, past;    // the sequence
+  int lo, hi, nt, nrt;      // its keys, key tiles and row tiles
+};
+
+// Sets the sequence of `s` and returns its tiles per KV head and row tile
+// times its row tiles (0: nothing for this kernel).
+template <int R, int TK>
+__device__ __forceinline__ int stream_seq(const StreamArgs& p, StreamPos& s, int b, int min_past) {
+  const PagedAttnArgs& a = p.a;
+  s.b = b;
+  if (p.prefix) {
+    s.row0 = 0, s.past = 0;
+    s.count = max(0, min(a.c.cu[a.c.batch], a.c.num_tokens));
+    s.lo = a.window ? min(a.shared, max(0, min_past + 1 - a.window)) : 0;
+    s.hi = a.shared;
+  } else {
+    const PagedSeq q = paged_seq(a.c, b, a.max_seq, a.shared);
+    s.row0 = q.row0, s.count = q.count, s.past = q.past;
+    s.lo = max(a.shared, a.window ? q.past + 1 - a.window : 0);
+    s.hi = q.past + q.count;
+  }
+  const int64_t rows = (int64_t)s.count * a.group;
+  if (rows == 0 || (!p.prefix && rows > p.max_rows)) {
+    s.count = 0;
+    s.nt = s.nrt = 0;
+    return 0;
+  }
+  s.nrt = (int)((rows + R - 1) / R);
+  s.nt = max(1, (s.hi - s.lo + TK - 1) / TK);
+  return s.nt * s.nrt;
+}
+
+template <typename T, int DP, int R>
+__global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_constant__ StreamArgs p) {
+  using C = StreamCfg<T, DP, R>;
+  constexpr bool F32 = C::F32;
+  constexpr int KW = C::KW, TK = C::TK, CHP = C::CHP, NS = C::NS, KS = C::KS, PARTS = Split<T>::PARTS;
+  constexpr int NPASS = DP / 64;       // blocks of 64 features of the output
+  constexpr int NR = R / 8;            // rows a lane holds
+  extern __shared__ __align__(128) unsigned char smem[];
+  unsigned char* ring = smem;
+  uint4* qf = reinterpret_cast<uint4*>(smem + C::RING);  // [QP][KS][32]
+  float* join = reinterpret_cast<float*>(smem + C::RING + C::QB);
+  float2* wml = reinterpret_cast<float2*>(smem + C::RING + C::QB + C::JOIN);  // [8][R]
+  __shared__ long long s_scan[8];
+  __shared__ long long s_u0base;
+  __shared__ int s_b0, s_min[8], s_last;
+  __shared__ float s_fac[R];   // score factor of a row
+  __shared__ int s_pos[R];     // position of a row, INT_MIN: no row
+  __shared__ float2 s_ml[R];   // the segment's maximum and sum
+
+  const PagedAttnArgs& a = p.a;
+  const PagedView& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const int D = c.D, G = c.kv_heads, nb = p.prefix ? 1 : c.batch;
+
+  // ---- this CTA's run of tiles
+  int min_past = 0;
+  if (p.prefix && a.window) {
+    min_past = INT_MAX;
+    for (int b = tid; b < c.batch; b += 256)
+      if (c.cu[b + 1] > c.cu[b]) min_past = min(min_past, max(0, c.past[b]));
+    min_past = __reduce_min_sync(~0u, min_past);
+    if (lane == 0) s_min[w] = min_past;
+    __syncthreads();
+    for (int i = 0; i < 8; i++) min_past = min(min_past, s_min[i]);
+    if (min_past > INT_MAX / 2) min_past = INT_MAX / 2;
+  }
+  StreamPos cur;
+  long long total = 0, u0 = 0, u1 = 0;
+  int runs = 1;  // CTAs with work: one tile each at least
+  for (int pass = 0; pass < 2; pass++) {  // total, then the sequence of u0
+    long long base = 0;
+    for (int b0 = 0; b0 < nb; b0 += 256) {
+      StreamPos t;
+      const long long n =
+          b0 + tid < nb ? (long long)stream_seq<R, TK>(p, t, b0 + tid, min_past) * G : 0;
+      long long x = n;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(~0u, x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane == 31) s_scan[w] = x;
+      __syncthreads();
+      long long all = 0, before = 0;
+      for (int i = 0; i < 8; i++) {
+        if (i < w) before += s_scan[i];
+        all += s_scan[i];
+      }
+      if (pass == 1) {
+        const long long start = base + before + x - n;
+        if (n && start <= u0 && u0 < start + n) {
+          s_b0 = b0 + tid;
+          s_u0base = start;
+        }
+      }
+      base += all;
+      __syncthreads();
+      if (pass == 0 && nb <= 256) {  // one block of sequences: find u0 without a second scan
+        total = all;
+        runs = (int)min((long long)gridDim.x, max(total, 1ll));
+        u0 = total * blockIdx.x / runs;
+        const long long start = before + x - n;
+        if (n && start <= u0 && u0 < start + n) {
+          s_b0 = tid;
+          s_u0base = start;
+        }
+      }
+    }
+    if (pass == 0) {
+      total = base;
+      runs = (int)min((long long)gridDim.x, max(total, 1ll));
+      u0 = total * blockIdx.x / runs;
+      u1 = total * (blockIdx.x + 1) / runs;
+      if (nb <= 256) break;
+    }
+  }
+  __syncthreads();
+  if ((int)blockIdx.x >= runs || u0 >= u1) return;
+  stream_seq<R, TK>(p, cur, s_b0, min_past);
+  long long seq_u = s_u0base;  // first tile of cur.b
+  {
+    const int off = (int)(u0 - seq_u);
+    cur.tile = off % cur.nt;
+    const int sg = off / cur.nt;
+    cur.g = sg % G;
+    cur.rt = sg / G;
+  }
+
+  // ---- loads
+  unsigned char* wring = ring + w * NS * C::WSTAGE;
+  const uint32_t wring_s = smem_u32(wring);
+  const int chunks = D * (int)sizeof(T) / 16;
+  StreamPos ld = cur;      // the tile to load next
+  long long lu = u0;
+  int ld_stage = 0;
+  unsigned valid_q[NS];    // per stage: bit r set when key r of the warp is there
+#pragma unroll
+  for (int i = 0; i < NS; i++) valid_q[i] = 0;
+  auto advance = [&](StreamPos& s) {
+    if (++s.tile < s.nt) return;
+    s.tile = 0;
+    if (++s.g < G) return;
+    s.g = 0;
+    if (++s.rt < s.nrt) return;
+    s.rt = 0;
+    for (int b = s.b + 1; b < nb; b++)
+      if (stream_seq<R, TK>(p, s, b, min_past)) return;
+  };
+  // the page of lane r's key (r < KW) of a tile, and whether it has one
+  auto page_of = [&](const StreamPos& s, int& slot) {
+    const int j = s.lo + s.tile * TK + w * KW + (lane & (KW - 1));
+    slot = 0;
+    if (j >= s.hi) return -1;
+    const int pg = p.page_div.div(j);
+    slot = j - pg * c.page_size;
+    return __ldg(c.table + (int64_t)(p.prefix ? 0 : s.b) * c.max_pages + pg);
+  };
+  int nslot = 0, npage = page_of(ld, nslot);  // of tile lu
+  auto issue = [&](unsigned& valid) {  // loads tile lu; fetches the page of the next one
+    const int page = npage, slot = nslot, g = ld.g;
+    const bool there = ld.lo + ld.tile * TK + w * KW + (lane & (KW - 1)) < ld.hi;
+    if (there && (page < 0 || page >= c.num_pages)) record_error(c.err, KERR_PAGED_PAGE);
+    const bool ok = there && page >= 0 && page < c.num_pages;
+    const long long off =
+        ok ? (long long)page * c.page_elems + (long long)slot * c.row_elems + (long long)g * D : -1;
+    valid = __ballot_sync(~0u, ok) & ((1u << KW) - 1);
+    if (++lu < u1) {
+      advance(ld);
+      npage = page_of(ld, nslot);
+    }
+    const uint32_t st = wring_s + ld_stage * C::WSTAGE;
+    constexpr int RPI = CHP >= 32 ? 1 : 32 / CHP;  // rows per instruction
+    const int ch = lane & (CHP - 1);
+#pragma unroll
+    for (int i = 0; i < KW / RPI; i++) {
+      const int r = i * RPI + lane / CHP;
+      const long long o = __shfl_sync(~0u, off, r);
+      const int bytes = o >= 0 && ch < chunks ? 16 : 0;
+      const long long e = bytes ? o + ch * (16 / (int)sizeof(T)) : 0;
+      cp16(st + r * C::ROWB + ((ch ^ ((r & 1) << 2)) << 4), static_cast<const T*>(c.key) + e, bytes);
+      cp16(st + KW * C::ROWB + r * C::ROWB + ((ch ^ (((r >> 1) & 3) << 1)) << 4),
+           static_cast<const T*>(c.value) + e, bytes);
+    }
+    if (++ld_stage == NS) ld_stage = 0;
+  };
+  auto commit = [] { asm volatile("cp.async.commit_group;\n" ::: "memory"); };
+#pragma unroll
+  for (int i = 0; i < NS - 1; i++) {
+    if (lu < u1) issue(valid_q[i]);
+    commit();
+  }
+
+  // ---- segments
+  int stage = 0;
+  for (long long u = u0; u < u1;) {
+    const int n = (int)min((long long)(cur.nt - cur.tile), u1 - u);  // tiles of this segment here
+    // q rows: warp w builds rows w, w + 8 of the A operands
+    __syncthreads();  // the last segment's operands are no longer read
+#pragma unroll
+    for (int rr = 0; rr < NR; rr++) {
+      const int r = w + 8 * rr;
+      const int idx = cur.rt * R + r;
+      const bool row = idx < cur.count * a.group;
+      const int tok = row ? idx / a.group : 0, h = cur.g * a.group + (row ? idx - tok * a.group : 0);
+      int pos = INT_MIN;
+      if (row) {
+        pos = cur.past + tok;
+        if (p.prefix) {
+          pos = INT_MAX / 2;  // past the prefix
+          if (a.window) {
+            const int b = paged_find(c, tok);
+            pos = b < c.batch ? c.past[b] + tok - c.cu[b] : INT_MAX / 2;
+          }
+        }
+      }
+      float x[DP / 32];
+      const float* src = a.q + (int64_t)(cur.row0 + tok) * a.q_stride + (int64_t)h * D;
+      constexpr int E = DP / 32;  // features of a lane, E at a time
+#pragma unroll
+      for (int e = 0; e < E; e++) x[e] = 0.f;
+      if (row) {
+        if (E == 4 && p.q_vec && 4 * lane + 3 < D) {
+          *reinterpret_cast<float4*>(x) = __ldg(reinterpret_cast<const float4*>(src) + lane);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; e++)
+            if (E * lane + e < D) x[e] = __ldg(src + E * lane + e);
+        }
+      }
+      float fac = p.t_scale;
+      if constexpr (!F32 && PARTS == 2) {  // fp16: the row's largest value into [2^13, 2^14)
+        float mx = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; e++) mx = fmaxf(mx, fabsf(x[e]));
+        mx = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(mx)));
+        int ex = (int)(__float_as_uint(mx) >> 23) - 127;
+        ex = max(-100, min(ex, 126));
+        const float up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
+#pragma unroll
+        for (int e = 0; e < E; e++) x[e] *= up;
+        fac *= __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
+      }
+      if (lane == 0) {
+        s_fac[r] = fac;
+        s_pos[r] = pos;
+      }
+      uint32_t* qw = reinterpret_cast<uint32_t*>(qf);
+      // word `reg` of k-step s of part pt for MMA lane ml
+      auto put = [&](int pt, int s, int ml, int reg, uint32_t v) {
+        qw[(((pt * KS + s) * 32) + ml) * 4 + reg] = v;
+      };
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const int d = E * lane + e;
+        if constexpr (F32) {  // chunk of 4: features 0, 1 in k-step 2i, 2, 3 in 2i + 1
+          const int ch = d >> 2, s = 2 * (ch >> 2) + ((d >> 1) & 1), ml = (r & 7) * 4 + (ch & 3);
+          uint32_t w0[2], w1[2];
+          Split<float>::one(x[e], w0);
+          Split<float>::one(x[e + 1], w1);
+#pragma unroll
+          for (int pt = 0; pt < 2; pt++) {
+            const int reg = R == 8 ? pt : rr, part = R == 8 ? 0 : pt;
+            put(part, s, ml, reg, w0[pt]);
+            put(part, s, ml, reg + 2, w1[pt]);
+          }
+        } else {  // chunk of 8: features 0..3 in k-step 2i, 4..7 in 2i + 1
+          const int ch = d >> 3, s = 2 * (ch >> 2) + ((d >> 2) & 1), ml = (r & 7) * 4 + (ch & 3);
+          const int hi2 = ((d >> 1) & 1) * 2;
+          uint32_t wd[PARTS];
+          Split<T>::pair(x[e], x[e + 1], wd);
+#pragma unroll
+          for (int pt = 0; pt < PARTS; pt++) {
+            if (R == 8)
+              put(pt >> 1, s, ml, (pt & 1) + hi2, wd[pt]);
+            else
+              put(pt, s, ml, rr + hi2, wd[pt]);
+          }
+          if (R == 8 && PARTS == 3) put(1, s, ml, 1 + hi2, 0u);
+        }
+      }
+    }
+    __syncthreads();
+    float fac[NR];
+    int pos[NR];
+    int pos_lo = INT_MAX, pos_hi = INT_MIN;  // over the tile's rows
+#pragma unroll
+    for (int rr = 0; rr < NR; rr++) {
+      fac[rr] = s_fac[(lane >> 2) + 8 * rr];
+      pos[rr] = s_pos[(lane >> 2) + 8 * rr];
+      if (pos[rr] != INT_MIN) {
+        pos_lo = min(pos_lo, pos[rr]);
+        pos_hi = max(pos_hi, pos[rr]);
+      }
+    }
+    pos_lo = __reduce_min_sync(~0u, pos_lo);
+    pos_hi = __reduce_max_sync(~0u, pos_hi);
+
+    float m[NR], l[NR], o[NPASS][8][4];
+#pragma unroll
+    for (int rr = 0; rr < NR; rr++) m[rr] = -INFINITY, l[rr] = 0.f;
+#pragma unroll
+    for (int x = 0; x < NPASS; x++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
+
+    for (int i = 0; i < n; i++, u++) {
+      // the tile NS - 1 ahead into the stage that was read last
+      __syncwarp();
+      unsigned next_valid = 0;
+      if (lu < u1) issue(next_valid);
+      commit();
+      asm volatile("cp.async.wait_group %0;\n" ::"n"(NS - 1) : "memory");
+      __syncwarp();
+      const unsigned valid = valid_q[0];
+#pragma unroll
+      for (int x = 0; x + 1 < NS - 1; x++) valid_q[x] = valid_q[x + 1];
+      valid_q[NS - 2] = next_valid;
+      const unsigned char* kt = wring + stage * C::WSTAGE;
+      const unsigned char* vt = kt + KW * C::ROWB;
+      if (++stage == NS) stage = 0;
+      const int base = cur.lo + (cur.tile + i) * TK + w * KW;
+      if (valid == 0) continue;
+
+      // scores
+      constexpr int NT = KW / 8;
+      float s[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+      const int row = lane >> 2, cl = lane & 3;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks += 2) {
+        const int ch = cl + 4 * (ks >> 1);
+        uint4 kv[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+          kv[t] = *reinterpret_cast<const uint4*>(kt + (row + 8 * t) * C::ROWB +
+                                                  ((ch ^ ((row & 1) << 2)) << 4));
+        if constexpr (F32) {
+          uint32_t kh[4], kl[4];
+          const float kx[4] = {__uint_as_float(kv[0].x), __uint_as_float(kv[0].y),
+                               __uint_as_float(kv[0].z), __uint_as_float(kv[0].w)};
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            uint32_t ww[2];
+            Split<float>::one(kx[e], ww);
+            kh[e] = ww[0], kl[e] = ww[1];
+          }
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const uint4 qa = qf[(ks + e) * 32 + lane];
+            mma_1688(s[0], qa, kh[2 * e], kh[2 * e + 1]);
+            mma_1688(s[0], qa, kl[2 * e], kl[2 * e + 1]);
+            if (R == 16) {
+              const uint4 ql = qf[(KS + ks + e) * 32 + lane];
+              mma_1688(s[0], ql, kh[2 * e], kh[2 * e + 1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int pt = 0; pt < C::QP; pt++) {
+            const uint4 q0 = qf[(pt * KS + ks) * 32 + lane], q1 = qf[(pt * KS + ks + 1) * 32 + lane];
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+              mma_16816(s[t], q0, kv[t].x, kv[t].y, T());
+              mma_16816(s[t], q1, kv[t].z, kv[t].w, T());
+            }
+          }
+        }
+      }
+
+      // softmax weights; rows (lane / 4) + 8 rr, keys base + 8 t + 2 cl + e
+      const bool full = valid == (1u << KW) - 1 && base + KW - 1 <= pos_lo &&
+                        (!a.window || base > pos_hi - a.window);
+      float pr[NR][NT][2];
+#pragma unroll
+      for (int rr = 0; rr < NR; rr++)
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float x = (R == 8 ? s[t][e] + s[t][e + 2] : s[t][2 * rr + e]) * fac[rr];
+            if (a.softcap > 0.f) x = tanhf(x);
+            pr[rr][t][e] = x * p.t_mul;
+          }
+      if (!full) {
+#pragma unroll
+        for (int rr = 0; rr < NR; rr++)
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const int k = 8 * t + 2 * cl + e, j = base + k;
+              if (!((valid >> k) & 1) || j > pos[rr] || (a.window && j <= pos[rr] - a.window))
+                pr[rr][t][e] = -INFINITY;
+            }
+      }
+      float corr[NR];
+#pragma unroll
+      for (int rr = 0; rr < NR; rr++) {
+        float mx = m[rr];
+#pragma unroll
+        for (int t = 0; t < NT; t++) mx = fmaxf(mx, fmaxf(pr[rr][t][0], pr[rr][t][1]));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+        const float mb = mx == -INFINITY ? 0.f : mx;
+        corr[rr] = ex2(m[rr] - mb);
+        m[rr] = mx;
+        // p scaled by 2^15 for fp16: its low part then keeps its bits
+        const float sub = PARTS == 2 && !F32 ? mb - 15.f : mb;
+        float sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            pr[rr][t][e] = ex2(pr[rr][t][e] - sub);
+            sum += pr[rr][t][e];
+          }
+        l[rr] = l[rr] * corr[rr] + sum;
+      }
+      if (__any_sync(~0u, corr[0] != 1.f || corr[NR - 1] != 1.f)) {
+#pragma unroll
+        for (int x = 0; x < NPASS; x++)
+#pragma unroll
+          for (int i2 = 0; i2 < 8; i2++) {
+            o[x][i2][0] *= corr[0], o[x][i2][1] *= corr[0];
+            o[x][i2][2] *= corr[NR - 1], o[x][i2][3] *= corr[NR - 1];
+          }
+      }
+
+      // A value that only some rows see must not reach the others as 0 * inf:
+      // such tiles (the border of the mask) are looked over, and one that holds
+      // an infinity or NaN is summed key by key.
+      bool odd = false;
+      if (!full) {
+#pragma unroll
+        for (int x = 0; x < KW * CHP / 32; x++) {
+          const uint4 v = reinterpret_cast<const uint4*>(vt)[x * 32 + lane];
+          const uint32_t ws[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            if constexpr (F32) {
+              odd |= (ws[e] & 0x7f800000u) == 0x7f800000u;
+            } else {
+              constexpr uint32_t inf = PARTS == 2 ? 0x7c00u : 0x7f80u;
+              odd |= (ws[e] & inf) == inf || ((ws[e] >> 16) & inf) == inf;
+            }
+          }
+        }
+        odd = __any_sync(~0u, odd);
+      }
+      if (odd) {
+        for (int k = 0; k < KW; k++) {
+          float pk[NR];
+#pragma unroll
+          for (int rr = 0; rr < NR; rr++) {
+            float mine = 0.f;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+              for (int e = 0; e < 2; e++)
+                if (k == 8 * t + 2 * cl + e) mine = pr[rr][t][e];
+            pk[rr] = __shfl_sync(~0u, mine, (lane & ~3) | ((k >> 1) & 3));
+          }
+          const T* vr = reinterpret_cast<const T*>(vt + k * C::ROWB);
+#pragma unroll
+          for (int x = 0; x < NPASS; x++)
+#pragma unroll
+            for (int i2 = 0; i2 < 8; i2++)
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                // feature of accumulator (x, i2, column 2 cl + e)
+                const int d = F32 ? x * 64 + (i2 >> 2) * 32 + (2 * cl + e) * 4 + (i2 & 3)
+                                  : x * 64 + (2 * cl + e) * 8 + i2;
+                constexpr int PC = 16 / (int)sizeof(T);
+                const int dd = ((d / PC) ^ (((k >> 1) & 3) << 1)) * PC + d % PC;
+                const float v = (float)vr[dd];
+#pragma unroll
+                for (int rr = 0; rr < NR; rr++)
+                  if (pk[rr] != 0.f) o[x][i2][2 * rr + e] = fmaf(pk[rr], v, o[x][i2][2 * rr + e]);
+              }
+        }
+        continue;
+      }
+
+      // o += p . v
+      if constexpr (F32) {
+        uint4 pa[2];
+        {
+          uint32_t w0[2], w1[2];
+          Split<float>::one(pr[0][0][0], w0);
+          Split<float>::one(pr[0][0][1], w1);
+          if (R == 8) {
+            pa[0] = make_uint4(w0[0], w0[1], w1[0], w1[1]);
+          } else {
+            uint32_t y0[2], y1[2];
+            Split<float>::one(pr[NR - 1][0][0], y0);
+            Split<float>::one(pr[NR - 1][0][1], y1);
+            pa[0] = make_uint4(w0[0], y0[0], w1[0], y1[0]);
+            pa[1] = make_uint4(w0[1], y0[1], w1[1], y1[1]);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < DP / 32; x++) {
+          const int ch = row + 8 * x;
+          const uint4 v0 = *reinterpret_cast<const uint4*>(vt + (2 * cl) * C::ROWB +
+                                                           ((ch ^ (cl << 1)) << 4));
+          const uint4 v1 = *reinterpret_cast<const uint4*>(vt + (2 * cl + 1) * C::ROWB +
+                                                           ((ch ^ (cl << 1)) << 4));
+          const uint32_t a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            uint32_t h0[2], h1[2];
+            Split<float>::one(__uint_as_float(a0[e]), h0);
+            Split<float>::one(__uint_as_float(a1[e]), h1);
+            float(&acc)[4] = o[x >> 1][(x & 1) * 4 + e];
+            mma_1688(acc, pa[0], h0[0], h1[0]);
+            mma_1688(acc, pa[0], h0[1], h1[1]);
+            if (R == 16) mma_1688(acc, pa[1], h0[0], h1[0]);
+          }
+        }
+      } else {
+        uint4 pa[C::QP];
+        {
+          uint32_t w0[PARTS], w1[PARTS];
+          Split<T>::pair(pr[0][0][0], pr[0][0][1], w0);
+          Split<T>::pair(pr[0][NT - 1][0], pr[0][NT - 1][1], w1);
+          if (R == 8) {
+            pa[0] = make_uint4(w0[0], w0[1], w1[0], w1[1]);
+            if (PARTS == 3) pa[C::QP - 1] = make_uint4(w0[PARTS - 1], 0u, w1[PARTS - 1], 0u);
+          } else {
+            uint32_t y0[PARTS], y1[PARTS];
+            Split<T>::pair(pr[NR - 1][0][0], pr[NR - 1][0][1], y0);
+            Split<T>::pair(pr[NR - 1][NT - 1][0], pr[NR - 1][NT - 1][1], y1);
+#pragma unroll
+            for (int pt = 0; pt < PARTS; pt++)
+              pa[pt < C::QP ? pt : 0] = make_uint4(w0[pt], y0[pt], w1[pt], y1[pt]);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < NPASS; x++) {
+          const int ch = row + 8 * x;
+          uint4 v[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int r = 2 * cl + (e & 1) + 8 * (e >> 1);
+            v[e] = *reinterpret_cast<const uint4*>(vt + r * C::ROWB + ((ch ^ (cl << 1)) << 4));
+          }
+          const uint32_t a0[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+          const uint32_t a1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+          const uint32_t a8[4] = {v[2].x, v[2].y, v[2].z, v[2].w};
+          const uint32_t a9[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
+            const uint32_t b0 = __byte_perm(a0[e >> 1], a1[e >> 1], sel);
+            const uint32_t b1 = __byte_perm(a8[e >> 1], a9[e >> 1], sel);
+#pragma unroll
+            for (int pt = 0; pt < C::QP; pt++) mma_16816(o[x][e], pa[pt], b0, b1, T());
+          }
+        }
+      }
+    }
+
+    // ---- the segment's end: join the warps
+    const int row = lane >> 2, cl = lane & 3;
+#pragma unroll
+    for (int rr = 0; rr < NR; rr++) {
+      l[rr] += __shfl_xor_sync(~0u, l[rr], 1);
+      l[rr] += __shfl_xor_sync(~0u, l[rr], 2);
+      if (cl == 0) wml[w * R + row + 8 * rr] = make_float2(m[rr], l[rr]);
+    }
+    const bool whole = n == cur.nt;
+    const long long seg_u = seq_u + (long long)(cur.rt * G + cur.g) * cur.nt;  // its first tile
+    const bool head = cur.tile != 0;  // begun in an earlier CTA
+    const int slot = 2 * blockIdx.x + (head ? 0 : 1);
+    // writes a row's value: final, or what the prefix pass hands on
+    auto finish = [&](int r, int d, float M, float L, float v) {
+      const int idx = cur.rt * R + r;
+      const int tok = idx / a.group, h = cur.g * a.group + idx - tok * a.group;
+      const int64_t at = (int64_t)(cur.row0 + tok) * a.heads + h;
+      if (p.prefix) {
+        p.pre_o[at * D + d] = v;
+        if (d == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * at) = make_float2(M, L);
+        return;
+      }
+      if (a.shared) {
+        const float2 pm = *reinterpret_cast<const float2*>(p.pre_ml + 2 * at);
+        const float mm = fmaxf(M, pm.x), mb = mm == -INFINITY ? 0.f : mm;
+        const float wa = ex2(M - mb), wb = ex2(pm.x - mb);
+        v = v * wa + p.pre_o[at * D + d] * wb;
+        L = L * wa + pm.y * wb;
+      }
+      a.out[at * D + d] = L == 0.f ? 0.f : v / L;
+    };
+    const int rows_here = min(R, cur.count * a.group - cur.rt * R);
+#pragma unroll
+    for (int x = 0; x < NPASS; x++)
+#pragma unroll
+      for (int rr = 0; rr < NR; rr++) {
+        float* dst = join + (w * 8 + row) * 64;
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+          for (int i2 = 0; i2 < 8; i2 += 4) {
+            float4 v;
+            float* vv = reinterpret_cast<float*>(&v);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              vv[k] = R == 8 ? o[x][i2 + k][e] + o[x][i2 + k][e + 2] : o[x][i2 + k][2 * rr + e];
+            const int d = F32 ? (i2 >> 2) * 32 + (2 * cl + e) * 4 : (2 * cl + e) * 8 + i2;
+            *reinterpret_cast<float4*>(dst + d) = v;
+          }
+        __syncthreads();
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+          const int e = tid + 256 * y, r8 = e >> 6, dd = e & 63, r = r8 + 8 * rr, d = x * 64 + dd;
+          float M = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 8; i++) M = fmaxf(M, wml[i * R + r].x);
+          const float mb = M == -INFINITY ? 0.f : M;
+          float L = 0.f, v = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const float2 q = wml[i * R + r];
+            const float f = ex2(q.x - mb);
+            L = fmaf(f, q.y, L);
+            v = fmaf(f, join[(i * 8 + r8) * 64 + dd], v);
+          }
+          if (r < rows_here && d < D) {
+            if (whole) {
+              finish(r, d, M, L, v);
+            } else {
+              p.part_o[((int64_t)slot * R + r) * DP + d] = v;
+              if (d == 0) {
+                p.part_ml[((int64_t)slot * R + r) * 2] = M;
+                p.part_ml[((int64_t)slot * R + r) * 2 + 1] = L;
+              }
+            }
+          }
+        }
+        __syncthreads();
+      }
+    if (!whole) {
+      // the runs that hold this segment: CTAs c0 .. c1
+      const int c0 = (int)(((seg_u + 1) * runs - 1) / total);
+      const int c1 = (int)(((seg_u + cur.nt) * runs - 1) / total);
+      const int np = c1 - c0 + 1;
+      if (tid == 0)  // releases this CTA's partials (ordered by the barrier), acquires the others'
+        s_last = atom_add_acq_rel_gpu(p.tickets + c0, 1u) == (unsigned)(np - 1);
+      __syncthreads();
+      if (s_last) {
+        for (int r = w; r < rows_here; r += 8) {  // weights of the pieces of a row
+          float M = -INFINITY;
+          for (int i = lane; i < np; i += 32) {
+            const int sl = 2 * (c0 + i) + (i == 0 ? 1 : 0);
+            M = fmaxf(M, __ldcg(p.part_ml + ((int64_t)sl * R + r) * 2));
+          }
+          for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, x));
+          const float mb = M == -INFINITY ? 0.f : M;
+          float L = 0.f;
+          for (int i = lane; i < np; i += 32) {
+            const int sl = 2 * (c0 + i) + (i == 0 ? 1 : 0);
+            const float2 q = __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((int64_t)sl * R + r) * 2));
+            const float f = ex2(q.x - mb);
+            join[i * R + r] = f;
+            L = fmaf(f, q.y, L);
+          }
+          for (int x = 16; x; x >>= 1) L += __shfl_xor_sync(~0u, L, x);
+          if (lane == 0) s_ml[r] = make_float2(M, L);
+        }
+        __syncthreads();
+        for (int e = tid; e < rows_here * D; e += 256) {
+          const int r = e / D, d = e - r * D;
+          float v = 0.f;
+#pragma unroll 8
+          for (int i = 0; i < np; i++) {
+            const int sl = 2 * (c0 + i) + (i == 0 ? 1 : 0);
+            v = fmaf(join[i * R + r], __ldcg(p.part_o + ((int64_t)sl * R + r) * DP + d), v);
+          }
+          finish(r, d, s_ml[r].x, s_ml[r].y, v);
+        }
+        if (tid == 0) p.tickets[c0] = 0u;
+      }
+    }
+    // ---- the next segment
+    if (u < u1) {
+      const int b = cur.b;
+      cur.tile += n - 1;
+      const long long span = (long long)cur.nt * cur.nrt * G;
+      advance(cur);
+      if (cur.b != b) seq_u += span;
+    }
+  }
+  asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+}
+
+}  // namespace ortc
