@@ -4,9 +4,9 @@
 //
 // One CTA per SM.  A segment is (sequence, tile of R query rows, KV head); its
 // keys are cut into tiles of 8 warps x KW keys, and the tiles of all segments,
-// in order, are cut into equal runs, one per CTA, whatever the
-// sequences' lengths are (read on the device; every CTA finds its run from a
-// scan over the batch).  Each warp owns KW keys of every tile with a ring of
+// in order (and a few places more for each segment), are cut into equal runs,
+// one per CTA, whatever the sequences' lengths are (read on the device; every
+// CTA finds its run from a scan over the batch).  Each warp owns KW keys of every tile with a ring of
 // its own in shared memory, filled by cp.async some tiles ahead, across
 // segment borders, and its own running maximum and sum (no CTA barrier inside
 // a segment); the warps' states are joined at a segment's end.  A segment that
@@ -160,6 +160,12 @@ struct StreamCfg {
   static constexpr int QB = QP * KS * 512;
   static constexpr int RING = 8 * NS * WSTAGE;
   static constexpr int JOIN = 8 * 8 * 64 * 4;       // [warp][8 rows][64 features]
+  // A segment's start and end (its operands, the join of the warps) cost about
+  // as much as three 64 KB tiles; the list counts them, so that a run of many
+  // short sequences is no longer than one of a long sequence.  Measured on 64
+  // sequences of 100 to 8191 keys: 113 us uncounted, 103, 93, 84.6, 85, 89 at
+  // 1, 2, 3, 4, 6.
+  static constexpr int EXTRA = 3 * 128 / DP;
   static constexpr int SMEM = RING + QB + JOIN + 8 * R * 8;  // + (max, sum) per warp and row
 };
 
@@ -170,9 +176,9 @@ struct StreamPos {
   int lo, hi, nt, nrt;      // its keys, key tiles and row tiles
 };
 
-// Sets the sequence of `s` and returns its tiles per KV head and row tile
-// times its row tiles (0: nothing for this kernel).
-template <int R, int TK>
+// Sets the sequence of `s` and returns its length in the list per KV head
+// (0: nothing for this kernel).
+template <int R, int TK, int EXTRA>
 __device__ __forceinline__ int stream_seq(const StreamArgs& p, StreamPos& s, int b, int min_past) {
   const PagedAttnArgs& a = p.a;
   s.b = b;
@@ -195,14 +201,14 @@ __device__ __forceinline__ int stream_seq(const StreamArgs& p, StreamPos& s, int
   }
   s.nrt = (int)((rows + R - 1) / R);
   s.nt = max(1, (s.hi - s.lo + TK - 1) / TK);
-  return s.nt * s.nrt;
+  return (s.nt + EXTRA) * s.nrt;
 }
 
 template <typename T, int DP, int R>
 __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_constant__ StreamArgs p) {
   using C = StreamCfg<T, DP, R>;
   constexpr bool F32 = C::F32;
-  constexpr int KW = C::KW, TK = C::TK, CHP = C::CHP, NS = C::NS, KS = C::KS, PARTS = Split<T>::PARTS;
+  constexpr int KW = C::KW, TK = C::TK, EXTRA = C::EXTRA, CHP = C::CHP, NS = C::NS, KS = C::KS, PARTS = Split<T>::PARTS;
   constexpr int NPASS = DP / 64;       // blocks of 64 features of the output
   constexpr int NR = R / 8;            // rows a lane holds
   extern __shared__ __align__(128) unsigned char smem[];
@@ -242,7 +248,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     for (int b0 = 0; b0 < nb; b0 += 256) {
       StreamPos t;
       const long long n =
-          b0 + tid < nb ? (long long)stream_seq<R, TK>(p, t, b0 + tid, min_past) * G : 0;
+          b0 + tid < nb ? (long long)stream_seq<R, TK, EXTRA>(p, t, b0 + tid, min_past) * G : 0;
       long long x = n;
       for (int o = 1; o < 32; o <<= 1) {
         const long long y = __shfl_up_sync(~0u, x, o);
@@ -285,22 +291,24 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
   }
   __syncthreads();
   if ((int)blockIdx.x >= runs || u0 >= u1) return;
-  stream_seq<R, TK>(p, cur, s_b0, min_past);
-  long long seq_u = s_u0base;  // first tile of cur.b
+  stream_seq<R, TK, EXTRA>(p, cur, s_b0, min_past);
+  long long seg_u = s_u0base;  // place of tile 0 of the segment in the list
   {
-    const int off = (int)(u0 - seq_u);
-    cur.tile = off % cur.nt;
-    const int sg = off / cur.nt;
-    cur.g = sg % G;
-    cur.rt = sg / G;
+    const int len = cur.nt + EXTRA;
+    const long long off = u0 - s_u0base, sg = off / len;
+    cur.tile = max(0, (int)(off - sg * len) - EXTRA);
+    cur.g = (int)(sg % G);
+    cur.rt = (int)(sg / G);
+    seg_u += sg * len + EXTRA;
   }
+  if (seg_u + cur.tile >= u1) return;  // a run inside a segment's extra places
 
   // ---- loads
   unsigned char* wring = ring + w * NS * C::WSTAGE;
   const uint32_t wring_s = smem_u32(wring);
   const int chunks = D * (int)sizeof(T) / 16;
   StreamPos ld = cur;      // the tile to load next
-  long long lu = u0;
+  long long lu = seg_u + cur.tile;  // its place in the list
   int ld_stage = 0;
   unsigned valid_q[NS];    // per stage: bit r set when key r of the warp is there
 #pragma unroll
@@ -313,7 +321,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     if (++s.rt < s.nrt) return;
     s.rt = 0;
     for (int b = s.b + 1; b < nb; b++)
-      if (stream_seq<R, TK>(p, s, b, min_past)) return;
+      if (stream_seq<R, TK, EXTRA>(p, s, b, min_past)) return;
   };
   // the page of lane r's key (r < KW) of a tile, and whether it has one
   auto page_of = [&](const StreamPos& s, int& slot) {
@@ -333,7 +341,8 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     const long long off =
         ok ? (long long)page * c.page_elems + (long long)slot * c.row_elems + (long long)g * D : -1;
     valid = __ballot_sync(~0u, ok) & ((1u << KW) - 1);
-    if (++lu < u1) {
+    lu += ld.tile + 1 == ld.nt ? 1 + EXTRA : 1;
+    if (lu < u1) {
       advance(ld);
       npage = page_of(ld, nslot);
     }
@@ -361,8 +370,8 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
 
   // ---- segments
   int stage = 0;
-  for (long long u = u0; u < u1;) {
-    const int n = (int)min((long long)(cur.nt - cur.tile), u1 - u);  // tiles of this segment here
+  for (;;) {
+    const int n = (int)min((long long)cur.nt, u1 - seg_u) - cur.tile;  // tiles of it in this run
     // q rows: warp w builds rows w, w + 8 of the A operands
     __syncthreads();  // the last segment's operands are no longer read
 #pragma unroll
@@ -464,15 +473,17 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     pos_lo = __reduce_min_sync(~0u, pos_lo);
     pos_hi = __reduce_max_sync(~0u, pos_hi);
 
-    float m[NR], l[NR], o[NPASS][8][4];
+    float m[NR], l[NR], o[NPASS][8][2 * NR];
 #pragma unroll
     for (int rr = 0; rr < NR; rr++) m[rr] = -INFINITY, l[rr] = 0.f;
 #pragma unroll
     for (int x = 0; x < NPASS; x++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
+      for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int e = 0; e < 2 * NR; e++) o[x][i][e] = 0.f;
 
-    for (int i = 0; i < n; i++, u++) {
+    for (int i = 0; i < n; i++) {
       // the tile NS - 1 ahead into the stage that was read last
       __syncwarp();
       unsigned next_valid = 0;
@@ -492,9 +503,11 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
 
       // scores
       constexpr int NT = KW / 8;
-      float s[NT][4];
+      float s[NT][2][4];  // two chains of products each
 #pragma unroll
-      for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[t][0][e] = s[t][1][e] = 0.f;
       const int row = lane >> 2, cl = lane & 3;
 #pragma unroll
       for (int ks = 0; ks < KS; ks += 2) {
@@ -517,11 +530,11 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             const uint4 qa = qf[(ks + e) * 32 + lane];
-            mma_1688(s[0], qa, kh[2 * e], kh[2 * e + 1]);
-            mma_1688(s[0], qa, kl[2 * e], kl[2 * e + 1]);
+            mma_1688(s[0][e], qa, kh[2 * e], kh[2 * e + 1]);
+            mma_1688(s[0][e], qa, kl[2 * e], kl[2 * e + 1]);
             if (R == 16) {
               const uint4 ql = qf[(KS + ks + e) * 32 + lane];
-              mma_1688(s[0], ql, kh[2 * e], kh[2 * e + 1]);
+              mma_1688(s[0][e], ql, kh[2 * e], kh[2 * e + 1]);
             }
           }
         } else {
@@ -530,8 +543,8 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
             const uint4 q0 = qf[(pt * KS + ks) * 32 + lane], q1 = qf[(pt * KS + ks + 1) * 32 + lane];
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-              mma_16816(s[t], q0, kv[t].x, kv[t].y, T());
-              mma_16816(s[t], q1, kv[t].z, kv[t].w, T());
+              mma_16816(s[t][0], q0, kv[t].x, kv[t].y, T());
+              mma_16816(s[t][1], q1, kv[t].z, kv[t].w, T());
             }
           }
         }
@@ -547,7 +560,9 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
         for (int t = 0; t < NT; t++)
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            float x = (R == 8 ? s[t][e] + s[t][e + 2] : s[t][2 * rr + e]) * fac[rr];
+            float x = s[t][0][2 * rr + e] + s[t][1][2 * rr + e];
+            if (R == 8) x += s[t][0][e + 2] + s[t][1][e + 2];
+            x *= fac[rr];
             if (a.softcap > 0.f) x = tanhf(x);
             pr[rr][t][e] = x * p.t_mul;
           }
@@ -586,16 +601,6 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
           }
         l[rr] = l[rr] * corr[rr] + sum;
       }
-      if (__any_sync(~0u, corr[0] != 1.f || corr[NR - 1] != 1.f)) {
-#pragma unroll
-        for (int x = 0; x < NPASS; x++)
-#pragma unroll
-          for (int i2 = 0; i2 < 8; i2++) {
-            o[x][i2][0] *= corr[0], o[x][i2][1] *= corr[0];
-            o[x][i2][2] *= corr[NR - 1], o[x][i2][3] *= corr[NR - 1];
-          }
-      }
-
       // A value that only some rows see must not reach the others as 0 * inf:
       // such tiles (the border of the mask) are looked over, and one that holds
       // an infinity or NaN is summed key by key.
@@ -618,6 +623,12 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
         odd = __any_sync(~0u, odd);
       }
       if (odd) {
+#pragma unroll
+        for (int x = 0; x < NPASS; x++)
+#pragma unroll
+          for (int i2 = 0; i2 < 8; i2++)
+#pragma unroll
+            for (int e = 0; e < 2 * NR; e++) o[x][i2][e] *= corr[e >> 1];
         for (int k = 0; k < KW; k++) {
           float pk[NR];
 #pragma unroll
@@ -651,7 +662,21 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
         continue;
       }
 
-      // o += p . v
+      // o = o corr + p . v, the products of a tile in accumulators of their own:
+      // the tensor cores' sums are cut off, not rounded, and over a long run of
+      // tiles that adds up (1.5e-6 of the result over 131000 keys, against 0.5e-6
+      // so)
+      auto add = [&](float(&acc)[2 * NR], const float(&d)[4]) {
+        if constexpr (R == 8) {
+          acc[0] = fmaf(acc[0], corr[0], d[0] + d[2]);
+          acc[1] = fmaf(acc[1], corr[0], d[1] + d[3]);
+        } else {
+          acc[0] = fmaf(acc[0], corr[0], d[0]);
+          acc[1] = fmaf(acc[1], corr[0], d[1]);
+          acc[2] = fmaf(acc[2], corr[NR - 1], d[2]);
+          acc[3] = fmaf(acc[3], corr[NR - 1], d[3]);
+        }
+      };
       if constexpr (F32) {
         uint4 pa[2];
         {
@@ -681,10 +706,11 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
             uint32_t h0[2], h1[2];
             Split<float>::one(__uint_as_float(a0[e]), h0);
             Split<float>::one(__uint_as_float(a1[e]), h1);
-            float(&acc)[4] = o[x >> 1][(x & 1) * 4 + e];
-            mma_1688(acc, pa[0], h0[0], h1[0]);
-            mma_1688(acc, pa[0], h0[1], h1[1]);
-            if (R == 16) mma_1688(acc, pa[1], h0[0], h1[0]);
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_1688(d, pa[0], h0[0], h1[0]);
+            mma_1688(d, pa[0], h0[1], h1[1]);
+            if (R == 16) mma_1688(d, pa[1], h0[0], h1[0]);
+            add(o[x >> 1][(x & 1) * 4 + e], d);
           }
         }
       } else {
@@ -723,8 +749,10 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
             const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
             const uint32_t b0 = __byte_perm(a0[e >> 1], a1[e >> 1], sel);
             const uint32_t b1 = __byte_perm(a8[e >> 1], a9[e >> 1], sel);
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int pt = 0; pt < C::QP; pt++) mma_16816(o[x][e], pa[pt], b0, b1, T());
+            for (int pt = 0; pt < C::QP; pt++) mma_16816(d, pa[pt], b0, b1, T());
+            add(o[x][e], d);
           }
         }
       }
@@ -739,7 +767,6 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
       if (cl == 0) wml[w * R + row + 8 * rr] = make_float2(m[rr], l[rr]);
     }
     const bool whole = n == cur.nt;
-    const long long seg_u = seq_u + (long long)(cur.rt * G + cur.g) * cur.nt;  // its first tile
     const bool head = cur.tile != 0;  // begun in an earlier CTA
     const int slot = 2 * blockIdx.x + (head ? 0 : 1);
     // writes a row's value: final, or what the prefix pass hands on
@@ -775,7 +802,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
             float* vv = reinterpret_cast<float*>(&v);
 #pragma unroll
             for (int k = 0; k < 4; k++)
-              vv[k] = R == 8 ? o[x][i2 + k][e] + o[x][i2 + k][e + 2] : o[x][i2 + k][2 * rr + e];
+              vv[k] = o[x][i2 + k][2 * rr + e];
             const int d = F32 ? (i2 >> 2) * 32 + (2 * cl + e) * 4 : (2 * cl + e) * 8 + i2;
             *reinterpret_cast<float4*>(dst + d) = v;
           }
@@ -852,13 +879,10 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
       }
     }
     // ---- the next segment
-    if (u < u1) {
-      const int b = cur.b;
-      cur.tile += n - 1;
-      const long long span = (long long)cur.nt * cur.nrt * G;
-      advance(cur);
-      if (cur.b != b) seq_u += span;
-    }
+    seg_u += cur.nt + EXTRA;
+    if (seg_u >= u1) break;
+    cur.tile = cur.nt - 1;
+    advance(cur);
   }
   asm volatile("cp.async.wait_group 0;\n" ::: "memory");
 }
