@@ -3,7 +3,7 @@
 #include <atomic>
 #include <climits>
 
-#include "paged_stream.cuh"
+#include "paged_tile.cuh"
 
 namespace ortc {
 namespace {
@@ -11,51 +11,108 @@ namespace {
 constexpr size_t kTicketBytes = 4096;  // kept zero between calls (csrc/paged.cu)
 size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Rows of one MMA tile: 8 when no sequence can have more (a row's parts then
-// share an MMA), else 16.
+// Query rows of a sequence and KV head up to which the stream kernel takes it.
+constexpr int kStreamRows = 64;
+
+// Rows of one MMA tile of the stream kernel: 8 when no sequence can have more
+// (a row's parts then share an MMA), else 16.
 int stream_rows(int64_t rows) { return rows <= 8 ? 8 : 16; }
 int padded_head(int D) { return D <= 64 ? 64 : 128; }
 
-template <typename T, int DP, int R>
-int launch_one(const StreamArgs& p, int grid, cudaStream_t st) {
-  using C = StreamCfg<T, DP, R>;
-  static std::atomic<unsigned long long> attr_set{0};  // per device
+// Whether the tile kernel may be used: 16-bit pages, a token's heads in a tile.
+bool tile_ok(const PagedAttnArgs& a) {
+  return a.c.type != ORT_CUDA_CACHE_F32 && a.group <= 64;
+}
+
+template <typename K>
+int set_smem(K kernel, int bytes, std::atomic<unsigned long long>& done) {
   int dev = 0;
   ORTC_CUDA(cudaGetDevice(&dev));
-  if (dev >= 64 || !(attr_set.load() >> dev & 1ull)) {
-    ORTC_CUDA(cudaFuncSetAttribute(paged_stream_kernel<T, DP, R>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    if (dev < 64) attr_set.fetch_or(1ull << dev);
+  if (dev >= 64 || !(done.load() >> dev & 1ull)) {
+    ORTC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (dev < 64) done.fetch_or(1ull << dev);
   }
+  return ORT_CUDA_OK;
+}
+
+template <typename T, int DP, int R>
+int launch_stream_one(const StreamArgs& p, int grid, cudaStream_t st) {
+  using C = StreamCfg<T, DP, R>;
+  static std::atomic<unsigned long long> attr_set{0};  // per device
+  const int rc = set_smem(paged_stream_kernel<T, DP, R>, C::SMEM, attr_set);
+  if (rc) return rc;
   paged_stream_kernel<T, DP, R><<<grid, 256, C::SMEM, st>>>(p);
   ORTC_CUDA(cudaGetLastError());
   return ORT_CUDA_OK;
 }
 
 template <typename T>
-int launch_type(const StreamArgs& p, int rows, int grid, cudaStream_t st) {
+int launch_stream_type(const StreamArgs& p, int rows, int grid, cudaStream_t st) {
   if (padded_head(p.a.c.D) == 64)
-    return rows == 8 ? launch_one<T, 64, 8>(p, grid, st) : launch_one<T, 64, 16>(p, grid, st);
-  return rows == 8 ? launch_one<T, 128, 8>(p, grid, st) : launch_one<T, 128, 16>(p, grid, st);
+    return rows == 8 ? launch_stream_one<T, 64, 8>(p, grid, st)
+                     : launch_stream_one<T, 64, 16>(p, grid, st);
+  return rows == 8 ? launch_stream_one<T, 128, 8>(p, grid, st)
+                   : launch_stream_one<T, 128, 16>(p, grid, st);
 }
 
 int launch_stream(const StreamArgs& p, int rows, int grid, cudaStream_t st, int64_t* launches) {
   int rc;
   if (p.a.c.type == ORT_CUDA_CACHE_F32)
-    rc = launch_type<float>(p, rows, grid, st);
+    rc = launch_stream_type<float>(p, rows, grid, st);
   else if (p.a.c.type == ORT_CUDA_CACHE_F16)
-    rc = launch_type<__half>(p, rows, grid, st);
+    rc = launch_stream_type<__half>(p, rows, grid, st);
   else
-    rc = launch_type<__nv_bfloat16>(p, rows, grid, st);
+    rc = launch_stream_type<__nv_bfloat16>(p, rows, grid, st);
   if (rc == ORT_CUDA_OK) (*launches)++;
   return rc;
 }
 
+template <typename T, int DP>
+int launch_tile_one(const StreamArgs& p, int grid, cudaStream_t st) {
+  using C = TileCfg<T, DP>;
+  static std::atomic<unsigned long long> attr_set{0};
+  int dev = 0;
+  ORTC_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !(attr_set.load() >> dev & 1ull)) {
+    // the register split draws on what the block is launched with
+    cudaFuncAttributes fa;
+    ORTC_CUDA(cudaFuncGetAttributes(&fa, paged_tile_kernel<T, DP>));
+    ORTC_CHECK(fa.numRegs >= kTileRegs, ORT_CUDA_ERR_UNSUPPORTED,
+               "paged attention: built with too few registers for the warpgroups' split");
+  }
+  const int rc = set_smem(paged_tile_kernel<T, DP>, C::SMEM, attr_set);
+  if (rc) return rc;
+  paged_tile_kernel<T, DP><<<grid, kTileThreads, C::SMEM, st>>>(p);
+  ORTC_CUDA(cudaGetLastError());
+  return ORT_CUDA_OK;
+}
+
+int launch_tile(const StreamArgs& p, int grid, cudaStream_t st, int64_t* launches) {
+  int rc;
+  if (p.a.c.type == ORT_CUDA_CACHE_F16)
+    rc = padded_head(p.a.c.D) == 64 ? launch_tile_one<__half, 64>(p, grid, st)
+                                    : launch_tile_one<__half, 128>(p, grid, st);
+  else
+    rc = padded_head(p.a.c.D) == 64 ? launch_tile_one<__nv_bfloat16, 64>(p, grid, st)
+                                    : launch_tile_one<__nv_bfloat16, 128>(p, grid, st);
+  if (rc == ORT_CUDA_OK) (*launches)++;
+  return rc;
+}
+
+// Whether the sequences' own keys, and the shared prefix, may need the tile kernel.
+bool tile_main(const PagedAttnArgs& a) {
+  return tile_ok(a) && (int64_t)a.max_seq * a.group > kStreamRows;
+}
+bool tile_prefix(const PagedAttnArgs& a) {
+  return tile_ok(a) && a.shared && (int64_t)a.c.num_tokens * a.group > kStreamRows;
+}
+size_t piece_rows(const PagedAttnArgs& a) { return tile_main(a) || tile_prefix(a) ? 128 : 16; }
+
 }  // namespace
 
 size_t paged_attention_scratch(const PagedAttnArgs& a, int sm_count) {
-  size_t n = kTicketBytes + al256((size_t)sm_count * 2 * 16 * 2 * 4) +
-             al256((size_t)sm_count * 2 * 16 * 128 * 4);
+  size_t n = kTicketBytes + al256((size_t)sm_count * 2 * piece_rows(a) * 2 * 4) +
+             al256((size_t)sm_count * 2 * piece_rows(a) * 128 * 4);
   if (a.shared) {
     const size_t rows = (size_t)a.c.num_tokens * a.heads;
     n += al256(rows * 8) + al256(rows * a.c.D * 4);
@@ -74,25 +131,34 @@ int launch_paged_attention(const PagedAttnArgs& a, void* scratch, int sm_count, 
   p.q_vec = ((uintptr_t)a.q & 15) == 0 && a.q_stride % 4 == 0;
   p.t_scale = a.softcap > 0.f ? a.scale / a.softcap : a.scale;
   p.t_mul = a.softcap > 0.f ? a.softcap * kLog2e : kLog2e;
-  p.max_rows = INT_MAX;
   char* at = static_cast<char*>(scratch);
   p.tickets = reinterpret_cast<unsigned*>(at);
   at += kTicketBytes;
   p.part_ml = reinterpret_cast<float*>(at);
-  at += al256((size_t)sm_count * 2 * 16 * 2 * 4);
+  at += al256((size_t)sm_count * 2 * piece_rows(a) * 2 * 4);
   p.part_o = reinterpret_cast<float*>(at);
-  at += al256((size_t)sm_count * 2 * 16 * 128 * 4);
+  at += al256((size_t)sm_count * 2 * piece_rows(a) * 128 * 4);
+  int rc;
   if (a.shared) {
     const size_t rows = (size_t)a.c.num_tokens * a.heads;
     p.pre_ml = reinterpret_cast<float*>(at);
     p.pre_o = reinterpret_cast<float*>(at + al256(rows * 8));
     StreamArgs q = p;
     q.prefix = 1;
-    const int rc = launch_stream(q, stream_rows((int64_t)a.c.num_tokens * a.group), sm_count, st,
-                                 launches);
+    q.max_rows = INT_MAX;
+    rc = tile_prefix(a)
+             ? launch_tile(q, sm_count, st, launches)
+             : launch_stream(q, stream_rows((int64_t)a.c.num_tokens * a.group), sm_count, st,
+                             launches);
     if (rc) return rc;
   }
-  return launch_stream(p, stream_rows((int64_t)a.max_seq * a.group), sm_count, st, launches);
+  p.max_rows = tile_ok(a) ? kStreamRows : INT_MAX;
+  if (tile_main(a)) {
+    rc = launch_tile(p, sm_count, st, launches);
+    if (rc) return rc;
+  }
+  const int64_t most = (int64_t)a.max_seq * a.group;
+  return launch_stream(p, stream_rows(std::min<int64_t>(most, p.max_rows)), sm_count, st, launches);
 }
 
 }  // namespace ortc

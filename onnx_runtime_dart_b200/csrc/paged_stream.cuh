@@ -75,6 +75,27 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Writes feature d of (token, head) `at` from its maximum, sum and unnormalised
+// value: the output, joined with what the prefix pass left, or, in the prefix
+// pass, that.
+__device__ __forceinline__ void paged_finish(const StreamArgs& p, int64_t at, int d, float M,
+                                             float L, float v) {
+  const PagedAttnArgs& a = p.a;
+  const int D = a.c.D;
+  if (p.prefix) {
+    p.pre_o[at * D + d] = v;
+    if (d == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * at) = make_float2(M, L);
+    return;
+  }
+  if (a.shared) {
+    const float2 pm = *reinterpret_cast<const float2*>(p.pre_ml + 2 * at);
+    const float mm = fmaxf(M, pm.x), mb = mm == -INFINITY ? 0.f : mm;
+    const float wa = ex2(M - mb), wb = ex2(pm.x - mb);
+    v = v * wa + p.pre_o[at * D + d] * wb;
+    L = L * wa + pm.y * wb;
+  }
+  a.out[at * D + d] = L == 0.f ? 0.f : v / L;
+}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
@@ -769,24 +790,10 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     const bool whole = n == cur.nt;
     const bool head = cur.tile != 0;  // begun in an earlier CTA
     const int slot = 2 * blockIdx.x + (head ? 0 : 1);
-    // writes a row's value: final, or what the prefix pass hands on
     auto finish = [&](int r, int d, float M, float L, float v) {
       const int idx = cur.rt * R + r;
       const int tok = idx / a.group, h = cur.g * a.group + idx - tok * a.group;
-      const int64_t at = (int64_t)(cur.row0 + tok) * a.heads + h;
-      if (p.prefix) {
-        p.pre_o[at * D + d] = v;
-        if (d == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * at) = make_float2(M, L);
-        return;
-      }
-      if (a.shared) {
-        const float2 pm = *reinterpret_cast<const float2*>(p.pre_ml + 2 * at);
-        const float mm = fmaxf(M, pm.x), mb = mm == -INFINITY ? 0.f : mm;
-        const float wa = ex2(M - mb), wb = ex2(pm.x - mb);
-        v = v * wa + p.pre_o[at * D + d] * wb;
-        L = L * wa + pm.y * wb;
-      }
-      a.out[at * D + d] = L == 0.f ? 0.f : v / L;
+      paged_finish(p, (int64_t)(cur.row0 + tok) * a.heads + h, d, M, L, v);
     };
     const int rows_here = min(R, cur.count * a.group - cur.rt * R);
 #pragma unroll

@@ -1,0 +1,753 @@
+// Attention over the paged KV cache for many query rows per sequence and KV
+// head (prompts, a large batch over a shared prefix), 16-bit pages: tiles of
+// 128 query rows on tcgen05.
+//
+// A segment is (sequence, tile of 128 / group tokens with all their query heads
+// of one KV head, KV head); its keys are cut into blocks of KB.  The segments
+// in order, each as long as its keys are many, are cut into equal runs, one per
+// CTA and SM, at block borders; a segment in several runs is joined by the last
+// CTA of them (a ticket), in run order.
+//
+// Roles: two softmax warpgroups, which take the blocks of a segment in turn
+// (one works on its block's weights while the tensor cores work for the
+// other), an MMA warp, a loader warp each for keys and values (cp.async by rows
+// of 16 bytes into the 128-byte swizzle, so pages may have any size).  A
+// warpgroup's thread owns one query row: it reads the row's scores from TMEM,
+// writes the weights back over them as the A operand of p.v, and adds each
+// block's product, which comes in TMEM columns of its own, to its fp32 output in
+// registers (so sums over many blocks are rounded, where the tensor cores cut
+// them off; there is no rescaling in TMEM).  The two warpgroups' states are
+// joined at the segment's end.
+//
+// fp32 results from 16-bit operands: q and the weights are split into parts of
+// the pages' type (csrc/paged_stream.cuh), each part an MMA of its own, the
+// smallest part first.  fp16: 2 + 2 MMAs a product, bf16: 3 + 3, so the tensor
+// bound is 1/2 (1/3) of the dense rate.
+//
+// TMEM columns: scores / weights of the two warpgroups (KB, or KB + KB / 2
+// where three parts need more than the scores), then their p.v (DP each).
+#pragma once
+
+#include "paged_stream.cuh"
+#include "tc.cuh"
+
+namespace ortc {
+
+template <typename T, int DP>
+struct TileCfg {
+  static constexpr int PARTS = Split<T>::PARTS;
+  static constexpr int KB = PARTS == 2 ? 128 : 64;   // keys of a block
+  static constexpr int SREG = PARTS == 2 ? KB : KB * 3 / 2;  // TMEM columns of scores / weights
+  static constexpr int QPART = 128 * DP * 2;         // bytes of one part of the q tile
+  static constexpr int QB = PARTS * QPART;
+  static constexpr int STAGE = KB * DP * 2;
+  static constexpr int NK = PARTS == 2 && DP == 128 ? 3 : 4;  // ring stages of keys
+  static constexpr int NV = PARTS == 2 && DP == 128 ? 2 : 4;  // and of values
+  static constexpr int DATA = QB + (NK + NV) * STAGE;
+  static constexpr int EXTRA = 2 * KB;  // what a segment's start and end cost, in keys
+  // data, (max, sum) of 128 rows, block validity, barriers, after alignment to 1024
+  static constexpr int SMEM = 1024 + DATA + 128 * 8 + 8 * 16 + 256;
+  static_assert(2 * SREG + 2 * DP <= 512, "TMEM");
+  static_assert(DP * 128 * 4 <= QB, "the output is staged in the q tile");
+};
+
+struct TilePos {
+  int b, rt, g;
+  int row0, count, past;
+  int lo, hi, nt, nrt;  // keys and blocks of this segment; row tiles of the sequence
+  int len;              // keys it counts as in the list (the causal border unclamped)
+  // the sequence: first base key, tiles whose keys start there
+  int base, ramp;
+};
+
+// Sets the sequence of `s`; its number of row tiles (0: not this kernel's).
+__device__ __forceinline__ int tile_seq(const StreamArgs& p, TilePos& s, int b, int min_past,
+                                        int TT) {
+  const PagedAttnArgs& a = p.a;
+  s.b = b;
+  s.nrt = 0;
+  if (p.prefix) {
+    s.row0 = 0, s.past = 0;
+    s.count = max(0, min(a.c.cu[a.c.batch], a.c.num_tokens));
+    s.base = a.window ? min(a.shared, max(0, min_past + 1 - a.window)) : 0;
+  } else {
+    const PagedSeq q = paged_seq(a.c, b, a.max_seq, a.shared);
+    s.row0 = q.row0, s.count = q.count, s.past = q.past;
+    if ((int64_t)q.count * a.group <= p.max_rows) return 0;
+    s.base = a.shared;
+  }
+  s.nrt = (s.count + TT - 1) / TT;
+  s.ramp = s.nrt;
+  if (!p.prefix && a.window) {
+    const long long x = (long long)s.base + a.window - 1 - s.past;
+    s.ramp = x < 0 ? 0 : (int)min((long long)s.nrt, x / TT + 1);
+  }
+  return s.nrt;
+}
+
+// Keys that row tiles 0 .. r - 1 of one KV head count as, with `extra` each.
+__device__ __forceinline__ long long tile_sum(const StreamArgs& p, const TilePos& s, int r, int TT,
+                                              int extra) {
+  if (p.prefix) return (long long)r * (max(1, p.a.shared - s.base) + extra);
+  const long long f = min(r, s.ramp), c = r - f;
+  return f * (s.past - s.base) + TT * (f * (f + 1) / 2) + c * (TT + p.a.window - 1) +
+         (long long)r * extra;
+}
+
+// Sets the segment (rt, g) of the sequence of `s`.
+template <int KB>
+__device__ __forceinline__ void tile_segment(const StreamArgs& p, TilePos& s, int rt, int g,
+                                             int TT) {
+  s.rt = rt, s.g = g;
+  if (p.prefix) {
+    s.lo = s.base, s.hi = p.a.shared;
+    s.len = max(1, s.hi - s.lo);
+  } else {
+    const int t0 = s.past + rt * TT;
+    s.lo = p.a.window ? max(s.base, t0 + 1 - p.a.window) : s.base;
+    s.hi = min(s.past + s.count, t0 + TT);
+    s.len = t0 + TT - s.lo;
+  }
+  s.nt = max(1, (s.hi - s.lo + KB - 1) / KB);
+}
+
+__device__ __forceinline__ void bar_sync(int id, int n) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
+}
+__device__ __forceinline__ bool bar_or(int id, int n, bool x) {
+  uint32_t y;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %3, 0;\n\t"
+      "bar.red.or.pred p, %1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(y)
+      : "r"(id), "r"(n), "r"((uint32_t)x)
+      : "memory");
+  return y != 0;
+}
+
+// tile_warp_regs: registers per thread after the split; they draw on what the
+// block was launched with (kTileRegs a thread), which launch_tile checks.
+constexpr int kTileThreads = 384, kTileSoftRegs = 216, kTileLoadRegs = 72, kTileRegs = 168;
+static_assert(256 * kTileSoftRegs + 128 * kTileLoadRegs <= kTileThreads * kTileRegs, "registers");
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    paged_tile_kernel(const __grid_constant__ StreamArgs p) {
+  using C = TileCfg<T, DP>;
+  constexpr int PARTS = C::PARTS, KB = C::KB, NK = C::NK, NV = C::NV, EX = C::EXTRA;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  unsigned char* qs = smem;                 // [part][DP / 64][128 rows][128 B], swizzled
+  unsigned char* ks = qs + C::QB;           // [NK][DP / 64][KB rows][128 B]
+  unsigned char* vs = ks + NK * C::STAGE;   // [NV] the same
+  float* ost = reinterpret_cast<float*>(qs);  // [DP][128] at a segment's end
+  float2* stats = reinterpret_cast<float2*>(smem + C::DATA);  // [128]
+  uint32_t* kvalid = reinterpret_cast<uint32_t*>(stats + 128);  // [8][4]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(kvalid + 32);
+  uint64_t *kfull = bars, *kempty = kfull + NK, *vfull = kempty + NK, *vempty = vfull + NV,
+           *sfull = vempty + NV, *pfull = sfull + 2, *pvfull = pfull + 2, *qfull = pvfull + 2;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(qfull + 1);
+  int* s_last = reinterpret_cast<int*>(tmem_at + 1);
+  static_assert((2 * 4 + 2 * 4 + 7) * 8 + 8 <= 256, "barriers");
+
+  const PagedAttnArgs& a = p.a;
+  const PagedView& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int D = c.D, G = c.kv_heads, nb = p.prefix ? 1 : c.batch, TT = 128 / a.group;
+
+  // ---- this CTA's run
+  int min_past = 0;
+  int* s_min = reinterpret_cast<int*>(stats);
+  if (p.prefix && a.window) {
+    min_past = INT_MAX / 2;
+    for (int b = tid; b < c.batch; b += kTileThreads)
+      if (c.cu[b + 1] > c.cu[b]) min_past = min(min_past, max(0, c.past[b]));
+    min_past = __reduce_min_sync(~0u, min_past);
+    if (lane == 0) s_min[warp] = min_past;
+    __syncthreads();
+    for (int i = 0; i < kTileThreads / 32; i++) min_past = min(min_past, s_min[i]);
+    __syncthreads();
+  }
+  long long* s_scan = reinterpret_cast<long long*>(stats);  // [12], then the start and sequence
+  long long total = 0, u0 = 0, u1 = 0;
+  int runs = 1;
+  for (int pass = 0; pass < 2; pass++) {  // the total, then the sequence of u0
+    long long base = 0;
+    for (int b0 = 0; b0 < nb; b0 += kTileThreads) {
+      TilePos t;
+      long long n = 0;
+      if (b0 + tid < nb) {
+        const int nrt = tile_seq(p, t, b0 + tid, min_past, TT);
+        if (nrt) n = tile_sum(p, t, nrt, TT, EX) * G;
+      }
+      long long x = n;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(~0u, x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane == 31) s_scan[warp] = x;
+      __syncthreads();
+      long long all = 0, before = 0;
+      for (int i = 0; i < kTileThreads / 32; i++) {
+        if (i < warp) before += s_scan[i];
+        all += s_scan[i];
+      }
+      if (pass == 1) {
+        const long long start = base + before + x - n;
+        if (n && start <= u0 && u0 < start + n) {
+          s_scan[16] = start;
+          s_scan[17] = b0 + tid;
+        }
+      }
+      base += all;
+      __syncthreads();
+    }
+    if (pass == 0) {
+      total = base;
+      if (total == 0) return;
+      runs = (int)min((long long)gridDim.x, max(1ll, total / KB));  // a run holds a block at least
+      if ((int)blockIdx.x >= runs) return;
+      u0 = total * blockIdx.x / runs;
+      u1 = total * (blockIdx.x + 1) / runs;
+    }
+  }
+  // the segment and block of u0; each role walks the list from here
+  TilePos cur;
+  long long seg;  // place of block 0 of the segment
+  int k0;
+  {
+    const long long off = u0 - s_scan[16];
+    tile_seq(p, cur, (int)s_scan[17], min_past, TT);
+    int lo = 0, hi = cur.nrt;  // the last row tile that starts at or before off
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (tile_sum(p, cur, mid, TT, EX) * G <= off)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    tile_segment<KB>(p, cur, lo, 0, TT);
+    const long long rem = off - tile_sum(p, cur, lo, TT, EX) * G, each = cur.len + EX;
+    cur.g = (int)(rem / each);
+    const long long in = rem - cur.g * each - EX;
+    seg = u0 - in;
+    k0 = in <= 0 ? 0 : (int)((in + KB - 1) / KB);
+  }
+  // to the next segment with a block in this run; false: none
+  auto next = [&](TilePos& s, long long& at, int& first) {
+    for (;;) {
+      at += s.len + EX;
+      if (at >= u1) return false;
+      first = 0;
+      if (s.g + 1 < G) {
+        tile_segment<KB>(p, s, s.rt, s.g + 1, TT);
+        return true;
+      }
+      if (s.rt + 1 < s.nrt) {
+        tile_segment<KB>(p, s, s.rt + 1, 0, TT);
+        return true;
+      }
+      int b = s.b + 1;
+      while (b < nb && !tile_seq(p, s, b, min_past, TT)) b++;
+      if (b >= nb) return false;
+      tile_segment<KB>(p, s, 0, 0, TT);
+      return true;
+    }
+  };
+  auto blocks = [&](const TilePos& s, long long at, int first) {
+    return (int)min((long long)s.nt, (u1 - at + KB - 1) / KB) - first;
+  };
+  if (seg + (long long)k0 * KB >= u1 || k0 >= cur.nt) {  // no block of this segment in the run
+    if (!next(cur, seg, k0)) return;
+  }
+  __syncthreads();  // s_scan has been read
+
+  if (tid == 0) {
+    for (int i = 0; i < NK; i++) mbar_init(kfull + i, 1), mbar_init(kempty + i, 1);
+    for (int i = 0; i < NV; i++) mbar_init(vfull + i, 1), mbar_init(vempty + i, 1);
+    for (int i = 0; i < 2; i++) mbar_init(sfull + i, 1), mbar_init(pfull + i, 128), mbar_init(pvfull + i, 1);
+    mbar_init(qfull, 256);
+    fence_mbarrier_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_at, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_at;
+  bool dead = false;  // a wait ran out: no more waits, every barrier is still met
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTileLoadRegs));
+    if (warp == 8) {
+      // ---- MMA
+      constexpr uint32_t id_s = idesc_f16(PARTS == 3, 128, KB);
+      constexpr uint32_t id_o = idesc_f16(PARTS == 3, 128, DP) | kIdescBMnMajor;
+      const uint32_t q_s = smem_u32(qs), k_s = smem_u32(ks), v_s = smem_u32(vs);
+      int kc = 0, vc = 0, pc[2] = {0, 0}, sc = 0;
+      auto wait = [&](uint64_t* bar, int parity) {
+        if (!dead && !mbar_wait(bar, parity)) {
+          dead = true;
+          record_error(c.err, KERR_WAIT_FULL);
+        }
+        dead = __any_sync(~0u, dead);
+        tc_fence_after();
+      };
+      auto scores = [&](int w) {  // s = q . k of the next block
+        const int st = kc % NK;
+        wait(kfull + st, (kc / NK) & 1);
+        kc++;
+        if (dead) return;
+        if (elect_one()) {
+          const uint32_t kb = k_s + st * C::STAGE;
+#pragma unroll
+          for (int pt = PARTS - 1; pt >= 0; pt--)
+#pragma unroll
+            for (int x = 0; x < DP / 16; x++)
+              mma_f16_ss(tmem + w * C::SREG,
+                         smem_desc_sw128(q_s + pt * C::QPART + (x >> 2) * 16384 + (x & 3) * 32),
+                         smem_desc_sw128(kb + (x >> 2) * (KB * 128) + (x & 3) * 32), id_s,
+                         pt != PARTS - 1 || x);
+          mma_commit(kempty + st);
+          mma_commit(sfull + w);
+        }
+        __syncwarp();
+      };
+      for (;;) {
+        const int n = blocks(cur, seg, k0);
+        wait(qfull, sc & 1);
+        sc++;
+        scores(0);
+        if (n > 1) scores(1);
+        for (int k = 0; k < n; k++) {
+          const int w = k & 1, st = vc % NV;
+          wait(pfull + w, pc[w] & 1);
+          pc[w]++;
+          wait(vfull + st, (vc / NV) & 1);
+          vc++;
+          if (!dead && elect_one()) {
+            const uint32_t vb = v_s + st * C::STAGE;
+#pragma unroll
+            for (int pt = PARTS - 1; pt >= 0; pt--)
+#pragma unroll
+              for (int x = 0; x < KB / 16; x++) {
+                const int col = pt < 2 ? 32 * (x >> 1) + 16 * pt + 8 * (x & 1)
+                                       : KB + 16 * (x >> 1) + 8 * (x & 1);
+                mma_f16_ts(tmem + 2 * C::SREG + w * DP, tmem + w * C::SREG + col,
+                           smem_desc_sw128_mn(vb + x * 2048, KB * 128), id_o,
+                           pt != PARTS - 1 || x);
+              }
+            mma_commit(vempty + st);
+            mma_commit(pvfull + w);
+          }
+          __syncwarp();
+          if (k + 2 < n) scores(w);
+        }
+        if (!next(cur, seg, k0)) break;
+      }
+    } else if (warp <= 10) {
+      // ---- loaders: warp 9 keys, warp 10 values
+      const bool is_k = warp == 9;
+      const int NS = is_k ? NK : NV;
+      uint64_t *full = is_k ? kfull : vfull, *empty = is_k ? kempty : vempty;
+      const uint32_t ring = smem_u32(is_k ? ks : vs);
+      const T* src = static_cast<const T*>(is_k ? c.key : c.value);
+      constexpr int CHP = DP / 8, RPI = 32 / CHP, LK = KB / 32;
+      const int chunks = D / 8, ch = lane & (CHP - 1);
+      int cnt = 0;
+      int pending = -1;  // a stage whose copies have not been announced
+      auto announce = [&] {  // its copies have landed (waited for): hand it to the MMA
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + pending);
+        pending = -1;
+      };
+      for (;;) {
+        const int n = blocks(cur, seg, k0);
+        for (int k = 0; k < n; k++, cnt++) {
+          const int st = cnt % NS, base = cur.lo + (k0 + k) * KB;
+          long long off[LK];
+#pragma unroll
+          for (int i = 0; i < LK; i++) {
+            const int j = base + 32 * i + lane;
+            off[i] = -1;
+            if (j < cur.hi) {
+              const int pg = p.page_div.div(j);
+              const int page = __ldg(c.table + (int64_t)(p.prefix ? 0 : cur.b) * c.max_pages + pg);
+              if (page >= 0 && page < c.num_pages)
+                off[i] = (long long)page * c.page_elems +
+                         (long long)(j - pg * c.page_size) * c.row_elems + (long long)cur.g * D;
+              else if (is_k)
+                record_error(c.err, KERR_PAGED_PAGE);
+            }
+          }
+          if (cnt >= NS && !dead) {
+            const int par = ((cnt / NS) - 1) & 1;
+            if (!__all_sync(~0u, mbar_try_wait(empty + st, par))) {
+              if (pending >= 0) {  // do not hold a landed stage back
+                asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+                announce();
+              }
+              if (!mbar_wait(empty + st, par)) {
+                dead = true;
+                record_error(c.err, KERR_WAIT_EMPTY);
+              }
+              dead = __any_sync(~0u, dead);
+            }
+          }
+          if (is_k) {
+#pragma unroll
+            for (int i = 0; i < LK; i++) {
+              const unsigned ok = __ballot_sync(~0u, off[i] >= 0);
+              if (lane == 0) kvalid[(cnt & 7) * 4 + i] = ok;
+            }
+          }
+          const uint32_t at = ring + st * C::STAGE + (ch >> 3) * (KB * 128);
+#pragma unroll
+          for (int i = 0; i < KB / RPI; i++) {
+            const int r = i * RPI + lane / CHP;
+            const long long o = __shfl_sync(~0u, off[i * RPI / 32], r & 31);
+            const int bytes = o >= 0 && ch < chunks ? 16 : 0;
+            cp16(at + r * 128 + (((ch & 7) ^ (r & 7)) << 4), src + (bytes ? o + ch * 8 : 0), bytes);
+          }
+          asm volatile("cp.async.commit_group;\n" ::: "memory");
+          if (pending >= 0) {
+            asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+            announce();
+          }
+          pending = st;
+        }
+        if (!next(cur, seg, k0)) break;
+      }
+      asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+      if (pending >= 0) announce();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTileSoftRegs));
+    // ---- softmax warpgroup wg; thread: query row `row` of the tile
+    const int wg = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t tl = tmem + (((uint32_t)(warp & 3) * 32) << 16);
+    const uint32_t ts = tl + wg * C::SREG, to = tl + 2 * C::SREG + wg * DP;
+    int sc = 0, gb = 0;  // this warpgroup's blocks so far; all blocks so far
+    auto wait = [&](uint64_t* bar, int parity) {
+      if (!dead && !mbar_wait(bar, parity)) {
+        dead = true;
+        record_error(c.err, KERR_WAIT_MMA);
+      }
+      __syncwarp();
+      tc_fence_after();
+    };
+    for (;;) {
+      const int n = blocks(cur, seg, k0);
+      const int tok0 = cur.rt * TT, rows_here = min(TT, cur.count - tok0) * a.group;
+      const bool has = row < rows_here;
+      const int tok = tok0 + (has ? row / a.group : 0);
+      const int head = cur.g * a.group + (has ? row % a.group : 0);
+      // q: this warpgroup's half of the features of every row
+      float fac = p.t_scale;
+      {
+        const float* src = a.q + (int64_t)(cur.row0 + tok) * a.q_stride + (int64_t)head * D;
+        auto load8 = [&](int ch, float (&x)[8]) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[e] = 0.f;
+          if (!has || 8 * ch >= D) return;
+          if (p.q_vec) {
+            *reinterpret_cast<float4*>(x) = __ldg(reinterpret_cast<const float4*>(src) + 2 * ch);
+            *reinterpret_cast<float4*>(x + 4) =
+                __ldg(reinterpret_cast<const float4*>(src) + 2 * ch + 1);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = __ldg(src + 8 * ch + e);
+          }
+        };
+        float up = 1.f;
+        if constexpr (PARTS == 2) {  // the row's largest value into [2^13, 2^14)
+          float mx = 0.f;
+#pragma unroll
+          for (int ch = 0; ch < DP / 8; ch++) {
+            float x[8];
+            load8(ch, x);
+#pragma unroll
+            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[e]));
+          }
+          int ex = (int)(__float_as_uint(mx) >> 23) - 127;
+          ex = max(-100, min(ex, 126));
+          up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
+          fac *= __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
+        }
+#pragma unroll
+        for (int y = 0; y < DP / 16; y++) {
+          const int ch = wg * (DP / 16) + y;
+          float x[8];
+          load8(ch, x);
+          uint32_t wd[4][PARTS];
+#pragma unroll
+          for (int e = 0; e < 4; e++) Split<T>::pair(x[2 * e] * up, x[2 * e + 1] * up, wd[e]);
+#pragma unroll
+          for (int pt = 0; pt < PARTS; pt++)
+            *reinterpret_cast<uint4*>(qs + pt * C::QPART + (ch >> 3) * 16384 + row * 128 +
+                                      (((ch & 7) ^ (row & 7)) << 4)) =
+                make_uint4(wd[0][pt], wd[1][pt], wd[2][pt], wd[3][pt]);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(qfull);
+      }
+      int pos = -1;  // the row's position (-1: no row), and what all rows see
+      int all_hi = cur.past + tok0, all_lo = cur.past + min(tok0 + TT, cur.count) - 1;
+      if (p.prefix) {
+        pos = all_hi = all_lo = INT_MAX / 2;
+        if (a.window) {
+          all_hi = -1;  // rows of different sequences: look at each
+          if (has) {
+            int lo = 0, hi = c.batch;
+            while (lo < hi) {
+              const int mid = (lo + hi) >> 1;
+              if (c.cu[mid + 1] <= tok)
+                lo = mid + 1;
+              else
+                hi = mid;
+            }
+            if (lo < c.batch) pos = c.past[lo] + tok - c.cu[lo];
+          }
+        }
+      } else if (has) {
+        pos = cur.past + tok;
+      }
+      const int from = a.window ? pos - a.window + 1 : 0;
+      const float cmul = fac * p.t_mul;
+
+      float m = -INFINITY, l = 0.f, o[DP];
+#pragma unroll
+      for (int i = 0; i < DP; i++) o[i] = 0.f;
+      for (int k = wg; k < n; k += 2) {
+        const int base = cur.lo + (k0 + k) * KB;
+        wait(sfull + wg, sc & 1);
+        uint32_t vw[KB / 32];
+        bool full = base + KB - 1 <= all_hi && base + KB <= cur.hi &&
+                    (!a.window || base > all_lo - a.window);
+#pragma unroll
+        for (int i = 0; i < KB / 32; i++) {
+          vw[i] = kvalid[((gb + k) & 7) * 4 + i];
+          full = full && vw[i] == ~0u;
+        }
+        if (!full) {  // the keys of each word that the row sees
+#pragma unroll
+          for (int i = 0; i < KB / 32; i++) {
+            const int x0 = max(from - (base + 32 * i), 0), x1 = min(pos - (base + 32 * i), 31);
+            vw[i] &= pos < base + 32 * i || x0 > x1 ? 0u : (~0u >> (31 - x1)) & (~0u << x0);
+          }
+        }
+        // the row's maximum
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < KB / 32; i++) {
+          uint32_t r[32];
+          tmem_ld32(ts + 32 * i, r);
+          tmem_ld_wait();
+          if (full) {
+#pragma unroll
+            for (int e = 0; e < 32; e++) mx = fmaxf(mx, __uint_as_float(r[e]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+              if ((vw[i] >> e) & 1) mx = fmaxf(mx, __uint_as_float(r[e]));
+          }
+        }
+        if (mx != -INFINITY) mx = a.softcap > 0.f ? tanhf(mx * fac) * p.t_mul : mx * cmul;
+        const float mn = fmaxf(m, mx), mb = mn == -INFINITY ? 0.f : mn;
+        const float corr = ex2(m - mb), sub = PARTS == 2 ? mb - 15.f : mb;
+        m = mn;
+
+        // values only some rows see: an infinity or NaN among them must not reach
+        // the others as 0 * inf (see paged_stream.cuh)
+        bool odd = false;
+        const unsigned char* vst = vs + ((gb + k) % NV) * C::STAGE;
+        if (!full) {
+          wait(vfull + (gb + k) % NV, ((gb + k) / NV) & 1);
+          for (int i = row; i < C::STAGE / 16; i += 128) {
+            const uint4 v = reinterpret_cast<const uint4*>(vst)[i];
+            const uint32_t ws[4] = {v.x, v.y, v.z, v.w};
+            constexpr uint32_t inf = PARTS == 2 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              odd |= (ws[e] & inf) == inf || ((ws[e] >> 16) & inf) == inf;
+          }
+          odd = bar_or(2 + wg, 128, odd);
+        }
+
+        // weights, over the scores
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < KB / 32; i++) {
+          uint32_t r[32];
+          tmem_ld32(ts + 32 * i, r);
+          tmem_ld_wait();
+          float x[32];
+          if (a.softcap > 0.f) {
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+              x[e] = ex2(fmaf(tanhf(__uint_as_float(r[e]) * fac), p.t_mul, -sub));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e++) x[e] = ex2(fmaf(__uint_as_float(r[e]), cmul, -sub));
+          }
+          if (!full) {
+#pragma unroll
+            for (int e = 0; e < 32; e++) x[e] = (vw[i] >> e) & 1 ? x[e] : 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e++) sum += x[e];
+          if (odd) {  // kept in fp32 for the sum below
+#pragma unroll
+            for (int e = 0; e < 32; e++) r[e] = __float_as_uint(x[e]);
+            uint32_t h[16];
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+#pragma unroll
+              for (int e = 0; e < 16; e++) h[e] = r[16 * y + e];
+              tmem_st16(ts + 32 * i + 16 * y, h);
+            }
+            continue;
+          }
+          uint32_t wd[PARTS][16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            uint32_t t[PARTS];
+            Split<T>::pair(x[2 * e], x[2 * e + 1], t);
+#pragma unroll
+            for (int pt = 0; pt < PARTS; pt++) wd[pt][e] = t[pt];
+          }
+          tmem_st16(ts + 32 * i, wd[0]);
+          tmem_st16(ts + 32 * i + 16, wd[1]);
+          if (PARTS == 3) tmem_st16(ts + KB + 16 * i, wd[PARTS - 1]);
+        }
+        l = l * corr + sum;
+        tmem_st_wait();
+        if (odd) {
+#pragma unroll
+          for (int i = 0; i < DP; i++) o[i] *= corr;
+          for (int j = 0; j < KB; j++) {
+            uint32_t r;
+            tmem_ld1(ts + j, r);
+            tmem_ld_wait();
+            const float w = __uint_as_float(r);
+#pragma unroll
+            for (int ch = 0; ch < DP / 8; ch++) {
+              const uint4 v = *reinterpret_cast<const uint4*>(
+                  vst + (ch >> 3) * (KB * 128) + j * 128 + (((ch & 7) ^ (j & 7)) << 4));
+              const T* ve = reinterpret_cast<const T*>(&v);
+#pragma unroll
+              for (int e = 0; e < 8; e++)
+                if (w != 0.f) o[8 * ch + e] = fmaf(w, (float)ve[e], o[8 * ch + e]);
+            }
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(pfull + wg);
+        wait(pvfull + wg, sc & 1);
+        sc++;
+        if (odd) continue;  // the product of what is not weights
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++) {
+          uint32_t r[32];
+          tmem_ld32(to + 32 * i, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; e++) o[32 * i + e] = fmaf(o[32 * i + e], corr, __uint_as_float(r[e]));
+        }
+      }
+      gb += n;
+
+      // ---- the segment's end: join the warpgroups, write rows by warps
+      auto at = [&](int d, int r) -> float& { return ost[d * 128 + (r ^ (d & 31))]; };
+      tc_fence_before();
+      bar_sync(1, 256);  // every MMA of the segment is done: the q tile is free
+      if (wg == 1) {
+#pragma unroll
+        for (int i = 0; i < DP; i++) at(i, row) = o[i];
+        stats[row] = make_float2(m, l);
+      }
+      bar_sync(1, 256);
+      if (wg == 0) {
+        const float2 s2 = stats[row];
+        const float M = fmaxf(m, s2.x), mb = M == -INFINITY ? 0.f : M;
+        const float w0 = ex2(m - mb), w1 = ex2(s2.x - mb);
+        stats[row] = make_float2(M, l * w0 + s2.y * w1);
+#pragma unroll
+        for (int i = 0; i < DP; i++) at(i, row) = o[i] * w0 + at(i, row) * w1;
+      }
+      bar_sync(1, 256);
+      const bool whole = n == cur.nt;
+      const int slot = 2 * blockIdx.x + (k0 ? 0 : 1);
+      auto place = [&](int r) {
+        const int t = r / a.group;
+        return (int64_t)(cur.row0 + tok0 + t) * a.heads + cur.g * a.group + r - t * a.group;
+      };
+      for (int r = warp; r < rows_here; r += 8) {
+        const float2 ml = stats[r];
+        if (whole) {
+          const int64_t to_row = place(r);
+          for (int d = lane; d < D; d += 32) paged_finish(p, to_row, d, ml.x, ml.y, at(d, r));
+        } else {
+          for (int d = lane; d < D; d += 32)
+            p.part_o[((int64_t)slot * 128 + r) * DP + d] = at(d, r);
+          if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * 128 + r) * 2) = ml;
+        }
+      }
+      if (!whole) {
+        const int c0 = (int)(((seg + 1) * runs - 1) / total);
+        const int c1 = (int)(((seg + (long long)(cur.nt - 1) * KB + 1) * runs - 1) / total);
+        const int np = c1 - c0 + 1;
+        bar_sync(1, 256);
+        if (tid == 0) *s_last = atom_add_acq_rel_gpu(p.tickets + c0, 1u) == (unsigned)(np - 1);
+        bar_sync(1, 256);
+        if (*s_last) {
+          for (int r = warp; r < rows_here; r += 8) {
+            auto piece = [&](int i) {
+              return (int64_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * 128 + r;
+            };
+            float M = -INFINITY;
+            for (int i = lane; i < np; i += 32) M = fmaxf(M, __ldcg(p.part_ml + piece(i) * 2));
+            for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, x));
+            const float mb = M == -INFINITY ? 0.f : M;
+            float L = 0.f, v[DP / 32];
+#pragma unroll
+            for (int x = 0; x < DP / 32; x++) v[x] = 0.f;
+            for (int i0 = 0; i0 < np; i0 += 32) {
+              float2 q = make_float2(-INFINITY, 0.f);
+              if (i0 + lane < np)
+                q = __ldcg(reinterpret_cast<const float2*>(p.part_ml + piece(i0 + lane) * 2));
+              const float f = ex2(q.x - mb);
+              L = fmaf(f, q.y, L);
+              for (int i = 0; i < min(32, np - i0); i++) {
+                const float w = __shfl_sync(~0u, f, i);
+#pragma unroll
+                for (int x = 0; x < DP / 32; x++)
+                  if (lane + 32 * x < D)
+                    v[x] = fmaf(w, __ldcg(p.part_o + piece(i0 + i) * DP + lane + 32 * x), v[x]);
+              }
+            }
+            for (int x = 16; x; x >>= 1) L += __shfl_xor_sync(~0u, L, x);
+            const int64_t to_row = place(r);
+#pragma unroll
+            for (int x = 0; x < DP / 32; x++)
+              if (lane + 32 * x < D) paged_finish(p, to_row, lane + 32 * x, M, L, v[x]);
+          }
+          if (tid == 0) p.tickets[c0] = 0u;
+        }
+      }
+      bar_sync(1, 256);  // the staged output has been read
+      if (!next(cur, seg, k0)) break;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace ortc

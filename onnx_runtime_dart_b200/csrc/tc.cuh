@@ -50,6 +50,21 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr) {
   return d;
 }
 
+// Shared-memory matrix descriptor of an MN-major operand in the same physical
+// layout (rows of 128 bytes along M or N, one per k, 8-row groups 1024 bytes
+// apart): blocks of 64 16-bit elements along M or N are `mn_stride` bytes apart
+// (leading byte offset), groups of 8 k 1024 bytes (stride byte offset).
+__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t saddr, uint32_t mn_stride) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)((mn_stride >> 4) & 0x3FFF) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+constexpr uint32_t kIdescBMnMajor = 1u << 16;  // B is MN-major
+
 // kind::f16 instruction descriptor: fp32 accumulator, A and B of the same
 // 16-bit type (0 = f16, 1 = bf16), both K-major, shape M x N.
 __host__ __device__ constexpr uint32_t idesc_f16(int ab_bf16, int M, int N) {
@@ -166,6 +181,9 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld1(uint32_t taddr, uint32_t& r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, uint4 a, uint4 b) {
   asm volatile(
