@@ -433,6 +433,12 @@ int encode_tma_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, ui
                   uint64_t d1, uint64_t stride1, uint32_t b0, uint32_t b1,
                   CUtensorMapSwizzle swz);
 
+// A 3-D tensor [d2][d1][d0] with pitches stride1, stride2 bytes, box b0 x 1 x b2,
+// 128-byte swizzle, zeros outside.
+int encode_tma_rows(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t d0,
+                    uint64_t d1, uint64_t d2, uint64_t stride1, uint64_t stride2, uint32_t b0,
+                    uint32_t b2);
+
 // ---- kernel launchers (each returns an ORT status) -----------------------
 // All pointers are device pointers; launches go to `st`.
 

@@ -67,8 +67,8 @@ int launch_stream(const StreamArgs& p, int rows, int grid, cudaStream_t st, int6
   return rc;
 }
 
-template <typename T, int DP>
-int launch_tile_one(const StreamArgs& p, int grid, cudaStream_t st) {
+template <typename T, int DP, bool CAP>
+int launch_tile_cap(const TileArgs& p, int grid, cudaStream_t st) {
   using C = TileCfg<T, DP>;
   static std::atomic<unsigned long long> attr_set{0};
   int dev = 0;
@@ -76,25 +76,47 @@ int launch_tile_one(const StreamArgs& p, int grid, cudaStream_t st) {
   if (dev >= 64 || !(attr_set.load() >> dev & 1ull)) {
     // the register split draws on what the block is launched with
     cudaFuncAttributes fa;
-    ORTC_CUDA(cudaFuncGetAttributes(&fa, paged_tile_kernel<T, DP>));
+    ORTC_CUDA(cudaFuncGetAttributes(&fa, paged_tile_kernel<T, DP, CAP>));
     ORTC_CHECK(fa.numRegs >= kTileRegs, ORT_CUDA_ERR_UNSUPPORTED,
                "paged attention: built with too few registers for the warpgroups' split");
   }
-  const int rc = set_smem(paged_tile_kernel<T, DP>, C::SMEM, attr_set);
+  const int rc = set_smem(paged_tile_kernel<T, DP, CAP>, C::SMEM, attr_set);
   if (rc) return rc;
-  paged_tile_kernel<T, DP><<<grid, kTileThreads, C::SMEM, st>>>(p);
+  paged_tile_kernel<T, DP, CAP><<<grid, kTileThreads, C::SMEM, st>>>(p);
   ORTC_CUDA(cudaGetLastError());
   return ORT_CUDA_OK;
 }
 
-int launch_tile(const StreamArgs& p, int grid, cudaStream_t st, int64_t* launches) {
+template <typename T, int DP>
+int launch_tile_one(const TileArgs& p, int grid, cudaStream_t st) {
+  return p.s.a.softcap > 0.f ? launch_tile_cap<T, DP, true>(p, grid, st)
+                           : launch_tile_cap<T, DP, false>(p, grid, st);
+}
+
+int launch_tile(const StreamArgs& s, int grid, cudaStream_t st, int64_t* launches) {
+  TileArgs p;
+  p.s = s;
+  const PagedView& c = s.a.c;
+  const bool f16 = c.type == ORT_CUDA_CACHE_F16;
+  const int64_t tokens = (int64_t)c.num_pages * c.page_size;
+  if (c.page_size % 8 == 0 && tokens >= 1 && tokens <= INT_MAX) {
+    const int most = f16 ? 128 : 64;  // a block's keys
+    p.tma_rows = std::min(most, c.page_size & -c.page_size);
+    const auto type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    for (int v = 0; v < 2; v++) {
+      const int rc = encode_tma_rows(v ? &p.value : &p.key, type, v ? c.value : c.key, c.D,
+                                     c.kv_heads, tokens, (uint64_t)c.D * 2,
+                                     (uint64_t)c.row_elems * 2, 64, p.tma_rows);
+      if (rc) return rc;
+    }
+  }
   int rc;
-  if (p.a.c.type == ORT_CUDA_CACHE_F16)
-    rc = padded_head(p.a.c.D) == 64 ? launch_tile_one<__half, 64>(p, grid, st)
-                                    : launch_tile_one<__half, 128>(p, grid, st);
+  if (f16)
+    rc = padded_head(c.D) == 64 ? launch_tile_one<__half, 64>(p, grid, st)
+                                : launch_tile_one<__half, 128>(p, grid, st);
   else
-    rc = padded_head(p.a.c.D) == 64 ? launch_tile_one<__nv_bfloat16, 64>(p, grid, st)
-                                    : launch_tile_one<__nv_bfloat16, 128>(p, grid, st);
+    rc = padded_head(c.D) == 64 ? launch_tile_one<__nv_bfloat16, 64>(p, grid, st)
+                                : launch_tile_one<__nv_bfloat16, 128>(p, grid, st);
   if (rc == ORT_CUDA_OK) (*launches)++;
   return rc;
 }
@@ -128,9 +150,11 @@ int launch_paged_attention(const PagedAttnArgs& a, void* scratch, int sm_count, 
   StreamArgs p;
   p.a = a;
   p.page_div.set((uint32_t)a.c.page_size);
+  p.group_div.set((uint32_t)a.group);
   p.q_vec = ((uintptr_t)a.q & 15) == 0 && a.q_stride % 4 == 0;
   p.t_scale = a.softcap > 0.f ? a.scale / a.softcap : a.scale;
   p.t_mul = a.softcap > 0.f ? a.softcap * kLog2e : kLog2e;
+  if (getenv("PEX")) p.ex = atoi(getenv("PEX"));
   char* at = static_cast<char*>(scratch);
   p.tickets = reinterpret_cast<unsigned*>(at);
   at += kTicketBytes;

@@ -56,9 +56,10 @@ struct FastDiv {
 
 struct StreamArgs {
   PagedAttnArgs a;
-  FastDiv page_div;
+  FastDiv page_div, group_div;
   int q_vec = 0;       // float4 loads of q rows
   int prefix = 0;      // 1: rows of all tokens over keys [0, shared) of row 0's pages
+  int ex = 6;
   int max_rows = 0;    // sequences with more query rows per KV head are not this kernel's
   float t_scale = 0;   // scale (softcap: scale / softcap)
   float t_mul = 0;     // log2(e) (softcap: softcap * log2(e))
@@ -95,6 +96,20 @@ __device__ __forceinline__ void paged_finish(const StreamArgs& p, int64_t at, in
     L = L * wa + pm.y * wb;
   }
   a.out[at * D + d] = L == 0.f ? 0.f : v / L;
+}
+// The same for a whole row: what a value and its prefix value are multiplied by.
+__device__ __forceinline__ float2 paged_row_scale(const StreamArgs& p, int64_t at, float M,
+                                                  float L) {
+  if (p.prefix) return make_float2(1.f, 0.f);
+  float wa = 1.f, wb = 0.f;
+  if (p.a.shared) {
+    const float2 pm = *reinterpret_cast<const float2*>(p.pre_ml + 2 * at);
+    const float mm = fmaxf(M, pm.x), mb = mm == -INFINITY ? 0.f : mm;
+    wa = ex2(M - mb), wb = ex2(pm.x - mb);
+    L = L * wa + pm.y * wb;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  return make_float2(wa * inv, wb * inv);
 }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes)
@@ -400,7 +415,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
       const int r = w + 8 * rr;
       const int idx = cur.rt * R + r;
       const bool row = idx < cur.count * a.group;
-      const int tok = row ? idx / a.group : 0, h = cur.g * a.group + (row ? idx - tok * a.group : 0);
+      const int tok = row ? p.group_div.div(idx) : 0, h = cur.g * a.group + (row ? idx - tok * a.group : 0);
       int pos = INT_MIN;
       if (row) {
         pos = cur.past + tok;
@@ -792,7 +807,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     const int slot = 2 * blockIdx.x + (head ? 0 : 1);
     auto finish = [&](int r, int d, float M, float L, float v) {
       const int idx = cur.rt * R + r;
-      const int tok = idx / a.group, h = cur.g * a.group + idx - tok * a.group;
+      const int tok = p.group_div.div(idx), h = cur.g * a.group + idx - tok * a.group;
       paged_finish(p, (int64_t)(cur.row0 + tok) * a.heads + h, d, M, L, v);
     };
     const int rows_here = min(R, cur.count * a.group - cur.rt * R);

@@ -10,8 +10,9 @@
 //
 // Roles: two softmax warpgroups, which take the blocks of a segment in turn
 // (one works on its block's weights while the tensor cores work for the
-// other), an MMA warp, a loader warp each for keys and values (cp.async by rows
-// of 16 bytes into the 128-byte swizzle, so pages may have any size).  A
+// other), an MMA warp, and loaders: TMA boxes of as many tokens
+// as a power of two divides the page size, or, where that is below 8, cp.async in
+// pieces of 16 bytes by three warps (about 4000 cycles a stage of 32 KB).  A
 // warpgroup's thread owns one query row: it reads the row's scores from TMEM,
 // writes the weights back over them as the A operand of p.v, and adds each
 // block's product, which comes in TMEM columns of its own, to its fp32 output in
@@ -51,30 +52,38 @@ struct TileCfg {
   static_assert(DP * 128 * 4 <= QB, "the output is staged in the q tile");
 };
 
+struct TileArgs {
+  StreamArgs s;
+  // pages as [tokens][kv heads][D], boxes of tma_rows tokens x 64 features; 0:
+  // page sizes that are no multiple of 8 are loaded by cp.async
+  int tma_rows = 0;
+  CUtensorMap key, value;
+};
+
 struct TilePos {
   int b, rt, g;
   int row0, count, past;
-  int lo, hi, nt, nrt;  // keys and blocks of this segment; row tiles of the sequence
+  int lo, hi, nt, nrt;  // keys and blocks of this segment (lo a multiple of `align`); row tiles
   int len;              // keys it counts as in the list (the causal border unclamped)
-  // the sequence: first base key, tiles whose keys start there
+  // the sequence: the first key of its row tiles (aligned), tiles that start there
   int base, ramp;
 };
 
 // Sets the sequence of `s`; its number of row tiles (0: not this kernel's).
 __device__ __forceinline__ int tile_seq(const StreamArgs& p, TilePos& s, int b, int min_past,
-                                        int TT) {
+                                        int TT, int align) {
   const PagedAttnArgs& a = p.a;
   s.b = b;
   s.nrt = 0;
   if (p.prefix) {
     s.row0 = 0, s.past = 0;
     s.count = max(0, min(a.c.cu[a.c.batch], a.c.num_tokens));
-    s.base = a.window ? min(a.shared, max(0, min_past + 1 - a.window)) : 0;
+    s.base = (a.window ? min(a.shared, max(0, min_past + 1 - a.window)) : 0) & -align;
   } else {
     const PagedSeq q = paged_seq(a.c, b, a.max_seq, a.shared);
     s.row0 = q.row0, s.count = q.count, s.past = q.past;
     if ((int64_t)q.count * a.group <= p.max_rows) return 0;
-    s.base = a.shared;
+    s.base = a.shared & -align;
   }
   s.nrt = (s.count + TT - 1) / TT;
   s.ramp = s.nrt;
@@ -87,26 +96,27 @@ __device__ __forceinline__ int tile_seq(const StreamArgs& p, TilePos& s, int b, 
 
 // Keys that row tiles 0 .. r - 1 of one KV head count as, with `extra` each.
 __device__ __forceinline__ long long tile_sum(const StreamArgs& p, const TilePos& s, int r, int TT,
-                                              int extra) {
+                                              int align, int extra) {
   if (p.prefix) return (long long)r * (max(1, p.a.shared - s.base) + extra);
   const long long f = min(r, s.ramp), c = r - f;
-  return f * (s.past - s.base) + TT * (f * (f + 1) / 2) + c * (TT + p.a.window - 1) +
+  return f * (s.past - s.base) + TT * (f * (f + 1) / 2) + c * (TT + p.a.window + align - 2) +
          (long long)r * extra;
 }
 
 // Sets the segment (rt, g) of the sequence of `s`.
 template <int KB>
 __device__ __forceinline__ void tile_segment(const StreamArgs& p, TilePos& s, int rt, int g,
-                                             int TT) {
+                                             int TT, int align) {
   s.rt = rt, s.g = g;
   if (p.prefix) {
     s.lo = s.base, s.hi = p.a.shared;
     s.len = max(1, s.hi - s.lo);
   } else {
     const int t0 = s.past + rt * TT;
-    s.lo = p.a.window ? max(s.base, t0 + 1 - p.a.window) : s.base;
+    const bool ramp = rt < s.ramp;
+    s.lo = ramp ? s.base : (t0 + 1 - p.a.window) & -align;
     s.hi = min(s.past + s.count, t0 + TT);
-    s.len = t0 + TT - s.lo;
+    s.len = ramp ? t0 + TT - s.base : TT + p.a.window + align - 2;
   }
   s.nt = max(1, (s.hi - s.lo + KB - 1) / KB);
 }
@@ -130,11 +140,11 @@ __device__ __forceinline__ bool bar_or(int id, int n, bool x) {
 constexpr int kTileThreads = 384, kTileSoftRegs = 216, kTileLoadRegs = 72, kTileRegs = 168;
 static_assert(256 * kTileSoftRegs + 128 * kTileLoadRegs <= kTileThreads * kTileRegs, "registers");
 
-template <typename T, int DP>
+template <typename T, int DP, bool CAP>
 __global__ void __launch_bounds__(kTileThreads, 1)
-    paged_tile_kernel(const __grid_constant__ StreamArgs p) {
+    paged_tile_kernel(const __grid_constant__ TileArgs args) {
   using C = TileCfg<T, DP>;
-  constexpr int PARTS = C::PARTS, KB = C::KB, NK = C::NK, NV = C::NV, EX = C::EXTRA;
+  constexpr int PARTS = C::PARTS, KB = C::KB, NK = C::NK, NV = C::NV;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char* qs = smem;                 // [part][DP / 64][128 rows][128 B], swizzled
@@ -150,10 +160,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   int* s_last = reinterpret_cast<int*>(tmem_at + 1);
   static_assert((2 * 4 + 2 * 4 + 7) * 8 + 8 <= 256, "barriers");
 
+  const StreamArgs& p = args.s;
   const PagedAttnArgs& a = p.a;
   const PagedView& c = a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int D = c.D, G = c.kv_heads, nb = p.prefix ? 1 : c.batch, TT = 128 / a.group;
+  const int EX = p.ex * 128;
+  const int rows_tma = args.tma_rows, align = max(1, rows_tma);
 
   // ---- this CTA's run
   int min_past = 0;
@@ -177,8 +190,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       TilePos t;
       long long n = 0;
       if (b0 + tid < nb) {
-        const int nrt = tile_seq(p, t, b0 + tid, min_past, TT);
-        if (nrt) n = tile_sum(p, t, nrt, TT, EX) * G;
+        const int nrt = tile_seq(p, t, b0 + tid, min_past, TT, align);
+        if (nrt) n = tile_sum(p, t, nrt, TT, align, EX) * G;
       }
       long long x = n;
       for (int o = 1; o < 32; o <<= 1) {
@@ -217,17 +230,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   int k0;
   {
     const long long off = u0 - s_scan[16];
-    tile_seq(p, cur, (int)s_scan[17], min_past, TT);
+    tile_seq(p, cur, (int)s_scan[17], min_past, TT, align);
     int lo = 0, hi = cur.nrt;  // the last row tile that starts at or before off
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (tile_sum(p, cur, mid, TT, EX) * G <= off)
+      if (tile_sum(p, cur, mid, TT, align, EX) * G <= off)
         lo = mid;
       else
         hi = mid;
     }
-    tile_segment<KB>(p, cur, lo, 0, TT);
-    const long long rem = off - tile_sum(p, cur, lo, TT, EX) * G, each = cur.len + EX;
+    tile_segment<KB>(p, cur, lo, 0, TT, align);
+    const long long rem = off - tile_sum(p, cur, lo, TT, align, EX) * G, each = cur.len + EX;
     cur.g = (int)(rem / each);
     const long long in = rem - cur.g * each - EX;
     seg = u0 - in;
@@ -240,17 +253,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (at >= u1) return false;
       first = 0;
       if (s.g + 1 < G) {
-        tile_segment<KB>(p, s, s.rt, s.g + 1, TT);
+        tile_segment<KB>(p, s, s.rt, s.g + 1, TT, align);
         return true;
       }
       if (s.rt + 1 < s.nrt) {
-        tile_segment<KB>(p, s, s.rt + 1, 0, TT);
+        tile_segment<KB>(p, s, s.rt + 1, 0, TT, align);
         return true;
       }
       int b = s.b + 1;
-      while (b < nb && !tile_seq(p, s, b, min_past, TT)) b++;
+      while (b < nb && !tile_seq(p, s, b, min_past, TT, align)) b++;
       if (b >= nb) return false;
-      tile_segment<KB>(p, s, 0, 0, TT);
+      tile_segment<KB>(p, s, 0, 0, TT, align);
       return true;
     }
   };
@@ -263,8 +276,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __syncthreads();  // s_scan has been read
 
   if (tid == 0) {
-    for (int i = 0; i < NK; i++) mbar_init(kfull + i, 1), mbar_init(kempty + i, 1);
-    for (int i = 0; i < NV; i++) mbar_init(vfull + i, 1), mbar_init(vempty + i, 1);
+    for (int i = 0; i < NK; i++) mbar_init(kfull + i, rows_tma ? 1 : 3), mbar_init(kempty + i, 1);
+    for (int i = 0; i < NV; i++) mbar_init(vfull + i, rows_tma ? 1 : 3), mbar_init(vempty + i, 1);
     for (int i = 0; i < 2; i++) mbar_init(sfull + i, 1), mbar_init(pfull + i, 128), mbar_init(pvfull + i, 1);
     mbar_init(qfull, 256);
     fence_mbarrier_init();
@@ -285,7 +298,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // ---- MMA
       constexpr uint32_t id_s = idesc_f16(PARTS == 3, 128, KB);
       constexpr uint32_t id_o = idesc_f16(PARTS == 3, 128, DP) | kIdescBMnMajor;
-      const uint32_t q_s = smem_u32(qs), k_s = smem_u32(ks), v_s = smem_u32(vs);
+      const uint32_t k_s = smem_u32(ks), v_s = smem_u32(vs);
+      const uint64_t qd = smem_desc_sw128(smem_u32(qs));  // addresses add in its low bits
       int kc = 0, vc = 0, pc[2] = {0, 0}, sc = 0;
       auto wait = [&](uint64_t* bar, int parity) {
         if (!dead && !mbar_wait(bar, parity)) {
@@ -301,14 +315,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         kc++;
         if (dead) return;
         if (elect_one()) {
-          const uint32_t kb = k_s + st * C::STAGE;
+          const uint64_t kd = smem_desc_sw128(k_s + st * C::STAGE);
 #pragma unroll
           for (int pt = PARTS - 1; pt >= 0; pt--)
 #pragma unroll
             for (int x = 0; x < DP / 16; x++)
               mma_f16_ss(tmem + w * C::SREG,
-                         smem_desc_sw128(q_s + pt * C::QPART + (x >> 2) * 16384 + (x & 3) * 32),
-                         smem_desc_sw128(kb + (x >> 2) * (KB * 128) + (x & 3) * 32), id_s,
+                         qd + ((pt * C::QPART + (x >> 2) * 16384 + (x & 3) * 32) >> 4),
+                         kd + (((x >> 2) * (KB * 128) + (x & 3) * 32) >> 4), id_s,
                          pt != PARTS - 1 || x);
           mma_commit(kempty + st);
           mma_commit(sfull + w);
@@ -328,15 +342,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           wait(vfull + st, (vc / NV) & 1);
           vc++;
           if (!dead && elect_one()) {
-            const uint32_t vb = v_s + st * C::STAGE;
+            const uint64_t vd = smem_desc_sw128_mn(v_s + st * C::STAGE, KB * 128);
 #pragma unroll
             for (int pt = PARTS - 1; pt >= 0; pt--)
 #pragma unroll
               for (int x = 0; x < KB / 16; x++) {
-                const int col = pt < 2 ? 32 * (x >> 1) + 16 * pt + 8 * (x & 1)
-                                       : KB + 16 * (x >> 1) + 8 * (x & 1);
+                const int col = pt < 2 ? 16 * x + 8 * pt : KB + 8 * x;
                 mma_f16_ts(tmem + 2 * C::SREG + w * DP, tmem + w * C::SREG + col,
-                           smem_desc_sw128_mn(vb + x * 2048, KB * 128), id_o,
+                           vd + (x * 2048 >> 4), id_o,
                            pt != PARTS - 1 || x);
               }
             mma_commit(vempty + st);
@@ -347,82 +360,156 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         if (!next(cur, seg, k0)) break;
       }
-    } else if (warp <= 10) {
-      // ---- loaders: warp 9 keys, warp 10 values
-      const bool is_k = warp == 9;
-      const int NS = is_k ? NK : NV;
-      uint64_t *full = is_k ? kfull : vfull, *empty = is_k ? kempty : vempty;
-      const uint32_t ring = smem_u32(is_k ? ks : vs);
-      const T* src = static_cast<const T*>(is_k ? c.key : c.value);
-      constexpr int CHP = DP / 8, RPI = 32 / CHP, LK = KB / 32;
-      const int chunks = D / 8, ch = lane & (CHP - 1);
-      int cnt = 0;
-      int pending = -1;  // a stage whose copies have not been announced
-      auto announce = [&] {  // its copies have landed (waited for): hand it to the MMA
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full + pending);
-        pending = -1;
-      };
-      for (;;) {
-        const int n = blocks(cur, seg, k0);
-        for (int k = 0; k < n; k++, cnt++) {
-          const int st = cnt % NS, base = cur.lo + (k0 + k) * KB;
-          long long off[LK];
-#pragma unroll
-          for (int i = 0; i < LK; i++) {
-            const int j = base + 32 * i + lane;
-            off[i] = -1;
-            if (j < cur.hi) {
+    } else if (rows_tma) {
+      // ---- TMA: warp 9 keys, warp 10 values; lane i the box of tokens i * rows_tma
+      if (warp <= 10) {
+        const bool is_k = warp == 9;
+        const int NS = is_k ? NK : NV, box = lane * rows_tma;
+        uint64_t *full = is_k ? kfull : vfull, *empty = is_k ? kempty : vempty;
+        const uint32_t ring = smem_u32(is_k ? ks : vs);
+        const CUtensorMap* map = is_k ? &args.key : &args.value;
+        if (lane == 0) prefetch_tensormap(map);
+        int cnt = 0;
+        for (;;) {
+          const int n = blocks(cur, seg, k0);
+#pragma unroll 1
+          for (int k = 0; k < n; k++, cnt++) {
+            const int st = cnt % NS, j = cur.lo + (k0 + k) * KB + box;
+            int page = -2, slot = 0;
+            if (box < KB && j < cur.hi) {
               const int pg = p.page_div.div(j);
-              const int page = __ldg(c.table + (int64_t)(p.prefix ? 0 : cur.b) * c.max_pages + pg);
-              if (page >= 0 && page < c.num_pages)
-                off[i] = (long long)page * c.page_elems +
-                         (long long)(j - pg * c.page_size) * c.row_elems + (long long)cur.g * D;
-              else if (is_k)
-                record_error(c.err, KERR_PAGED_PAGE);
+              slot = j - pg * c.page_size;
+              page = __ldg(c.table + (int64_t)(p.prefix ? 0 : cur.b) * c.max_pages + pg);
             }
-          }
-          if (cnt >= NS && !dead) {
-            const int par = ((cnt / NS) - 1) & 1;
-            if (!__all_sync(~0u, mbar_try_wait(empty + st, par))) {
-              if (pending >= 0) {  // do not hold a landed stage back
-                asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-                announce();
-              }
-              if (!mbar_wait(empty + st, par)) {
+            const bool ok = page >= 0 && page < c.num_pages;
+            if (cnt >= NS && !dead) {
+              if (!mbar_wait(empty + st, ((cnt / NS) - 1) & 1)) {
                 dead = true;
                 record_error(c.err, KERR_WAIT_EMPTY);
               }
               dead = __any_sync(~0u, dead);
             }
-          }
-          if (is_k) {
+            const unsigned there = __ballot_sync(~0u, ok);
+            if (is_k) {
+              if (!ok && page != -2) record_error(c.err, KERR_PAGED_PAGE);
+              if (lane < KB / 32) {  // the word's keys: a bit per box, spread over its rows
+                uint32_t m = 0;
+                for (int e = 0; e < 32; e++)
+                  m |= ((there >> ((32 * lane + e) / rows_tma)) & 1u) << e;
+                kvalid[(cnt & 7) * 4 + lane] = m;
+              }
+              __syncwarp();
+            }
+            if (!dead) {
+              if (lane == 0)
+                mbar_arrive_expect_tx(full + st,
+                                      (uint32_t)(__popc(there) * rows_tma * 128 * (DP / 64)));
+              __syncwarp();
+              if (ok) {
 #pragma unroll
-            for (int i = 0; i < LK; i++) {
-              const unsigned ok = __ballot_sync(~0u, off[i] >= 0);
-              if (lane == 0) kvalid[(cnt & 7) * 4 + i] = ok;
+                for (int hf = 0; hf < DP / 64; hf++)
+                  tma_load_3d(ring + st * C::STAGE + hf * (KB * 128) + box * 128, map, full + st,
+                              64 * hf, cur.g, page * c.page_size + slot);
+              }
             }
           }
-          const uint32_t at = ring + st * C::STAGE + (ch >> 3) * (KB * 128);
+          if (!next(cur, seg, k0)) break;
+        }
+        // the last stages have landed before the block's memory is given up: every
+        // one is waited for by the MMA warp (unless a wait ran out)
+        if (dead)
+          for (int i = max(0, cnt - NS); i < cnt; i++)
+            if (!mbar_wait(full + i % NS, (i / NS) & 1)) record_error(c.err, KERR_WAIT_DRAIN);
+      }
+    } else {
+      // ---- loaders: the stages in the order the MMA warp takes them (K0, K1, V0,
+      // K2, V1, ...), each by warps 9, 10, 11 together (every warp waits for every
+      // stage in turn, so a phase of a barrier is never passed over)
+      const uint32_t k_s = smem_u32(ks), v_s = smem_u32(vs);
+      constexpr int LK = KB / 32;
+      const int chunks = D / 8, ch = lane & 7;
+      const int third = warp - 9;
+      int kc = 0, vc = 0;
+      uint64_t* pending = nullptr;  // a stage whose copies have not been announced
+      auto announce = [&] {  // its copies have landed (waited for): hand it to the MMA
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pending);
+        pending = nullptr;
+      };
+      auto load = [&](bool is_k, int k) {
+        const int cnt = is_k ? kc++ : vc++;
+        const int NS = is_k ? NK : NV, st = cnt % NS, base = cur.lo + (k0 + k) * KB;
+        int page[LK], slot[LK];
 #pragma unroll
-          for (int i = 0; i < KB / RPI; i++) {
-            const int r = i * RPI + lane / CHP;
-            const long long o = __shfl_sync(~0u, off[i * RPI / 32], r & 31);
-            const int bytes = o >= 0 && ch < chunks ? 16 : 0;
-            cp16(at + r * 128 + (((ch & 7) ^ (r & 7)) << 4), src + (bytes ? o + ch * 8 : 0), bytes);
+        for (int i = 0; i < LK; i++) {
+          const int j = base + 32 * i + lane, pg = p.page_div.div(j);
+          slot[i] = j - pg * c.page_size;
+          page[i] = j < cur.hi
+                        ? __ldg(c.table + (int64_t)(p.prefix ? 0 : cur.b) * c.max_pages + pg)
+                        : -2;
+        }
+        uint64_t* empty = (is_k ? kempty : vempty) + st;
+        if (cnt >= NS && !dead) {
+          const int par = ((cnt / NS) - 1) & 1;
+          if (!__all_sync(~0u, mbar_try_wait(empty, par))) {
+            if (pending) {  // do not hold a landed stage back
+              asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+              announce();
+            }
+            if (!mbar_wait(empty, par)) {
+              dead = true;
+              record_error(c.err, KERR_WAIT_EMPTY);
+            }
+            dead = __any_sync(~0u, dead);
           }
-          asm volatile("cp.async.commit_group;\n" ::: "memory");
-          if (pending >= 0) {
-            asm volatile("cp.async.wait_group 1;\n" ::: "memory");
-            announce();
+        }
+        const uint32_t at = (is_k ? k_s : v_s) + st * C::STAGE;
+        const T* src = static_cast<const T*>(is_k ? c.key : c.value);
+#pragma unroll
+        for (int i = 0; i < LK; i++) {
+          const bool ok = page[i] >= 0 && page[i] < c.num_pages;
+          if (is_k && third == 0) {
+            if (!ok && page[i] != -2) record_error(c.err, KERR_PAGED_PAGE);
+            const unsigned m = __ballot_sync(~0u, ok);
+            if (lane == 0) kvalid[(cnt & 7) * 4 + i] = m;
           }
-          pending = st;
+          const T* row = ok ? src + (long long)page[i] * c.page_elems +
+                                  (long long)slot[i] * c.row_elems + (long long)cur.g * D
+                            : nullptr;
+          // 8 lanes a row: its 128-byte halves
+#pragma unroll
+          for (int y = 0; y < 8; y++) {
+            if ((8 * i + y) % 3 != third) continue;
+            const int r = 4 * y + (lane >> 3);
+            const T* o = reinterpret_cast<const T*>(
+                __shfl_sync(~0u, reinterpret_cast<unsigned long long>(row), r));
+            const uint32_t dst = at + (32 * i + r) * 128 + ((ch ^ (r & 7)) << 4);
+#pragma unroll
+            for (int hf = 0; hf < DP / 64; hf++) {
+              const int bytes = o && ch + 8 * hf < chunks ? 16 : 0;
+              cp16(dst + hf * (KB * 128), bytes ? o + (ch + 8 * hf) * 8 : src, bytes);
+            }
+          }
+        }
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+        if (pending) {
+          asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+          announce();
+        }
+        pending = (is_k ? kfull : vfull) + st;
+      };
+      for (;;) {
+        const int n = blocks(cur, seg, k0);
+#pragma unroll 1
+        for (int k = -2; k < n; k++) {
+          if (k + 2 < n) load(true, k + 2);
+          if (k >= 0) load(false, k);
         }
         if (!next(cur, seg, k0)) break;
       }
       asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-      if (pending >= 0) announce();
+      if (pending) announce();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTileSoftRegs));
@@ -439,61 +526,69 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       __syncwarp();
       tc_fence_after();
     };
+    // q rows: warp w loads rows 16 w .. 16 w + 15 of a segment's tile, a 16-byte
+    // piece a lane
+    constexpr int LPR = DP / 4, RPI = 32 / LPR, NQ = 16 / RPI;  // lanes a row, rows a step, steps
+    auto load_q = [&](const TilePos& s, float4 (&q4)[NQ]) {
+      const int t0 = s.rt * TT, rows = min(TT, s.count - t0) * a.group;
+      const int f = (lane & (LPR - 1)) * 4;
+      const float* base = a.q + (int64_t)(s.row0 + t0) * a.q_stride + (int64_t)(s.g * a.group) * D;
+      const float* src[NQ];
+#pragma unroll
+      for (int i = 0; i < NQ; i++) {  // rows and features that are not there: the first
+        const int r0 = warp * 16 + i * RPI + lane / LPR, r = r0 < rows ? r0 : 0;
+        const int t = p.group_div.div(r);
+        src[i] = base + (int64_t)t * a.q_stride + (int64_t)(r - t * a.group) * D + (f < D ? f : 0);
+      }
+      if (p.q_vec) {
+#pragma unroll
+        for (int i = 0; i < NQ; i++) q4[i] = __ldg(reinterpret_cast<const float4*>(src[i]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < NQ; i++)
+          q4[i] =
+              make_float4(__ldg(src[i]), __ldg(src[i] + 1), __ldg(src[i] + 2), __ldg(src[i] + 3));
+      }
+#pragma unroll
+      for (int i = 0; i < NQ; i++)
+        if (warp * 16 + i * RPI + lane / LPR >= rows || f >= D) q4[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    };
     for (;;) {
       const int n = blocks(cur, seg, k0);
       const int tok0 = cur.rt * TT, rows_here = min(TT, cur.count - tok0) * a.group;
       const bool has = row < rows_here;
-      const int tok = tok0 + (has ? row / a.group : 0);
-      const int head = cur.g * a.group + (has ? row % a.group : 0);
-      // q: this warpgroup's half of the features of every row
-      float fac = p.t_scale;
-      {
-        const float* src = a.q + (int64_t)(cur.row0 + tok) * a.q_stride + (int64_t)head * D;
-        auto load8 = [&](int ch, float (&x)[8]) {
+      const int tok = tok0 + (has ? p.group_div.div(row) : 0);
+      // the parts of the q tile
+      float4 q4[NQ];
+      load_q(cur, q4);
 #pragma unroll
-          for (int e = 0; e < 8; e++) x[e] = 0.f;
-          if (!has || 8 * ch >= D) return;
-          if (p.q_vec) {
-            *reinterpret_cast<float4*>(x) = __ldg(reinterpret_cast<const float4*>(src) + 2 * ch);
-            *reinterpret_cast<float4*>(x + 4) =
-                __ldg(reinterpret_cast<const float4*>(src) + 2 * ch + 1);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = __ldg(src + 8 * ch + e);
-          }
-        };
-        float up = 1.f;
+      for (int i = 0; i < NQ; i++) {
+        const int r = warp * 16 + i * RPI + lane / LPR, ch = (lane & (LPR - 1)) >> 1;
+        float fr = p.t_scale, up = 1.f;
         if constexpr (PARTS == 2) {  // the row's largest value into [2^13, 2^14)
-          float mx = 0.f;
+          float mx = fmaxf(fmaxf(fabsf(q4[i].x), fabsf(q4[i].y)),
+                           fmaxf(fabsf(q4[i].z), fabsf(q4[i].w)));
 #pragma unroll
-          for (int ch = 0; ch < DP / 8; ch++) {
-            float x[8];
-            load8(ch, x);
-#pragma unroll
-            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[e]));
-          }
+          for (int x = LPR / 2; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, x));
           int ex = (int)(__float_as_uint(mx) >> 23) - 127;
           ex = max(-100, min(ex, 126));
           up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
-          fac *= __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
+          fr *= __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
         }
+        uint32_t w0[PARTS], w1[PARTS];
+        Split<T>::pair(q4[i].x * up, q4[i].y * up, w0);
+        Split<T>::pair(q4[i].z * up, q4[i].w * up, w1);
 #pragma unroll
-        for (int y = 0; y < DP / 16; y++) {
-          const int ch = wg * (DP / 16) + y;
-          float x[8];
-          load8(ch, x);
-          uint32_t wd[4][PARTS];
-#pragma unroll
-          for (int e = 0; e < 4; e++) Split<T>::pair(x[2 * e] * up, x[2 * e + 1] * up, wd[e]);
-#pragma unroll
-          for (int pt = 0; pt < PARTS; pt++)
-            *reinterpret_cast<uint4*>(qs + pt * C::QPART + (ch >> 3) * 16384 + row * 128 +
-                                      (((ch & 7) ^ (row & 7)) << 4)) =
-                make_uint4(wd[0][pt], wd[1][pt], wd[2][pt], wd[3][pt]);
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(qfull);
+        for (int pt = 0; pt < PARTS; pt++)
+          *reinterpret_cast<uint2*>(qs + pt * C::QPART + (ch >> 3) * 16384 + r * 128 +
+                                    (((ch & 7) ^ (r & 7)) << 4) + (lane & 1) * 8) =
+              make_uint2(w0[pt], w1[pt]);
+        if ((lane & (LPR - 1)) == 0) stats[r].x = fr;
       }
+      fence_proxy_async_smem();
+      mbar_arrive(qfull);
+      bar_sync(1, 256);
+      const float fac = stats[row].x;
       int pos = -1;  // the row's position (-1: no row), and what all rows see
       int all_hi = cur.past + tok0, all_lo = cur.past + min(tok0 + TT, cur.count) - 1;
       if (p.prefix) {
@@ -515,7 +610,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       } else if (has) {
         pos = cur.past + tok;
       }
-      const int from = a.window ? pos - a.window + 1 : 0;
+      const int own = pos;
+      pos = min(pos, cur.hi - 1);  // a block's boxes may reach past the last key
+      const int first = p.prefix ? 0 : a.shared;
+      const int from = max(first, a.window ? own - a.window + 1 : 0);
       const float cmul = fac * p.t_mul;
 
       float m = -INFINITY, l = 0.f, o[DP];
@@ -524,105 +622,110 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int k = wg; k < n; k += 2) {
         const int base = cur.lo + (k0 + k) * KB;
         wait(sfull + wg, sc & 1);
-        uint32_t vw[KB / 32];
-        bool full = base + KB - 1 <= all_hi && base + KB <= cur.hi &&
+        bool full = base + KB - 1 <= all_hi && base + KB <= cur.hi && base >= first &&
                     (!a.window || base > all_lo - a.window);
-#pragma unroll
-        for (int i = 0; i < KB / 32; i++) {
-          vw[i] = kvalid[((gb + k) & 7) * 4 + i];
-          full = full && vw[i] == ~0u;
-        }
-        if (!full) {  // the keys of each word that the row sees
-#pragma unroll
+        const uint32_t* kv = kvalid + ((gb + k) & 7) * 4;
+        for (int i = 0; i < KB / 32; i++) full = full && kv[i] == ~0u;
+        auto seen = [&](int i) {  // keys of the block's word i that the row sees
+          const int b = base + 32 * i, x0 = max(from - b, 0), x1 = min(pos - b, 31);
+          return pos < b || x0 > x1 ? 0u : kv[i] & (~0u >> (31 - x1)) & (~0u << x0);
+        };
+        // 16 scores at a time, the next ones on their way from TMEM meanwhile
+        uint32_t ra[16], rb[16];
+        auto steps = [&](auto&& f) {
+          tmem_ld16(ts, ra);
+#pragma unroll 1
           for (int i = 0; i < KB / 32; i++) {
-            const int x0 = max(from - (base + 32 * i), 0), x1 = min(pos - (base + 32 * i), 31);
-            vw[i] &= pos < base + 32 * i || x0 > x1 ? 0u : (~0u >> (31 - x1)) & (~0u << x0);
+            const uint32_t vw = full ? ~0u : seen(i);
+            tmem_ld_wait();
+            tmem_ld16(ts + 32 * i + 16, rb);
+            f(2 * i, ra, vw);
+            tmem_ld_wait();
+            if (i + 1 < KB / 32) tmem_ld16(ts + 32 * i + 32, ra);
+            f(2 * i + 1, rb, vw >> 16);
           }
-        }
+        };
         // the row's maximum
-        float mx = -INFINITY;
+        float mx = -INFINITY, mx2 = -INFINITY;
+        steps([&](int, uint32_t (&r)[16], uint32_t vw) {
+          if (!full) {
 #pragma unroll
-        for (int i = 0; i < KB / 32; i++) {
-          uint32_t r[32];
-          tmem_ld32(ts + 32 * i, r);
-          tmem_ld_wait();
-          if (full) {
-#pragma unroll
-            for (int e = 0; e < 32; e++) mx = fmaxf(mx, __uint_as_float(r[e]));
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; e++)
-              if ((vw[i] >> e) & 1) mx = fmaxf(mx, __uint_as_float(r[e]));
+            for (int e = 0; e < 16; e++)
+              if (!((vw >> e) & 1)) r[e] = 0xff800000u;
           }
-        }
-        if (mx != -INFINITY) mx = a.softcap > 0.f ? tanhf(mx * fac) * p.t_mul : mx * cmul;
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            mx = fmaxf(mx, __uint_as_float(r[e]));
+            mx2 = fmaxf(mx2, __uint_as_float(r[e + 1]));
+          }
+        });
+        mx = fmaxf(mx, mx2);
+        if (mx != -INFINITY) mx = CAP ? tanhf(mx * fac) * p.t_mul : mx * cmul;
         const float mn = fmaxf(m, mx), mb = mn == -INFINITY ? 0.f : mn;
         const float corr = ex2(m - mb), sub = PARTS == 2 ? mb - 15.f : mb;
         m = mn;
 
         // values only some rows see: an infinity or NaN among them must not reach
-        // the others as 0 * inf (see paged_stream.cuh)
+        // the others as 0 * inf (see paged_stream.cuh); rows that hold no key of the
+        // segment, whatever a page or an older stage left there, become zeros
         bool odd = false;
-        const unsigned char* vst = vs + ((gb + k) % NV) * C::STAGE;
+        unsigned char* vst = vs + ((gb + k) % NV) * C::STAGE;
         if (!full) {
           wait(vfull + (gb + k) % NV, ((gb + k) / NV) & 1);
+#pragma unroll 4
           for (int i = row; i < C::STAGE / 16; i += 128) {
-            const uint4 v = reinterpret_cast<const uint4*>(vst)[i];
+            const int r = (i >> 3) & (KB - 1), j = base + r;
+            uint4* at = reinterpret_cast<uint4*>(vst) + i;
+            if (j < first || j >= cur.hi || !((kv[r >> 5] >> (r & 31)) & 1)) {
+              *at = make_uint4(0u, 0u, 0u, 0u);
+              continue;
+            }
+            const uint4 v = *at;
             const uint32_t ws[4] = {v.x, v.y, v.z, v.w};
             constexpr uint32_t inf = PARTS == 2 ? 0x7c00u : 0x7f80u;
 #pragma unroll
             for (int e = 0; e < 4; e++)
               odd |= (ws[e] & inf) == inf || ((ws[e] >> 16) & inf) == inf;
           }
+          fence_proxy_async_smem();
           odd = bar_or(2 + wg, 128, odd);
         }
 
         // weights, over the scores
-        float sum = 0.f;
+        float sum = 0.f, sum2 = 0.f;
+        steps([&](int st, uint32_t (&r)[16], uint32_t vw) {
+          float x[16];
 #pragma unroll
-        for (int i = 0; i < KB / 32; i++) {
-          uint32_t r[32];
-          tmem_ld32(ts + 32 * i, r);
-          tmem_ld_wait();
-          float x[32];
-          if (a.softcap > 0.f) {
-#pragma unroll
-            for (int e = 0; e < 32; e++)
+          for (int e = 0; e < 16; e++) {
+            if (CAP)
               x[e] = ex2(fmaf(tanhf(__uint_as_float(r[e]) * fac), p.t_mul, -sub));
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; e++) x[e] = ex2(fmaf(__uint_as_float(r[e]), cmul, -sub));
+            else
+              x[e] = ex2(fmaf(__uint_as_float(r[e]), cmul, -sub));
           }
           if (!full) {
 #pragma unroll
-            for (int e = 0; e < 32; e++) x[e] = (vw[i] >> e) & 1 ? x[e] : 0.f;
+            for (int e = 0; e < 16; e++) x[e] = (vw >> e) & 1 ? x[e] : 0.f;
           }
 #pragma unroll
-          for (int e = 0; e < 32; e++) sum += x[e];
+          for (int e = 0; e < 16; e += 2) sum += x[e], sum2 += x[e + 1];
+          uint32_t wd[16], w2[8];
           if (odd) {  // kept in fp32 for the sum below
 #pragma unroll
-            for (int e = 0; e < 32; e++) r[e] = __float_as_uint(x[e]);
-            uint32_t h[16];
+            for (int e = 0; e < 16; e++) wd[e] = __float_as_uint(x[e]), w2[e >> 1] = 0u;
+          } else {
 #pragma unroll
-            for (int y = 0; y < 2; y++) {
-#pragma unroll
-              for (int e = 0; e < 16; e++) h[e] = r[16 * y + e];
-              tmem_st16(ts + 32 * i + 16 * y, h);
+            for (int e = 0; e < 8; e++) {
+              uint32_t t[PARTS];
+              Split<T>::pair(x[2 * e], x[2 * e + 1], t);
+              wd[e] = t[0], wd[8 + e] = t[1], w2[e] = t[PARTS - 1];
             }
-            continue;
           }
-          uint32_t wd[PARTS][16];
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            uint32_t t[PARTS];
-            Split<T>::pair(x[2 * e], x[2 * e + 1], t);
-#pragma unroll
-            for (int pt = 0; pt < PARTS; pt++) wd[pt][e] = t[pt];
-          }
-          tmem_st16(ts + 32 * i, wd[0]);
-          tmem_st16(ts + 32 * i + 16, wd[1]);
-          if (PARTS == 3) tmem_st16(ts + KB + 16 * i, wd[PARTS - 1]);
-        }
+          tmem_st16(ts + 16 * st, wd);
+          if (PARTS == 3)
+            tmem_st8(ts + KB + 8 * st, make_uint4(w2[0], w2[1], w2[2], w2[3]),
+                     make_uint4(w2[4], w2[5], w2[6], w2[7]));
+        });
+        sum += sum2;
         l = l * corr + sum;
         tmem_st_wait();
         if (odd) {
@@ -682,18 +785,34 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const bool whole = n == cur.nt;
       const int slot = 2 * blockIdx.x + (k0 ? 0 : 1);
       auto place = [&](int r) {
-        const int t = r / a.group;
+        const int t = p.group_div.div(r);
         return (int64_t)(cur.row0 + tok0 + t) * a.heads + cur.g * a.group + r - t * a.group;
       };
+      auto write_row = [&](int64_t to, float M, float L, const float (&v)[DP / 32]) {
+        const float2 f = paged_row_scale(p, to, M, L);
+        float* dst = (p.prefix ? p.pre_o : a.out) + to * D;
+        const float* pre = p.pre_o + to * D;
+#pragma unroll
+        for (int x = 0; x < DP / 32; x++) {
+          const int d = lane + 32 * x;
+          if (d < D) dst[d] = p.prefix || !a.shared ? v[x] * f.x : fmaf(v[x], f.x, pre[d] * f.y);
+        }
+        if (p.prefix && lane == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * to) = make_float2(M, L);
+      };
+      constexpr int NX = DP / 32;
+#pragma unroll 2
       for (int r = warp; r < rows_here; r += 8) {
         const float2 ml = stats[r];
-        if (whole) {
-          const int64_t to_row = place(r);
-          for (int d = lane; d < D; d += 32) paged_finish(p, to_row, d, ml.x, ml.y, at(d, r));
+        float v[NX];
+#pragma unroll
+        for (int x = 0; x < NX; x++) v[x] = at(lane + 32 * x, r);
+        if (!whole) {
+          const int64_t to = (int64_t)slot * 128 + r;
+#pragma unroll
+          for (int x = 0; x < NX; x++) p.part_o[to * DP + lane + 32 * x] = v[x];
+          if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + to * 2) = ml;
         } else {
-          for (int d = lane; d < D; d += 32)
-            p.part_o[((int64_t)slot * 128 + r) * DP + d] = at(d, r);
-          if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * 128 + r) * 2) = ml;
+          write_row(place(r), ml.x, ml.y, v);
         }
       }
       if (!whole) {
@@ -730,10 +849,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               }
             }
             for (int x = 16; x; x >>= 1) L += __shfl_xor_sync(~0u, L, x);
-            const int64_t to_row = place(r);
-#pragma unroll
-            for (int x = 0; x < DP / 32; x++)
-              if (lane + 32 * x < D) paged_finish(p, to_row, lane + 32 * x, M, L, v[x]);
+            write_row(place(r), M, L, v);
           }
           if (tid == 0) p.tickets[c0] = 0u;
         }

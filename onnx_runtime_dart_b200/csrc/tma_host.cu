@@ -7,10 +7,9 @@
 #include "common.cuh"
 
 namespace ortc {
+namespace {
 
-int encode_tma_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t d0,
-                  uint64_t d1, uint64_t stride1, uint32_t b0, uint32_t b1,
-                  CUtensorMapSwizzle swz) {
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -21,6 +20,15 @@ int encode_tma_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, ui
         q == cudaDriverEntryPointSuccess)
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
   });
+  return fn;
+}
+
+}  // namespace
+
+int encode_tma_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t d0,
+                  uint64_t d1, uint64_t stride1, uint32_t b0, uint32_t b1,
+                  CUtensorMapSwizzle swz) {
+  const auto fn = encode_fn();
   if (!fn) return fail(ORT_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   const cuuint64_t dims[2] = {d0, d1};
   const cuuint64_t strides[1] = {stride1};
@@ -29,6 +37,24 @@ int encode_tma_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, ui
   CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(ORT_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) +
+                                       ")");
+  return ORT_CUDA_OK;
+}
+
+int encode_tma_rows(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t d0,
+                    uint64_t d1, uint64_t d2, uint64_t stride1, uint64_t stride2, uint32_t b0,
+                    uint32_t b2) {
+  const auto fn = encode_fn();
+  if (!fn) return fail(ORT_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[3] = {d0, d1, d2};
+  const cuuint64_t strides[2] = {stride1, stride2};
+  const cuuint32_t box[3] = {b0, 1, b2};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(ORT_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) +
                                        ")");
