@@ -152,9 +152,9 @@ int launch_paged_attention(const PagedAttnArgs& a, void* scratch, int sm_count, 
   p.page_div.set((uint32_t)a.c.page_size);
   p.group_div.set((uint32_t)a.group);
   p.q_vec = ((uintptr_t)a.q & 15) == 0 && a.q_stride % 4 == 0;
+  p.out_vec = ((uintptr_t)a.out & 15) == 0;
   p.t_scale = a.softcap > 0.f ? a.scale / a.softcap : a.scale;
   p.t_mul = a.softcap > 0.f ? a.softcap * kLog2e : kLog2e;
-  if (getenv("PEX")) p.ex = atoi(getenv("PEX"));
   char* at = static_cast<char*>(scratch);
   p.tickets = reinterpret_cast<unsigned*>(at);
   at += kTicketBytes;

@@ -57,9 +57,8 @@ struct FastDiv {
 struct StreamArgs {
   PagedAttnArgs a;
   FastDiv page_div, group_div;
-  int q_vec = 0;       // float4 loads of q rows
+  int q_vec = 0, out_vec = 0;  // 16-byte loads of q rows, stores of out
   int prefix = 0;      // 1: rows of all tokens over keys [0, shared) of row 0's pages
-  int ex = 6;
   int max_rows = 0;    // sequences with more query rows per KV head are not this kernel's
   float t_scale = 0;   // scale (softcap: scale / softcap)
   float t_mul = 0;     // log2(e) (softcap: softcap * log2(e))
@@ -76,28 +75,8 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Writes feature d of (token, head) `at` from its maximum, sum and unnormalised
-// value: the output, joined with what the prefix pass left, or, in the prefix
-// pass, that.
-__device__ __forceinline__ void paged_finish(const StreamArgs& p, int64_t at, int d, float M,
-                                             float L, float v) {
-  const PagedAttnArgs& a = p.a;
-  const int D = a.c.D;
-  if (p.prefix) {
-    p.pre_o[at * D + d] = v;
-    if (d == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * at) = make_float2(M, L);
-    return;
-  }
-  if (a.shared) {
-    const float2 pm = *reinterpret_cast<const float2*>(p.pre_ml + 2 * at);
-    const float mm = fmaxf(M, pm.x), mb = mm == -INFINITY ? 0.f : mm;
-    const float wa = ex2(M - mb), wb = ex2(pm.x - mb);
-    v = v * wa + p.pre_o[at * D + d] * wb;
-    L = L * wa + pm.y * wb;
-  }
-  a.out[at * D + d] = L == 0.f ? 0.f : v / L;
-}
-// The same for a whole row: what a value and its prefix value are multiplied by.
+// What a row's unnormalised values, and those that the prefix pass left, are
+// multiplied by, from the row's maximum and sum.
 __device__ __forceinline__ float2 paged_row_scale(const StreamArgs& p, int64_t at, float M,
                                                   float L) {
   if (p.prefix) return make_float2(1.f, 0.f);
@@ -195,14 +174,14 @@ struct StreamCfg {
   static constexpr int QP = R == 8 ? (Split<T>::PARTS + 1) / 2 : Split<T>::PARTS;
   static constexpr int QB = QP * KS * 512;
   static constexpr int RING = 8 * NS * WSTAGE;
-  static constexpr int JOIN = 8 * 8 * 64 * 4;       // [warp][8 rows][64 features]
-  // A segment's start and end (its operands, the join of the warps) cost about
-  // as much as three 64 KB tiles; the list counts them, so that a run of many
-  // short sequences is no longer than one of a long sequence.  Measured on 64
-  // sequences of 100 to 8191 keys: 113 us uncounted, 103, 93, 84.6, 85, 89 at
-  // 1, 2, 3, 4, 6.
-  static constexpr int EXTRA = 3 * 128 / DP;
-  static constexpr int SMEM = RING + QB + JOIN + 8 * R * 8;  // + (max, sum) per warp and row
+  // A segment's start and end cost about as much as two 64 KB tiles; the list
+  // counts them, so that a run of many short sequences is no longer than one of a
+  // long sequence.  Measured at 1, 2, 3 tiles: 64 sequences of 100 to 8191 keys 86.2,
+  // 82.1, 84.0 us (uncounted 113), one of 131000 keys 95.8, 94.8, 94.8 us.
+  static constexpr int EXTRA = 2 * 128 / DP;
+  static_assert(R * DP * 4 <= WSTAGE, "a warp's output is handed over in its free stage");
+  // the ring, two sets of operands, (max, sum) per warp and row
+  static constexpr int SMEM = RING + 2 * QB + 8 * R * 8;
 };
 
 // Where a CTA is in the list of tiles: tile `tile` of segment (b, rt, g).
@@ -240,6 +219,33 @@ __device__ __forceinline__ int stream_seq(const StreamArgs& p, StreamPos& s, int
   return (s.nt + EXTRA) * s.nrt;
 }
 
+// Writes features d .. d + 3 of query row idx of a segment's sequence and KV head
+// (D is a multiple of 8): the output, joined with what the prefix pass left, or, in
+// the prefix pass, that.
+__device__ __forceinline__ void stream_finish(const StreamArgs& p, const StreamPos& s, int idx,
+                                              int d, float M, float L, float4 v) {
+  const PagedAttnArgs& a = p.a;
+  const int tok = p.group_div.div(idx), h = s.g * a.group + idx - tok * a.group, D = a.c.D;
+  const int64_t at = (int64_t)(s.row0 + tok) * a.heads + h;
+  if (p.prefix) {
+    *reinterpret_cast<float4*>(p.pre_o + at * D + d) = v;
+    if (d == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * at) = make_float2(M, L);
+    return;
+  }
+  const float2 f = paged_row_scale(p, at, M, L);
+  v.x *= f.x, v.y *= f.x, v.z *= f.x, v.w *= f.x;
+  if (a.shared) {
+    const float4 t = *reinterpret_cast<const float4*>(p.pre_o + at * D + d);
+    v.x = fmaf(t.x, f.y, v.x), v.y = fmaf(t.y, f.y, v.y);
+    v.z = fmaf(t.z, f.y, v.z), v.w = fmaf(t.w, f.y, v.w);
+  }
+  float* dst = a.out + at * D + d;
+  if (p.out_vec)
+    *reinterpret_cast<float4*>(dst) = v;
+  else
+    dst[0] = v.x, dst[1] = v.y, dst[2] = v.z, dst[3] = v.w;
+}
+
 template <typename T, int DP, int R>
 __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_constant__ StreamArgs p) {
   using C = StreamCfg<T, DP, R>;
@@ -249,15 +255,13 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
   constexpr int NR = R / 8;            // rows a lane holds
   extern __shared__ __align__(128) unsigned char smem[];
   unsigned char* ring = smem;
-  uint4* qf = reinterpret_cast<uint4*>(smem + C::RING);  // [QP][KS][32]
-  float* join = reinterpret_cast<float*>(smem + C::RING + C::QB);
-  float2* wml = reinterpret_cast<float2*>(smem + C::RING + C::QB + C::JOIN);  // [8][R]
+  uint4* qf = reinterpret_cast<uint4*>(smem + C::RING);  // [2][QP][KS][32]: segments in turn
+  float2* wml = reinterpret_cast<float2*>(smem + C::RING + 2 * C::QB);  // [8][R]
   __shared__ long long s_scan[8];
   __shared__ long long s_u0base;
   __shared__ int s_b0, s_min[8], s_last;
-  __shared__ float s_fac[R];   // score factor of a row
-  __shared__ int s_pos[R];     // position of a row, INT_MIN: no row
-  __shared__ float2 s_ml[R];   // the segment's maximum and sum
+  __shared__ float s_fac[2][R];   // score factor of a row
+  __shared__ int s_pos[2][R];     // position of a row, INT_MIN: no row
 
   const PagedAttnArgs& a = p.a;
   const PagedView& c = a.c;
@@ -404,21 +408,50 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     commit();
   }
 
-  // ---- segments
-  int stage = 0;
-  for (;;) {
-    const int n = (int)min((long long)cur.nt, u1 - seg_u) - cur.tile;  // tiles of it in this run
-    // q rows: warp w builds rows w, w + 8 of the A operands
-    __syncthreads();  // the last segment's operands are no longer read
+  // ---- q rows: warp w brings rows w, w + 8 of a segment's tile into registers and,
+  // later, as A operands into one of the two sets
+  constexpr int E = DP / 32;  // features of a lane
+  float qx[NR][E];
+  auto row_of = [&](const StreamPos& s, int r, int& tok, int& h) {
+    const int idx = s.rt * R + r;
+    const bool row = idx < s.count * a.group;
+    tok = row ? p.group_div.div(idx) : 0;
+    h = s.g * a.group + (row ? idx - tok * a.group : 0);
+    return row;
+  };
+  auto load_q = [&](const StreamPos& s) {
+#pragma unroll
+    for (int rr = 0; rr < NR; rr++) {
+      int tok, h;
+      const bool row = row_of(s, w + 8 * rr, tok, h);
+      const float* src = a.q + (int64_t)(s.row0 + tok) * a.q_stride + (int64_t)h * D;
+#pragma unroll
+      for (int e = 0; e < E; e++) qx[rr][e] = 0.f;
+      if (!row) continue;
+      if (E == 4 && p.q_vec && 4 * lane + 3 < D) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(src) + lane);
+        qx[rr][0] = v.x, qx[rr][1] = v.y, qx[rr][E - 2] = v.z, qx[rr][E - 1] = v.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          if (E * lane + e < D) qx[rr][e] = __ldg(src + E * lane + e);
+      }
+    }
+  };
+  auto build_q = [&](const StreamPos& s, int set) {
+    uint32_t* qw = reinterpret_cast<uint32_t*>(qf + set * (C::QB / 16));
+    // word `reg` of k-step s of part pt for MMA lane ml
+    auto put = [&](int pt, int s, int ml, int reg, uint32_t v) {
+      qw[(((pt * KS + s) * 32) + ml) * 4 + reg] = v;
+    };
 #pragma unroll
     for (int rr = 0; rr < NR; rr++) {
       const int r = w + 8 * rr;
-      const int idx = cur.rt * R + r;
-      const bool row = idx < cur.count * a.group;
-      const int tok = row ? p.group_div.div(idx) : 0, h = cur.g * a.group + (row ? idx - tok * a.group : 0);
+      int tok, h;
+      const bool row = row_of(s, r, tok, h);
       int pos = INT_MIN;
       if (row) {
-        pos = cur.past + tok;
+        pos = s.past + tok;
         if (p.prefix) {
           pos = INT_MAX / 2;  // past the prefix
           if (a.window) {
@@ -427,20 +460,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
           }
         }
       }
-      float x[DP / 32];
-      const float* src = a.q + (int64_t)(cur.row0 + tok) * a.q_stride + (int64_t)h * D;
-      constexpr int E = DP / 32;  // features of a lane, E at a time
-#pragma unroll
-      for (int e = 0; e < E; e++) x[e] = 0.f;
-      if (row) {
-        if (E == 4 && p.q_vec && 4 * lane + 3 < D) {
-          *reinterpret_cast<float4*>(x) = __ldg(reinterpret_cast<const float4*>(src) + lane);
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; e++)
-            if (E * lane + e < D) x[e] = __ldg(src + E * lane + e);
-        }
-      }
+      float(&x)[E] = qx[rr];
       float fac = p.t_scale;
       if constexpr (!F32 && PARTS == 2) {  // fp16: the row's largest value into [2^13, 2^14)
         float mx = 0.f;
@@ -455,14 +475,9 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
         fac *= __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
       }
       if (lane == 0) {
-        s_fac[r] = fac;
-        s_pos[r] = pos;
+        s_fac[set][r] = fac;
+        s_pos[set][r] = pos;
       }
-      uint32_t* qw = reinterpret_cast<uint32_t*>(qf);
-      // word `reg` of k-step s of part pt for MMA lane ml
-      auto put = [&](int pt, int s, int ml, int reg, uint32_t v) {
-        qw[(((pt * KS + s) * 32) + ml) * 4 + reg] = v;
-      };
 #pragma unroll
       for (int e = 0; e < E; e += 2) {
         const int d = E * lane + e;
@@ -493,14 +508,30 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
         }
       }
     }
-    __syncthreads();
+  };
+
+  // ---- segments
+  int stage = 0, set = 0;
+  load_q(cur);
+  build_q(cur, 0);
+  __syncthreads();
+  for (;;) {
+    const int n = (int)min((long long)cur.nt, u1 - seg_u) - cur.tile;  // tiles of it in this run
+    const bool more = seg_u + cur.nt + EXTRA < u1;
+    StreamPos nx = cur;  // the next segment: its q rows come while this one's keys do
+    if (more) {
+      nx.tile = nx.nt - 1;
+      advance(nx);
+      load_q(nx);
+    }
+    const uint4* qs = qf + set * (C::QB / 16);
     float fac[NR];
     int pos[NR];
     int pos_lo = INT_MAX, pos_hi = INT_MIN;  // over the tile's rows
 #pragma unroll
     for (int rr = 0; rr < NR; rr++) {
-      fac[rr] = s_fac[(lane >> 2) + 8 * rr];
-      pos[rr] = s_pos[(lane >> 2) + 8 * rr];
+      fac[rr] = s_fac[set][(lane >> 2) + 8 * rr];
+      pos[rr] = s_pos[set][(lane >> 2) + 8 * rr];
       if (pos[rr] != INT_MIN) {
         pos_lo = min(pos_lo, pos[rr]);
         pos_hi = max(pos_hi, pos[rr]);
@@ -565,18 +596,18 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
           }
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            const uint4 qa = qf[(ks + e) * 32 + lane];
+            const uint4 qa = qs[(ks + e) * 32 + lane];
             mma_1688(s[0][e], qa, kh[2 * e], kh[2 * e + 1]);
             mma_1688(s[0][e], qa, kl[2 * e], kl[2 * e + 1]);
             if (R == 16) {
-              const uint4 ql = qf[(KS + ks + e) * 32 + lane];
+              const uint4 ql = qs[(KS + ks + e) * 32 + lane];
               mma_1688(s[0][e], ql, kh[2 * e], kh[2 * e + 1]);
             }
           }
         } else {
 #pragma unroll
           for (int pt = 0; pt < C::QP; pt++) {
-            const uint4 q0 = qf[(pt * KS + ks) * 32 + lane], q1 = qf[(pt * KS + ks + 1) * 32 + lane];
+            const uint4 q0 = qs[(pt * KS + ks) * 32 + lane], q1 = qs[(pt * KS + ks + 1) * 32 + lane];
 #pragma unroll
             for (int t = 0; t < NT; t++) {
               mma_16816(s[t][0], q0, kv[t].x, kv[t].y, T());
@@ -794,117 +825,111 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
       }
     }
 
-    // ---- the segment's end: join the warps
+    // ---- the segment's end: each warp hands over its rows' state, the output in the
+    // stage of its ring that the next load will fill
     const int row = lane >> 2, cl = lane & 3;
+    __syncwarp();  // the stage has been read
+    float* mine = reinterpret_cast<float*>(wring + (stage == 0 ? NS - 1 : stage - 1) * C::WSTAGE);
 #pragma unroll
     for (int rr = 0; rr < NR; rr++) {
       l[rr] += __shfl_xor_sync(~0u, l[rr], 1);
       l[rr] += __shfl_xor_sync(~0u, l[rr], 2);
       if (cl == 0) wml[w * R + row + 8 * rr] = make_float2(m[rr], l[rr]);
-    }
-    const bool whole = n == cur.nt;
-    const bool head = cur.tile != 0;  // begun in an earlier CTA
-    const int slot = 2 * blockIdx.x + (head ? 0 : 1);
-    auto finish = [&](int r, int d, float M, float L, float v) {
-      const int idx = cur.rt * R + r;
-      const int tok = p.group_div.div(idx), h = cur.g * a.group + idx - tok * a.group;
-      paged_finish(p, (int64_t)(cur.row0 + tok) * a.heads + h, d, M, L, v);
-    };
-    const int rows_here = min(R, cur.count * a.group - cur.rt * R);
 #pragma unroll
-    for (int x = 0; x < NPASS; x++)
-#pragma unroll
-      for (int rr = 0; rr < NR; rr++) {
-        float* dst = join + (w * 8 + row) * 64;
+      for (int x = 0; x < NPASS; x++)
 #pragma unroll
         for (int e = 0; e < 2; e++)
 #pragma unroll
           for (int i2 = 0; i2 < 8; i2 += 4) {
-            float4 v;
-            float* vv = reinterpret_cast<float*>(&v);
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-              vv[k] = o[x][i2 + k][2 * rr + e];
-            const int d = F32 ? (i2 >> 2) * 32 + (2 * cl + e) * 4 : (2 * cl + e) * 8 + i2;
-            *reinterpret_cast<float4*>(dst + d) = v;
+            // features d .. d + 3, pieces of 16 bytes swizzled by the row
+            const int d = x * 64 + (F32 ? (i2 >> 2) * 32 + (2 * cl + e) * 4 : (2 * cl + e) * 8 + i2);
+            *reinterpret_cast<float4*>(mine + (row + 8 * rr) * DP + (((d >> 2) ^ row) << 2)) =
+                make_float4(o[x][i2][2 * rr + e], o[x][i2 + 1][2 * rr + e], o[x][i2 + 2][2 * rr + e],
+                            o[x][i2 + 3][2 * rr + e]);
           }
-        __syncthreads();
+    }
+    if (more) build_q(nx, set ^ 1);
+    const int free_stage = (stage == 0 ? NS - 1 : stage - 1) * C::WSTAGE;
+    __syncthreads();
+    const bool whole = n == cur.nt;
+    const bool head = cur.tile != 0;  // begun in an earlier CTA
+    const int slot = 2 * blockIdx.x + (head ? 0 : 1);
+    const int rows_here = min(R, cur.count * a.group - cur.rt * R);
+    for (int e = tid; e < rows_here * (DP / 4); e += 256) {
+      const int r = e / (DP / 4), q = e % (DP / 4);
+      float M = -INFINITY;
 #pragma unroll
-        for (int y = 0; y < 2; y++) {
-          const int e = tid + 256 * y, r8 = e >> 6, dd = e & 63, r = r8 + 8 * rr, d = x * 64 + dd;
-          float M = -INFINITY;
+      for (int i = 0; i < 8; i++) M = fmaxf(M, wml[i * R + r].x);
+      const float mb = M == -INFINITY ? 0.f : M;
+      float L = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int i = 0; i < 8; i++) M = fmaxf(M, wml[i * R + r].x);
-          const float mb = M == -INFINITY ? 0.f : M;
-          float L = 0.f, v = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const float2 q = wml[i * R + r];
-            const float f = ex2(q.x - mb);
-            L = fmaf(f, q.y, L);
-            v = fmaf(f, join[(i * 8 + r8) * 64 + dd], v);
-          }
-          if (r < rows_here && d < D) {
-            if (whole) {
-              finish(r, d, M, L, v);
-            } else {
-              p.part_o[((int64_t)slot * R + r) * DP + d] = v;
-              if (d == 0) {
-                p.part_ml[((int64_t)slot * R + r) * 2] = M;
-                p.part_ml[((int64_t)slot * R + r) * 2 + 1] = L;
-              }
-            }
-          }
-        }
-        __syncthreads();
+      for (int i = 0; i < 8; i++) {
+        const float2 s2 = wml[i * R + r];
+        const float f = ex2(s2.x - mb);
+        // every warp is at the same stage of its ring
+        const float4 t = *reinterpret_cast<const float4*>(
+            ring + i * NS * C::WSTAGE + free_stage + (r * DP + ((q ^ (r & 7)) << 2)) * 4);
+        L = fmaf(f, s2.y, L);
+        v.x = fmaf(f, t.x, v.x), v.y = fmaf(f, t.y, v.y);
+        v.z = fmaf(f, t.z, v.z), v.w = fmaf(f, t.w, v.w);
       }
+      if (4 * q >= D) continue;
+      if (whole) {
+        stream_finish(p, cur, cur.rt * R + r, 4 * q, M, L, v);
+      } else {
+        const int64_t at = (int64_t)slot * R + r;
+        *reinterpret_cast<float4*>(p.part_o + at * DP + 4 * q) = v;
+        if (q == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
+      }
+    }
     if (!whole) {
       // the runs that hold this segment: CTAs c0 .. c1
       const int c0 = (int)(((seg_u + 1) * runs - 1) / total);
       const int c1 = (int)(((seg_u + cur.nt) * runs - 1) / total);
       const int np = c1 - c0 + 1;
+      __syncthreads();
       if (tid == 0)  // releases this CTA's partials (ordered by the barrier), acquires the others'
         s_last = atom_add_acq_rel_gpu(p.tickets + c0, 1u) == (unsigned)(np - 1);
       __syncthreads();
       if (s_last) {
-        for (int r = w; r < rows_here; r += 8) {  // weights of the pieces of a row
+        for (int r = w; r < rows_here; r += 8) {
+          auto piece = [&](int i) { return (int64_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * R + r; };
           float M = -INFINITY;
-          for (int i = lane; i < np; i += 32) {
-            const int sl = 2 * (c0 + i) + (i == 0 ? 1 : 0);
-            M = fmaxf(M, __ldcg(p.part_ml + ((int64_t)sl * R + r) * 2));
-          }
+          for (int i = lane; i < np; i += 32) M = fmaxf(M, __ldcg(p.part_ml + piece(i) * 2));
           for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, x));
           const float mb = M == -INFINITY ? 0.f : M;
           float L = 0.f;
-          for (int i = lane; i < np; i += 32) {
-            const int sl = 2 * (c0 + i) + (i == 0 ? 1 : 0);
-            const float2 q = __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((int64_t)sl * R + r) * 2));
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          const bool in = 4 * lane < D;
+          for (int i0 = 0; i0 < np; i0 += 32) {
+            float2 q = make_float2(-INFINITY, 0.f);
+            if (i0 + lane < np)
+              q = __ldcg(reinterpret_cast<const float2*>(p.part_ml + piece(i0 + lane) * 2));
             const float f = ex2(q.x - mb);
-            join[i * R + r] = f;
             L = fmaf(f, q.y, L);
+            const int k = min(32, np - i0);
+#pragma unroll 8
+            for (int i = 0; i < k; i++) {
+              const float f1 = __shfl_sync(~0u, f, i);
+              if (!in) continue;
+              const float4 t = __ldcg(
+                  reinterpret_cast<const float4*>(p.part_o + piece(i0 + i) * DP + 4 * lane));
+              v.x = fmaf(f1, t.x, v.x), v.y = fmaf(f1, t.y, v.y);
+              v.z = fmaf(f1, t.z, v.z), v.w = fmaf(f1, t.w, v.w);
+            }
           }
           for (int x = 16; x; x >>= 1) L += __shfl_xor_sync(~0u, L, x);
-          if (lane == 0) s_ml[r] = make_float2(M, L);
-        }
-        __syncthreads();
-        for (int e = tid; e < rows_here * D; e += 256) {
-          const int r = e / D, d = e - r * D;
-          float v = 0.f;
-#pragma unroll 8
-          for (int i = 0; i < np; i++) {
-            const int sl = 2 * (c0 + i) + (i == 0 ? 1 : 0);
-            v = fmaf(join[i * R + r], __ldcg(p.part_o + ((int64_t)sl * R + r) * DP + d), v);
-          }
-          finish(r, d, s_ml[r].x, s_ml[r].y, v);
+          if (in) stream_finish(p, cur, cur.rt * R + r, 4 * lane, M, L, v);
         }
         if (tid == 0) p.tickets[c0] = 0u;
       }
     }
-    // ---- the next segment
+    if (!more) break;
+    __syncthreads();  // the handed-over states have been read
     seg_u += cur.nt + EXTRA;
-    if (seg_u >= u1) break;
-    cur.tile = cur.nt - 1;
-    advance(cur);
+    cur = nx;
+    set ^= 1;
   }
   asm volatile("cp.async.wait_group 0;\n" ::: "memory");
 }

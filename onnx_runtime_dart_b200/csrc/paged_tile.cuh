@@ -29,6 +29,8 @@
 // where three parts need more than the scores), then their p.v (DP each).
 #pragma once
 
+#include <type_traits>
+
 #include "paged_stream.cuh"
 #include "tc.cuh"
 
@@ -45,9 +47,12 @@ struct TileCfg {
   static constexpr int NK = PARTS == 2 && DP == 128 ? 3 : 4;  // ring stages of keys
   static constexpr int NV = PARTS == 2 && DP == 128 ? 2 : 4;  // and of values
   static constexpr int DATA = QB + (NK + NV) * STAGE;
-  static constexpr int EXTRA = 2 * KB;  // what a segment's start and end cost, in keys
-  // data, (max, sum) of 128 rows, block validity, barriers, after alignment to 1024
-  static constexpr int SMEM = 1024 + DATA + 128 * 8 + 8 * 16 + 256;
+  // What a segment's start and end cost, in keys: a 4096-token fp16 prompt took 690,
+  // 445, 391, 368, 377 us at 3, 6, 8, 10, 12 blocks, a mixed bf16 step 240, 244, 263
+  // us at 6, 8, 12 (12, 16, 24 half blocks), a shared prefix 159, 151, 151 us at 3, 6, 10.
+  static constexpr int EXTRA = 8 * KB;
+  // data, (max, sum) of 128 rows by both warpgroups, block validity, barriers
+  static constexpr int SMEM = DATA + 2 * 128 * 8 + 8 * 16 + 256;
   static_assert(2 * SREG + 2 * DP <= 512, "TMEM");
   static_assert(DP * 128 * 4 <= QB, "the output is staged in the q tile");
 };
@@ -135,6 +140,55 @@ __device__ __forceinline__ bool bar_or(int id, int n, bool x) {
   return y != 0;
 }
 
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+
+// The parts of a packed pair (Split::pair with the differences in one
+// instruction each).
+template <typename T>
+__device__ __forceinline__ void split2(uint64_t x, uint32_t (&w)[Split<T>::PARTS]) {
+  const uint64_t minus1 = pack2(-1.f, -1.f);
+#pragma unroll
+  for (int i = 0; i < Split<T>::PARTS; i++) {
+    const float2 v = unpack2(x);
+    float2 f;
+    if constexpr (Split<T>::PARTS == 2) {
+      const __half2 h = __floats2half2_rn(v.x, v.y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      f = __half22float2(h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      f = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    }
+    if (i + 1 < Split<T>::PARTS) x = fma2(pack2(f.x, f.y), minus1, x);
+  }
+}
+
 // tile_warp_regs: registers per thread after the split; they draw on what the
 // block was launched with (kTileRegs a thread), which launch_tile checks.
 constexpr int kTileThreads = 384, kTileSoftRegs = 216, kTileLoadRegs = 72, kTileRegs = 168;
@@ -144,15 +198,15 @@ template <typename T, int DP, bool CAP>
 __global__ void __launch_bounds__(kTileThreads, 1)
     paged_tile_kernel(const __grid_constant__ TileArgs args) {
   using C = TileCfg<T, DP>;
-  constexpr int PARTS = C::PARTS, KB = C::KB, NK = C::NK, NV = C::NV;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  constexpr int PARTS = C::PARTS, KB = C::KB, NK = C::NK, NV = C::NV, EX = C::EXTRA;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = smem_raw;  // 1024-byte aligned: the kernel has no other shared memory
   unsigned char* qs = smem;                 // [part][DP / 64][128 rows][128 B], swizzled
   unsigned char* ks = qs + C::QB;           // [NK][DP / 64][KB rows][128 B]
   unsigned char* vs = ks + NK * C::STAGE;   // [NV] the same
   float* ost = reinterpret_cast<float*>(qs);  // [DP][128] at a segment's end
-  float2* stats = reinterpret_cast<float2*>(smem + C::DATA);  // [128]
-  uint32_t* kvalid = reinterpret_cast<uint32_t*>(stats + 128);  // [8][4]
+  float2* stats = reinterpret_cast<float2*>(smem + C::DATA);  // [2][128]
+  uint32_t* kvalid = reinterpret_cast<uint32_t*>(stats + 256);  // [8][4]
   uint64_t* bars = reinterpret_cast<uint64_t*>(kvalid + 32);
   uint64_t *kfull = bars, *kempty = kfull + NK, *vfull = kempty + NK, *vempty = vfull + NV,
            *sfull = vempty + NV, *pfull = sfull + 2, *pvfull = pfull + 2, *qfull = pvfull + 2;
@@ -165,7 +219,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const PagedView& c = a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int D = c.D, G = c.kv_heads, nb = p.prefix ? 1 : c.batch, TT = 128 / a.group;
-  const int EX = p.ex * 128;
   const int rows_tma = args.tma_rows, align = max(1, rows_tma);
 
   // ---- this CTA's run
@@ -568,8 +621,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if constexpr (PARTS == 2) {  // the row's largest value into [2^13, 2^14)
           float mx = fmaxf(fmaxf(fabsf(q4[i].x), fabsf(q4[i].y)),
                            fmaxf(fabsf(q4[i].z), fabsf(q4[i].w)));
+          if (LPR == 32) {
+            mx = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(mx)));
+          } else {
 #pragma unroll
-          for (int x = LPR / 2; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, x));
+            for (int x = LPR / 2; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, x));
+          }
           int ex = (int)(__float_as_uint(mx) >> 23) - 127;
           ex = max(-100, min(ex, 126));
           up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
@@ -616,9 +673,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int from = max(first, a.window ? own - a.window + 1 : 0);
       const float cmul = fac * p.t_mul;
 
-      float m = -INFINITY, l = 0.f, o[DP];
+      float m = -INFINITY, l = 0.f;
+      uint64_t o[DP / 2];  // pairs of features
 #pragma unroll
-      for (int i = 0; i < DP; i++) o[i] = 0.f;
+      for (int i = 0; i < DP / 2; i++) o[i] = 0;
       for (int k = wg; k < n; k += 2) {
         const int base = cur.lo + (k0 + k) * KB;
         wait(sfull + wg, sc & 1);
@@ -630,35 +688,32 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           const int b = base + 32 * i, x0 = max(from - b, 0), x1 = min(pos - b, 31);
           return pos < b || x0 > x1 ? 0u : kv[i] & (~0u >> (31 - x1)) & (~0u << x0);
         };
-        // 16 scores at a time, the next ones on their way from TMEM meanwhile
-        uint32_t ra[16], rb[16];
-        auto steps = [&](auto&& f) {
-          tmem_ld16(ts, ra);
-#pragma unroll 1
-          for (int i = 0; i < KB / 32; i++) {
-            const uint32_t vw = full ? ~0u : seen(i);
-            tmem_ld_wait();
-            tmem_ld16(ts + 32 * i + 16, rb);
-            f(2 * i, ra, vw);
-            tmem_ld_wait();
-            if (i + 1 < KB / 32) tmem_ld16(ts + 32 * i + 32, ra);
-            f(2 * i + 1, rb, vw >> 16);
-          }
-        };
         // the row's maximum
         float mx = -INFINITY, mx2 = -INFINITY;
-        steps([&](int, uint32_t (&r)[16], uint32_t vw) {
-          if (!full) {
+        if (full) {
 #pragma unroll
-            for (int e = 0; e < 16; e++)
-              if (!((vw >> e) & 1)) r[e] = 0xff800000u;
-          }
+          for (int i = 0; i < KB / 64; i++) {
+            uint32_t r[64];
+            tmem_ld64(ts + 64 * i, r);
+            tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            mx = fmaxf(mx, __uint_as_float(r[e]));
-            mx2 = fmaxf(mx2, __uint_as_float(r[e + 1]));
+            for (int e = 0; e < 64; e += 4) {
+              mx = max3(mx, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+              mx2 = max3(mx2, __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+            }
           }
-        });
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < KB / 32; i++) {
+            uint32_t r[32];
+            tmem_ld32(ts + 32 * i, r);
+            const uint32_t vw = seen(i);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+              if ((vw >> e) & 1) mx = fmaxf(mx, __uint_as_float(r[e]));
+          }
+        }
         mx = fmaxf(mx, mx2);
         if (mx != -INFINITY) mx = CAP ? tanhf(mx * fac) * p.t_mul : mx * cmul;
         const float mn = fmaxf(m, mx), mb = mn == -INFINITY ? 0.f : mn;
@@ -672,51 +727,64 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         unsigned char* vst = vs + ((gb + k) % NV) * C::STAGE;
         if (!full) {
           wait(vfull + (gb + k) % NV, ((gb + k) / NV) & 1);
-#pragma unroll 4
-          for (int i = row; i < C::STAGE / 16; i += 128) {
-            const int r = (i >> 3) & (KB - 1), j = base + r;
-            uint4* at = reinterpret_cast<uint4*>(vst) + i;
-            if (j < first || j >= cur.hi || !((kv[r >> 5] >> (r & 31)) & 1)) {
-              *at = make_uint4(0u, 0u, 0u, 0u);
-              continue;
-            }
-            const uint4 v = *at;
-            const uint32_t ws[4] = {v.x, v.y, v.z, v.w};
-            constexpr uint32_t inf = PARTS == 2 ? 0x7c00u : 0x7f80u;
+          // a thread looks over one row (KB = 64: half a row)
+          constexpr int TPR = 128 / KB, CPT = DP / 8 / TPR;
+          const int r = row & (KB - 1), j = base + r, ch0 = row / KB * CPT;
+          const bool there = j >= first && j < cur.hi && ((kv[r >> 5] >> (r & 31)) & 1);
+          constexpr uint32_t up = PARTS == 2 ? 0x04000400u : 0x00800080u;
+          uint32_t top = 0;  // exponents of all ones carry into the halves' sign bits
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-              odd |= (ws[e] & inf) == inf || ((ws[e] >> 16) & inf) == inf;
+          for (int y = 0; y < CPT; y++) {
+            const int ch = ch0 + y;
+            uint4* at = reinterpret_cast<uint4*>(vst + (ch >> 3) * (KB * 128) + r * 128 +
+                                                 (((ch & 7) ^ (r & 7)) << 4));
+            if (there) {
+              const uint4 v = *at;
+              top |= ((v.x & 0x7fff7fffu) + up) | ((v.y & 0x7fff7fffu) + up) |
+                     ((v.z & 0x7fff7fffu) + up) | ((v.w & 0x7fff7fffu) + up);
+            } else {
+              *at = make_uint4(0u, 0u, 0u, 0u);
+            }
           }
+          odd = (top & 0x80008000u) != 0;
           fence_proxy_async_smem();
           odd = bar_or(2 + wg, 128, odd);
         }
 
         // weights, over the scores
-        float sum = 0.f, sum2 = 0.f;
-        steps([&](int st, uint32_t (&r)[16], uint32_t vw) {
-          float x[16];
+        uint64_t sums[2] = {0, 0};
+        const uint64_t cmul2 = pack2(cmul, cmul), sub2 = pack2(-sub, -sub);
+        // 16 scores: exp2, their sum, the parts
+        auto weigh = [&](auto masked, int st, const uint32_t (&r)[16], uint32_t vw) {
+          uint64_t x[8];
 #pragma unroll
-          for (int e = 0; e < 16; e++) {
+          for (int e = 0; e < 8; e++) {
+            float2 t = make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
             if (CAP)
-              x[e] = ex2(fmaf(tanhf(__uint_as_float(r[e]) * fac), p.t_mul, -sub));
+              t = make_float2(fmaf(tanhf(t.x * fac), p.t_mul, -sub),
+                              fmaf(tanhf(t.y * fac), p.t_mul, -sub));
             else
-              x[e] = ex2(fmaf(__uint_as_float(r[e]), cmul, -sub));
+              t = unpack2(fma2(pack2(t.x, t.y), cmul2, sub2));
+            t.x = ex2(t.x), t.y = ex2(t.y);
+            if (masked) {
+              t.x = (vw >> (2 * e)) & 1 ? t.x : 0.f;
+              t.y = (vw >> (2 * e + 1)) & 1 ? t.y : 0.f;
+            }
+            x[e] = pack2(t.x, t.y);
+            sums[e & 1] = add2(sums[e & 1], x[e]);
           }
-          if (!full) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) x[e] = (vw >> e) & 1 ? x[e] : 0.f;
-          }
-#pragma unroll
-          for (int e = 0; e < 16; e += 2) sum += x[e], sum2 += x[e + 1];
           uint32_t wd[16], w2[8];
-          if (odd) {  // kept in fp32 for the sum below
+          if (masked && odd) {  // kept in fp32 for the sum below
 #pragma unroll
-            for (int e = 0; e < 16; e++) wd[e] = __float_as_uint(x[e]), w2[e >> 1] = 0u;
+            for (int e = 0; e < 8; e++) {
+              const float2 t = unpack2(x[e]);
+              wd[2 * e] = __float_as_uint(t.x), wd[2 * e + 1] = __float_as_uint(t.y), w2[e] = 0u;
+            }
           } else {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
               uint32_t t[PARTS];
-              Split<T>::pair(x[2 * e], x[2 * e + 1], t);
+              split2<T>(x[e], t);
               wd[e] = t[0], wd[8 + e] = t[1], w2[e] = t[PARTS - 1];
             }
           }
@@ -724,13 +792,36 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (PARTS == 3)
             tmem_st8(ts + KB + 8 * st, make_uint4(w2[0], w2[1], w2[2], w2[3]),
                      make_uint4(w2[4], w2[5], w2[6], w2[7]));
-        });
-        sum += sum2;
-        l = l * corr + sum;
+        };
+        if (full) {  // the next scores on their way from TMEM meanwhile
+          uint32_t ra[16], rb[16];
+          tmem_ld16(ts, ra);
+#pragma unroll 1
+          for (int i = 0; i < KB / 32; i++) {
+            tmem_ld_wait();
+            tmem_ld16(ts + 32 * i + 16, rb);
+            weigh(std::false_type(), 2 * i, ra, 0u);
+            tmem_ld_wait();
+            if (i + 1 < KB / 32) tmem_ld16(ts + 32 * i + 32, ra);
+            weigh(std::false_type(), 2 * i + 1, rb, 0u);
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < KB / 16; i++) {
+            uint32_t r[16];
+            tmem_ld16(ts + 16 * i, r);
+            const uint32_t vw = seen(i >> 1) >> (16 * (i & 1));
+            tmem_ld_wait();
+            weigh(std::true_type(), i, r, vw);
+          }
+        }
+        const float2 sa = unpack2(add2(sums[0], sums[1]));
+        l = l * corr + (sa.x + sa.y);
         tmem_st_wait();
+        const uint64_t corr2 = pack2(corr, corr);
         if (odd) {
 #pragma unroll
-          for (int i = 0; i < DP; i++) o[i] *= corr;
+          for (int i = 0; i < DP / 2; i++) o[i] = fma2(o[i], corr2, 0);
           for (int j = 0; j < KB; j++) {
             uint32_t r;
             tmem_ld1(ts + j, r);
@@ -742,8 +833,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                   vst + (ch >> 3) * (KB * 128) + j * 128 + (((ch & 7) ^ (j & 7)) << 4));
               const T* ve = reinterpret_cast<const T*>(&v);
 #pragma unroll
-              for (int e = 0; e < 8; e++)
-                if (w != 0.f) o[8 * ch + e] = fmaf(w, (float)ve[e], o[8 * ch + e]);
+              for (int e = 0; e < 4; e++)
+                if (w != 0.f)
+                  o[4 * ch + e] = fma2(pack2(w, w), pack2((float)ve[2 * e], (float)ve[2 * e + 1]),
+                                       o[4 * ch + e]);
             }
           }
         }
@@ -758,7 +851,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tmem_ld32(to + 32 * i, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 32; e++) o[32 * i + e] = fmaf(o[32 * i + e], corr, __uint_as_float(r[e]));
+          for (int e = 0; e < 16; e++)
+            o[16 * i + e] = fma2(o[16 * i + e], corr2, pack2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])));
         }
       }
       gb += n;
@@ -767,20 +861,52 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       auto at = [&](int d, int r) -> float& { return ost[d * 128 + (r ^ (d & 31))]; };
       tc_fence_before();
       bar_sync(1, 256);  // every MMA of the segment is done: the q tile is free
-      if (wg == 1) {
+      // each warpgroup hands over half of the features and joins the other half
+      auto hand = [&](auto half) {
 #pragma unroll
-        for (int i = 0; i < DP; i++) at(i, row) = o[i];
-        stats[row] = make_float2(m, l);
-      }
+        for (int i = 0; i < DP / 4; i++) {
+          const float2 v = unpack2(o[half * (DP / 4) + i]);
+          at(half * (DP / 2) + 2 * i, row) = v.x;
+          at(half * (DP / 2) + 2 * i + 1, row) = v.y;
+        }
+      };
+      auto join = [&](auto half, float mine, float theirs) {
+#pragma unroll
+        for (int i0 = 0; i0 < DP / 4; i0 += 8) {
+          float2 t[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int d = half * (DP / 2) + 2 * (i0 + i);
+            t[i] = make_float2(at(d, row), at(d + 1, row));
+          }
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int d = half * (DP / 2) + 2 * (i0 + i);
+            const float2 v = unpack2(o[d / 2]);
+            at(d, row) = v.x * mine + t[i].x * theirs;
+            at(d + 1, row) = v.y * mine + t[i].y * theirs;
+          }
+        }
+      };
+      using H0 = std::integral_constant<int, 0>;
+      using H1 = std::integral_constant<int, 1>;
+      stats[wg * 128 + row] = make_float2(m, l);
+      if (wg == 0)
+        hand(H1());
+      else
+        hand(H0());
       bar_sync(1, 256);
-      if (wg == 0) {
-        const float2 s2 = stats[row];
-        const float M = fmaxf(m, s2.x), mb = M == -INFINITY ? 0.f : M;
-        const float w0 = ex2(m - mb), w1 = ex2(s2.x - mb);
-        stats[row] = make_float2(M, l * w0 + s2.y * w1);
-#pragma unroll
-        for (int i = 0; i < DP; i++) at(i, row) = o[i] * w0 + at(i, row) * w1;
-      }
+      const float2 s2 = stats[(wg ^ 1) * 128 + row];
+      const float M = fmaxf(m, s2.x), mb = M == -INFINITY ? 0.f : M;
+      const float mine = ex2(m - mb), theirs = ex2(s2.x - mb);
+      if (wg == 0)
+        join(H0(), mine, theirs);
+      else
+        join(H1(), mine, theirs);
+      bar_sync(1, 256);
+      // (stats[0..127] becomes the joined pair; a thread reads only its own row's
+      // other half above, so the second half of the array is no longer needed)
+      if (wg == 0) stats[row] = make_float2(M, l * mine + s2.y * theirs);
       bar_sync(1, 256);
       const bool whole = n == cur.nt;
       const int slot = 2 * blockIdx.x + (k0 ? 0 : 1);
@@ -800,7 +926,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (p.prefix && lane == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * to) = make_float2(M, L);
       };
       constexpr int NX = DP / 32;
-#pragma unroll 2
+#pragma unroll 4
       for (int r = warp; r < rows_here; r += 8) {
         const float2 ml = stats[r];
         float v[NX];
