@@ -3,6 +3,7 @@
 #include <atomic>
 #include <climits>
 
+#include "paged_rows.cuh"
 #include "paged_tile.cuh"
 
 namespace ortc {
@@ -19,10 +20,9 @@ constexpr int kStreamRows = 64;
 int stream_rows(int64_t rows) { return rows <= 8 ? 8 : 16; }
 int padded_head(int D) { return D <= 64 ? 64 : 128; }
 
-// Whether the tile kernel may be used: 16-bit pages, a token's heads in a tile.
-bool tile_ok(const PagedAttnArgs& a) {
-  return a.c.type != ORT_CUDA_CACHE_F32 && a.group <= 64;
-}
+// Whether tiles of 128 rows may be used (csrc/paged_tile.cuh for 16-bit pages,
+// csrc/paged_rows.cuh for fp32): two tokens' heads at least fit one.
+bool tile_ok(const PagedAttnArgs& a) { return a.group <= 64; }
 
 template <typename K>
 int set_smem(K kernel, int bytes, std::atomic<unsigned long long>& done) {
@@ -93,7 +93,23 @@ int launch_tile_one(const TileArgs& p, int grid, cudaStream_t st) {
                            : launch_tile_cap<T, DP, false>(p, grid, st);
 }
 
+template <int DP>
+int launch_rows(const StreamArgs& p, int grid, cudaStream_t st) {
+  static std::atomic<unsigned long long> attr_set{0};
+  const int rc = set_smem(paged_rows_kernel<DP>, RowsCfg<DP>::SMEM, attr_set);
+  if (rc) return rc;
+  paged_rows_kernel<DP><<<grid, 256, RowsCfg<DP>::SMEM, st>>>(p);
+  ORTC_CUDA(cudaGetLastError());
+  return ORT_CUDA_OK;
+}
+
 int launch_tile(const StreamArgs& s, int grid, cudaStream_t st, int64_t* launches) {
+  if (s.a.c.type == ORT_CUDA_CACHE_F32) {
+    const int rc = padded_head(s.a.c.D) == 64 ? launch_rows<64>(s, grid, st)
+                                              : launch_rows<128>(s, grid, st);
+    if (rc == ORT_CUDA_OK) (*launches)++;
+    return rc;
+  }
   TileArgs p;
   p.s = s;
   const PagedView& c = s.a.c;
@@ -121,7 +137,7 @@ int launch_tile(const StreamArgs& s, int grid, cudaStream_t st, int64_t* launche
   return rc;
 }
 
-// Whether the sequences' own keys, and the shared prefix, may need the tile kernel.
+// Whether the sequences' own keys, and the shared prefix, may need tiles of 128 rows.
 bool tile_main(const PagedAttnArgs& a) {
   return tile_ok(a) && (int64_t)a.max_seq * a.group > kStreamRows;
 }

@@ -219,14 +219,285 @@ __device__ __forceinline__ int stream_seq(const StreamArgs& p, StreamPos& s, int
   return (s.nt + EXTRA) * s.nrt;
 }
 
-// Writes features d .. d + 3 of query row idx of a segment's sequence and KV head
-// (D is a multiple of 8): the output, joined with what the prefix pass left, or, in
-// the prefix pass, that.
-__device__ __forceinline__ void stream_finish(const StreamArgs& p, const StreamPos& s, int idx,
-                                              int d, float M, float L, float4 v) {
+// One step of a warp: KW keys at `base` (bit r of `valid`: key r is there) in
+// shared memory at kt, vt against its R rows, whose operands are qs, score factors
+// fac, positions pos (from pos_lo to pos_hi over the rows); m, l, o: the rows'
+// running maximum, this lane's part of the sum, output.
+template <typename T, int DP, int R>
+__device__ __forceinline__ void stream_step(const uint4* qs, const unsigned char* kt,
+                                            const unsigned char* vt, unsigned valid, int base,
+                                            const float (&fac)[R / 8], const int (&pos)[R / 8],
+                                            int pos_lo, int pos_hi, int window, bool softcap,
+                                            float t_mul, float (&m)[R / 8], float (&l)[R / 8],
+                                            float (&o)[DP / 64][8][R / 4]) {
+  using C = StreamCfg<T, DP, R>;
+  constexpr bool F32 = C::F32;
+  constexpr int KW = C::KW, CHP = C::CHP, KS = C::KS, PARTS = Split<T>::PARTS, NPASS = DP / 64;
+  constexpr int NR = R / 8;
+  const int lane = threadIdx.x & 31;
+  // scores
+  constexpr int NT = KW / 8;
+  float s[NT][2][4];  // two chains of products each
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) s[t][0][e] = s[t][1][e] = 0.f;
+  const int row = lane >> 2, cl = lane & 3;
+#pragma unroll
+  for (int ks = 0; ks < KS; ks += 2) {
+    const int ch = cl + 4 * (ks >> 1);
+    uint4 kv[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+      kv[t] = *reinterpret_cast<const uint4*>(kt + (row + 8 * t) * C::ROWB +
+                                              ((ch ^ ((row & 1) << 2)) << 4));
+    if constexpr (F32) {
+      uint32_t kh[4], kl[4];
+      const float kx[4] = {__uint_as_float(kv[0].x), __uint_as_float(kv[0].y),
+                           __uint_as_float(kv[0].z), __uint_as_float(kv[0].w)};
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        uint32_t ww[2];
+        Split<float>::one(kx[e], ww);
+        kh[e] = ww[0], kl[e] = ww[1];
+      }
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const uint4 qa = qs[(ks + e) * 32 + lane];
+        mma_1688(s[0][e], qa, kh[2 * e], kh[2 * e + 1]);
+        mma_1688(s[0][e], qa, kl[2 * e], kl[2 * e + 1]);
+        if (R == 16) {
+          const uint4 ql = qs[(KS + ks + e) * 32 + lane];
+          mma_1688(s[0][e], ql, kh[2 * e], kh[2 * e + 1]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int pt = 0; pt < C::QP; pt++) {
+        const uint4 q0 = qs[(pt * KS + ks) * 32 + lane], q1 = qs[(pt * KS + ks + 1) * 32 + lane];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          mma_16816(s[t][0], q0, kv[t].x, kv[t].y, T());
+          mma_16816(s[t][1], q1, kv[t].z, kv[t].w, T());
+        }
+      }
+    }
+  }
+
+  // softmax weights; rows (lane / 4) + 8 rr, keys base + 8 t + 2 cl + e
+  const bool full = valid == (1u << KW) - 1 && base + KW - 1 <= pos_lo &&
+                    (!window || base > pos_hi - window);
+  float pr[NR][NT][2];
+#pragma unroll
+  for (int rr = 0; rr < NR; rr++)
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float x = s[t][0][2 * rr + e] + s[t][1][2 * rr + e];
+        if (R == 8) x += s[t][0][e + 2] + s[t][1][e + 2];
+        x *= fac[rr];
+        if (softcap) x = tanhf(x);
+        pr[rr][t][e] = x * t_mul;
+      }
+  if (!full) {
+#pragma unroll
+    for (int rr = 0; rr < NR; rr++)
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const int k = 8 * t + 2 * cl + e, j = base + k;
+          if (!((valid >> k) & 1) || j > pos[rr] || (window && j <= pos[rr] - window))
+            pr[rr][t][e] = -INFINITY;
+        }
+  }
+  float corr[NR];
+#pragma unroll
+  for (int rr = 0; rr < NR; rr++) {
+    float mx = m[rr];
+#pragma unroll
+    for (int t = 0; t < NT; t++) mx = fmaxf(mx, fmaxf(pr[rr][t][0], pr[rr][t][1]));
+    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+    const float mb = mx == -INFINITY ? 0.f : mx;
+    corr[rr] = ex2(m[rr] - mb);
+    m[rr] = mx;
+    // p scaled by 2^15 for fp16: its low part then keeps its bits
+    const float sub = PARTS == 2 && !F32 ? mb - 15.f : mb;
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        pr[rr][t][e] = ex2(pr[rr][t][e] - sub);
+        sum += pr[rr][t][e];
+      }
+    l[rr] = l[rr] * corr[rr] + sum;
+  }
+  // A value that only some rows see must not reach the others as 0 * inf:
+  // such tiles (the border of the mask) are looked over, and one that holds
+  // an infinity or NaN is summed key by key.
+  bool odd = false;
+  if (!full) {
+#pragma unroll
+    for (int x = 0; x < KW * CHP / 32; x++) {
+      const uint4 v = reinterpret_cast<const uint4*>(vt)[x * 32 + lane];
+      const uint32_t ws[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if constexpr (F32) {
+          odd |= (ws[e] & 0x7f800000u) == 0x7f800000u;
+        } else {
+          constexpr uint32_t inf = PARTS == 2 ? 0x7c00u : 0x7f80u;
+          odd |= (ws[e] & inf) == inf || ((ws[e] >> 16) & inf) == inf;
+        }
+      }
+    }
+    odd = __any_sync(~0u, odd);
+  }
+  if (odd) {
+#pragma unroll
+    for (int x = 0; x < NPASS; x++)
+#pragma unroll
+      for (int i2 = 0; i2 < 8; i2++)
+#pragma unroll
+        for (int e = 0; e < 2 * NR; e++) o[x][i2][e] *= corr[e >> 1];
+    for (int k = 0; k < KW; k++) {
+      float pk[NR];
+#pragma unroll
+      for (int rr = 0; rr < NR; rr++) {
+        float mine = 0.f;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+            if (k == 8 * t + 2 * cl + e) mine = pr[rr][t][e];
+        pk[rr] = __shfl_sync(~0u, mine, (lane & ~3) | ((k >> 1) & 3));
+      }
+      const T* vr = reinterpret_cast<const T*>(vt + k * C::ROWB);
+#pragma unroll
+      for (int x = 0; x < NPASS; x++)
+#pragma unroll
+        for (int i2 = 0; i2 < 8; i2++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            // feature of accumulator (x, i2, column 2 cl + e)
+            const int d = F32 ? x * 64 + (i2 >> 2) * 32 + (2 * cl + e) * 4 + (i2 & 3)
+                              : x * 64 + (2 * cl + e) * 8 + i2;
+            constexpr int PC = 16 / (int)sizeof(T);
+            const int dd = ((d / PC) ^ (((k >> 1) & 3) << 1)) * PC + d % PC;
+            const float v = (float)vr[dd];
+#pragma unroll
+            for (int rr = 0; rr < NR; rr++)
+              if (pk[rr] != 0.f) o[x][i2][2 * rr + e] = fmaf(pk[rr], v, o[x][i2][2 * rr + e]);
+          }
+    }
+    return;
+  }
+
+  // o = o corr + p . v, the products of a tile in accumulators of their own:
+  // the tensor cores' sums are cut off, not rounded, and over a long run of
+  // tiles that adds up (1.5e-6 of the result over 131000 keys, against 0.5e-6
+  // so)
+  auto add = [&](float(&acc)[2 * NR], const float(&d)[4]) {
+    if constexpr (R == 8) {
+      acc[0] = fmaf(acc[0], corr[0], d[0] + d[2]);
+      acc[1] = fmaf(acc[1], corr[0], d[1] + d[3]);
+    } else {
+      acc[0] = fmaf(acc[0], corr[0], d[0]);
+      acc[1] = fmaf(acc[1], corr[0], d[1]);
+      acc[2] = fmaf(acc[2], corr[NR - 1], d[2]);
+      acc[3] = fmaf(acc[3], corr[NR - 1], d[3]);
+    }
+  };
+  if constexpr (F32) {
+    uint4 pa[2];
+    {
+      uint32_t w0[2], w1[2];
+      Split<float>::one(pr[0][0][0], w0);
+      Split<float>::one(pr[0][0][1], w1);
+      if (R == 8) {
+        pa[0] = make_uint4(w0[0], w0[1], w1[0], w1[1]);
+      } else {
+        uint32_t y0[2], y1[2];
+        Split<float>::one(pr[NR - 1][0][0], y0);
+        Split<float>::one(pr[NR - 1][0][1], y1);
+        pa[0] = make_uint4(w0[0], y0[0], w1[0], y1[0]);
+        pa[1] = make_uint4(w0[1], y0[1], w1[1], y1[1]);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < DP / 32; x++) {
+      const int ch = row + 8 * x;
+      const uint4 v0 = *reinterpret_cast<const uint4*>(vt + (2 * cl) * C::ROWB +
+                                                       ((ch ^ (cl << 1)) << 4));
+      const uint4 v1 = *reinterpret_cast<const uint4*>(vt + (2 * cl + 1) * C::ROWB +
+                                                       ((ch ^ (cl << 1)) << 4));
+      const uint32_t a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        uint32_t h0[2], h1[2];
+        Split<float>::one(__uint_as_float(a0[e]), h0);
+        Split<float>::one(__uint_as_float(a1[e]), h1);
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_1688(d, pa[0], h0[0], h1[0]);
+        mma_1688(d, pa[0], h0[1], h1[1]);
+        if (R == 16) mma_1688(d, pa[1], h0[0], h1[0]);
+        add(o[x >> 1][(x & 1) * 4 + e], d);
+      }
+    }
+  } else {
+    uint4 pa[C::QP];
+    {
+      uint32_t w0[PARTS], w1[PARTS];
+      Split<T>::pair(pr[0][0][0], pr[0][0][1], w0);
+      Split<T>::pair(pr[0][NT - 1][0], pr[0][NT - 1][1], w1);
+      if (R == 8) {
+        pa[0] = make_uint4(w0[0], w0[1], w1[0], w1[1]);
+        if (PARTS == 3) pa[C::QP - 1] = make_uint4(w0[PARTS - 1], 0u, w1[PARTS - 1], 0u);
+      } else {
+        uint32_t y0[PARTS], y1[PARTS];
+        Split<T>::pair(pr[NR - 1][0][0], pr[NR - 1][0][1], y0);
+        Split<T>::pair(pr[NR - 1][NT - 1][0], pr[NR - 1][NT - 1][1], y1);
+#pragma unroll
+        for (int pt = 0; pt < PARTS; pt++)
+          pa[pt < C::QP ? pt : 0] = make_uint4(w0[pt], y0[pt], w1[pt], y1[pt]);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < NPASS; x++) {
+      const int ch = row + 8 * x;
+      uint4 v[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int r = 2 * cl + (e & 1) + 8 * (e >> 1);
+        v[e] = *reinterpret_cast<const uint4*>(vt + r * C::ROWB + ((ch ^ (cl << 1)) << 4));
+      }
+      const uint32_t a0[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+      const uint32_t a1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+      const uint32_t a8[4] = {v[2].x, v[2].y, v[2].z, v[2].w};
+      const uint32_t a9[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
+        const uint32_t b0 = __byte_perm(a0[e >> 1], a1[e >> 1], sel);
+        const uint32_t b1 = __byte_perm(a8[e >> 1], a9[e >> 1], sel);
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int pt = 0; pt < C::QP; pt++) mma_16816(d, pa[pt], b0, b1, T());
+        add(o[x][e], d);
+      }
+    }
+  }
+}
+
+// Writes features d .. d + 3 of (token, head) `at` (D is a multiple of 8): the output,
+// joined with what the prefix pass left, or, in the prefix pass, that.
+__device__ __forceinline__ void write4(const StreamArgs& p, int64_t at, int d, float M, float L,
+                                       float4 v) {
   const PagedAttnArgs& a = p.a;
-  const int tok = p.group_div.div(idx), h = s.g * a.group + idx - tok * a.group, D = a.c.D;
-  const int64_t at = (int64_t)(s.row0 + tok) * a.heads + h;
+  const int D = a.c.D;
   if (p.prefix) {
     *reinterpret_cast<float4*>(p.pre_o + at * D + d) = v;
     if (d == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * at) = make_float2(M, L);
@@ -246,6 +517,13 @@ __device__ __forceinline__ void stream_finish(const StreamArgs& p, const StreamP
     dst[0] = v.x, dst[1] = v.y, dst[2] = v.z, dst[3] = v.w;
 }
 
+// The same for query row idx of a segment's sequence and KV head.
+__device__ __forceinline__ void stream_finish(const StreamArgs& p, const StreamPos& s, int idx,
+                                              int d, float M, float L, float4 v) {
+  const int tok = p.group_div.div(idx), h = s.g * p.a.group + idx - tok * p.a.group;
+  write4(p, (int64_t)(s.row0 + tok) * p.a.heads + h, d, M, L, v);
+}
+
 template <typename T, int DP, int R>
 __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_constant__ StreamArgs p) {
   using C = StreamCfg<T, DP, R>;
@@ -253,7 +531,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
   constexpr int KW = C::KW, TK = C::TK, EXTRA = C::EXTRA, CHP = C::CHP, NS = C::NS, KS = C::KS, PARTS = Split<T>::PARTS;
   constexpr int NPASS = DP / 64;       // blocks of 64 features of the output
   constexpr int NR = R / 8;            // rows a lane holds
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* ring = smem;
   uint4* qf = reinterpret_cast<uint4*>(smem + C::RING);  // [2][QP][KS][32]: segments in turn
   float2* wml = reinterpret_cast<float2*>(smem + C::RING + 2 * C::QB);  // [8][R]
@@ -568,261 +846,8 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
       const int base = cur.lo + (cur.tile + i) * TK + w * KW;
       if (valid == 0) continue;
 
-      // scores
-      constexpr int NT = KW / 8;
-      float s[NT][2][4];  // two chains of products each
-#pragma unroll
-      for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) s[t][0][e] = s[t][1][e] = 0.f;
-      const int row = lane >> 2, cl = lane & 3;
-#pragma unroll
-      for (int ks = 0; ks < KS; ks += 2) {
-        const int ch = cl + 4 * (ks >> 1);
-        uint4 kv[NT];
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-          kv[t] = *reinterpret_cast<const uint4*>(kt + (row + 8 * t) * C::ROWB +
-                                                  ((ch ^ ((row & 1) << 2)) << 4));
-        if constexpr (F32) {
-          uint32_t kh[4], kl[4];
-          const float kx[4] = {__uint_as_float(kv[0].x), __uint_as_float(kv[0].y),
-                               __uint_as_float(kv[0].z), __uint_as_float(kv[0].w)};
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            uint32_t ww[2];
-            Split<float>::one(kx[e], ww);
-            kh[e] = ww[0], kl[e] = ww[1];
-          }
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const uint4 qa = qs[(ks + e) * 32 + lane];
-            mma_1688(s[0][e], qa, kh[2 * e], kh[2 * e + 1]);
-            mma_1688(s[0][e], qa, kl[2 * e], kl[2 * e + 1]);
-            if (R == 16) {
-              const uint4 ql = qs[(KS + ks + e) * 32 + lane];
-              mma_1688(s[0][e], ql, kh[2 * e], kh[2 * e + 1]);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int pt = 0; pt < C::QP; pt++) {
-            const uint4 q0 = qs[(pt * KS + ks) * 32 + lane], q1 = qs[(pt * KS + ks + 1) * 32 + lane];
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-              mma_16816(s[t][0], q0, kv[t].x, kv[t].y, T());
-              mma_16816(s[t][1], q1, kv[t].z, kv[t].w, T());
-            }
-          }
-        }
-      }
-
-      // softmax weights; rows (lane / 4) + 8 rr, keys base + 8 t + 2 cl + e
-      const bool full = valid == (1u << KW) - 1 && base + KW - 1 <= pos_lo &&
-                        (!a.window || base > pos_hi - a.window);
-      float pr[NR][NT][2];
-#pragma unroll
-      for (int rr = 0; rr < NR; rr++)
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            float x = s[t][0][2 * rr + e] + s[t][1][2 * rr + e];
-            if (R == 8) x += s[t][0][e + 2] + s[t][1][e + 2];
-            x *= fac[rr];
-            if (a.softcap > 0.f) x = tanhf(x);
-            pr[rr][t][e] = x * p.t_mul;
-          }
-      if (!full) {
-#pragma unroll
-        for (int rr = 0; rr < NR; rr++)
-#pragma unroll
-          for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              const int k = 8 * t + 2 * cl + e, j = base + k;
-              if (!((valid >> k) & 1) || j > pos[rr] || (a.window && j <= pos[rr] - a.window))
-                pr[rr][t][e] = -INFINITY;
-            }
-      }
-      float corr[NR];
-#pragma unroll
-      for (int rr = 0; rr < NR; rr++) {
-        float mx = m[rr];
-#pragma unroll
-        for (int t = 0; t < NT; t++) mx = fmaxf(mx, fmaxf(pr[rr][t][0], pr[rr][t][1]));
-        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-        const float mb = mx == -INFINITY ? 0.f : mx;
-        corr[rr] = ex2(m[rr] - mb);
-        m[rr] = mx;
-        // p scaled by 2^15 for fp16: its low part then keeps its bits
-        const float sub = PARTS == 2 && !F32 ? mb - 15.f : mb;
-        float sum = 0.f;
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            pr[rr][t][e] = ex2(pr[rr][t][e] - sub);
-            sum += pr[rr][t][e];
-          }
-        l[rr] = l[rr] * corr[rr] + sum;
-      }
-      // A value that only some rows see must not reach the others as 0 * inf:
-      // such tiles (the border of the mask) are looked over, and one that holds
-      // an infinity or NaN is summed key by key.
-      bool odd = false;
-      if (!full) {
-#pragma unroll
-        for (int x = 0; x < KW * CHP / 32; x++) {
-          const uint4 v = reinterpret_cast<const uint4*>(vt)[x * 32 + lane];
-          const uint32_t ws[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            if constexpr (F32) {
-              odd |= (ws[e] & 0x7f800000u) == 0x7f800000u;
-            } else {
-              constexpr uint32_t inf = PARTS == 2 ? 0x7c00u : 0x7f80u;
-              odd |= (ws[e] & inf) == inf || ((ws[e] >> 16) & inf) == inf;
-            }
-          }
-        }
-        odd = __any_sync(~0u, odd);
-      }
-      if (odd) {
-#pragma unroll
-        for (int x = 0; x < NPASS; x++)
-#pragma unroll
-          for (int i2 = 0; i2 < 8; i2++)
-#pragma unroll
-            for (int e = 0; e < 2 * NR; e++) o[x][i2][e] *= corr[e >> 1];
-        for (int k = 0; k < KW; k++) {
-          float pk[NR];
-#pragma unroll
-          for (int rr = 0; rr < NR; rr++) {
-            float mine = 0.f;
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-              for (int e = 0; e < 2; e++)
-                if (k == 8 * t + 2 * cl + e) mine = pr[rr][t][e];
-            pk[rr] = __shfl_sync(~0u, mine, (lane & ~3) | ((k >> 1) & 3));
-          }
-          const T* vr = reinterpret_cast<const T*>(vt + k * C::ROWB);
-#pragma unroll
-          for (int x = 0; x < NPASS; x++)
-#pragma unroll
-            for (int i2 = 0; i2 < 8; i2++)
-#pragma unroll
-              for (int e = 0; e < 2; e++) {
-                // feature of accumulator (x, i2, column 2 cl + e)
-                const int d = F32 ? x * 64 + (i2 >> 2) * 32 + (2 * cl + e) * 4 + (i2 & 3)
-                                  : x * 64 + (2 * cl + e) * 8 + i2;
-                constexpr int PC = 16 / (int)sizeof(T);
-                const int dd = ((d / PC) ^ (((k >> 1) & 3) << 1)) * PC + d % PC;
-                const float v = (float)vr[dd];
-#pragma unroll
-                for (int rr = 0; rr < NR; rr++)
-                  if (pk[rr] != 0.f) o[x][i2][2 * rr + e] = fmaf(pk[rr], v, o[x][i2][2 * rr + e]);
-              }
-        }
-        continue;
-      }
-
-      // o = o corr + p . v, the products of a tile in accumulators of their own:
-      // the tensor cores' sums are cut off, not rounded, and over a long run of
-      // tiles that adds up (1.5e-6 of the result over 131000 keys, against 0.5e-6
-      // so)
-      auto add = [&](float(&acc)[2 * NR], const float(&d)[4]) {
-        if constexpr (R == 8) {
-          acc[0] = fmaf(acc[0], corr[0], d[0] + d[2]);
-          acc[1] = fmaf(acc[1], corr[0], d[1] + d[3]);
-        } else {
-          acc[0] = fmaf(acc[0], corr[0], d[0]);
-          acc[1] = fmaf(acc[1], corr[0], d[1]);
-          acc[2] = fmaf(acc[2], corr[NR - 1], d[2]);
-          acc[3] = fmaf(acc[3], corr[NR - 1], d[3]);
-        }
-      };
-      if constexpr (F32) {
-        uint4 pa[2];
-        {
-          uint32_t w0[2], w1[2];
-          Split<float>::one(pr[0][0][0], w0);
-          Split<float>::one(pr[0][0][1], w1);
-          if (R == 8) {
-            pa[0] = make_uint4(w0[0], w0[1], w1[0], w1[1]);
-          } else {
-            uint32_t y0[2], y1[2];
-            Split<float>::one(pr[NR - 1][0][0], y0);
-            Split<float>::one(pr[NR - 1][0][1], y1);
-            pa[0] = make_uint4(w0[0], y0[0], w1[0], y1[0]);
-            pa[1] = make_uint4(w0[1], y0[1], w1[1], y1[1]);
-          }
-        }
-#pragma unroll
-        for (int x = 0; x < DP / 32; x++) {
-          const int ch = row + 8 * x;
-          const uint4 v0 = *reinterpret_cast<const uint4*>(vt + (2 * cl) * C::ROWB +
-                                                           ((ch ^ (cl << 1)) << 4));
-          const uint4 v1 = *reinterpret_cast<const uint4*>(vt + (2 * cl + 1) * C::ROWB +
-                                                           ((ch ^ (cl << 1)) << 4));
-          const uint32_t a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            uint32_t h0[2], h1[2];
-            Split<float>::one(__uint_as_float(a0[e]), h0);
-            Split<float>::one(__uint_as_float(a1[e]), h1);
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_1688(d, pa[0], h0[0], h1[0]);
-            mma_1688(d, pa[0], h0[1], h1[1]);
-            if (R == 16) mma_1688(d, pa[1], h0[0], h1[0]);
-            add(o[x >> 1][(x & 1) * 4 + e], d);
-          }
-        }
-      } else {
-        uint4 pa[C::QP];
-        {
-          uint32_t w0[PARTS], w1[PARTS];
-          Split<T>::pair(pr[0][0][0], pr[0][0][1], w0);
-          Split<T>::pair(pr[0][NT - 1][0], pr[0][NT - 1][1], w1);
-          if (R == 8) {
-            pa[0] = make_uint4(w0[0], w0[1], w1[0], w1[1]);
-            if (PARTS == 3) pa[C::QP - 1] = make_uint4(w0[PARTS - 1], 0u, w1[PARTS - 1], 0u);
-          } else {
-            uint32_t y0[PARTS], y1[PARTS];
-            Split<T>::pair(pr[NR - 1][0][0], pr[NR - 1][0][1], y0);
-            Split<T>::pair(pr[NR - 1][NT - 1][0], pr[NR - 1][NT - 1][1], y1);
-#pragma unroll
-            for (int pt = 0; pt < PARTS; pt++)
-              pa[pt < C::QP ? pt : 0] = make_uint4(w0[pt], y0[pt], w1[pt], y1[pt]);
-          }
-        }
-#pragma unroll
-        for (int x = 0; x < NPASS; x++) {
-          const int ch = row + 8 * x;
-          uint4 v[4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int r = 2 * cl + (e & 1) + 8 * (e >> 1);
-            v[e] = *reinterpret_cast<const uint4*>(vt + r * C::ROWB + ((ch ^ (cl << 1)) << 4));
-          }
-          const uint32_t a0[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
-          const uint32_t a1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
-          const uint32_t a8[4] = {v[2].x, v[2].y, v[2].z, v[2].w};
-          const uint32_t a9[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
-            const uint32_t b0 = __byte_perm(a0[e >> 1], a1[e >> 1], sel);
-            const uint32_t b1 = __byte_perm(a8[e >> 1], a9[e >> 1], sel);
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int pt = 0; pt < C::QP; pt++) mma_16816(d, pa[pt], b0, b1, T());
-            add(o[x][e], d);
-          }
-        }
-      }
+      stream_step<T, DP, R>(qs, kt, vt, valid, base, fac, pos, pos_lo, pos_hi, a.window,
+                            a.softcap > 0.f, p.t_mul, m, l, o);
     }
 
     // ---- the segment's end: each warp hands over its rows' state, the output in the

@@ -31,7 +31,7 @@
 
 #include <type_traits>
 
-#include "paged_stream.cuh"
+#include "paged_segments.cuh"
 #include "tc.cuh"
 
 namespace ortc {
@@ -64,67 +64,6 @@ struct TileArgs {
   int tma_rows = 0;
   CUtensorMap key, value;
 };
-
-struct TilePos {
-  int b, rt, g;
-  int row0, count, past;
-  int lo, hi, nt, nrt;  // keys and blocks of this segment (lo a multiple of `align`); row tiles
-  int len;              // keys it counts as in the list (the causal border unclamped)
-  // the sequence: the first key of its row tiles (aligned), tiles that start there
-  int base, ramp;
-};
-
-// Sets the sequence of `s`; its number of row tiles (0: not this kernel's).
-__device__ __forceinline__ int tile_seq(const StreamArgs& p, TilePos& s, int b, int min_past,
-                                        int TT, int align) {
-  const PagedAttnArgs& a = p.a;
-  s.b = b;
-  s.nrt = 0;
-  if (p.prefix) {
-    s.row0 = 0, s.past = 0;
-    s.count = max(0, min(a.c.cu[a.c.batch], a.c.num_tokens));
-    s.base = (a.window ? min(a.shared, max(0, min_past + 1 - a.window)) : 0) & -align;
-  } else {
-    const PagedSeq q = paged_seq(a.c, b, a.max_seq, a.shared);
-    s.row0 = q.row0, s.count = q.count, s.past = q.past;
-    if ((int64_t)q.count * a.group <= p.max_rows) return 0;
-    s.base = a.shared & -align;
-  }
-  s.nrt = (s.count + TT - 1) / TT;
-  s.ramp = s.nrt;
-  if (!p.prefix && a.window) {
-    const long long x = (long long)s.base + a.window - 1 - s.past;
-    s.ramp = x < 0 ? 0 : (int)min((long long)s.nrt, x / TT + 1);
-  }
-  return s.nrt;
-}
-
-// Keys that row tiles 0 .. r - 1 of one KV head count as, with `extra` each.
-__device__ __forceinline__ long long tile_sum(const StreamArgs& p, const TilePos& s, int r, int TT,
-                                              int align, int extra) {
-  if (p.prefix) return (long long)r * (max(1, p.a.shared - s.base) + extra);
-  const long long f = min(r, s.ramp), c = r - f;
-  return f * (s.past - s.base) + TT * (f * (f + 1) / 2) + c * (TT + p.a.window + align - 2) +
-         (long long)r * extra;
-}
-
-// Sets the segment (rt, g) of the sequence of `s`.
-template <int KB>
-__device__ __forceinline__ void tile_segment(const StreamArgs& p, TilePos& s, int rt, int g,
-                                             int TT, int align) {
-  s.rt = rt, s.g = g;
-  if (p.prefix) {
-    s.lo = s.base, s.hi = p.a.shared;
-    s.len = max(1, s.hi - s.lo);
-  } else {
-    const int t0 = s.past + rt * TT;
-    const bool ramp = rt < s.ramp;
-    s.lo = ramp ? s.base : (t0 + 1 - p.a.window) & -align;
-    s.hi = min(s.past + s.count, t0 + TT);
-    s.len = ramp ? t0 + TT - s.base : TT + p.a.window + align - 2;
-  }
-  s.nt = max(1, (s.hi - s.lo + KB - 1) / KB);
-}
 
 __device__ __forceinline__ void bar_sync(int id, int n) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
@@ -218,115 +157,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const PagedAttnArgs& a = p.a;
   const PagedView& c = a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int D = c.D, G = c.kv_heads, nb = p.prefix ? 1 : c.batch, TT = 128 / a.group;
+  const int D = c.D, TT = 128 / a.group;
   const int rows_tma = args.tma_rows, align = max(1, rows_tma);
 
   // ---- this CTA's run
-  int min_past = 0;
-  int* s_min = reinterpret_cast<int*>(stats);
-  if (p.prefix && a.window) {
-    min_past = INT_MAX / 2;
-    for (int b = tid; b < c.batch; b += kTileThreads)
-      if (c.cu[b + 1] > c.cu[b]) min_past = min(min_past, max(0, c.past[b]));
-    min_past = __reduce_min_sync(~0u, min_past);
-    if (lane == 0) s_min[warp] = min_past;
-    __syncthreads();
-    for (int i = 0; i < kTileThreads / 32; i++) min_past = min(min_past, s_min[i]);
-    __syncthreads();
-  }
-  long long* s_scan = reinterpret_cast<long long*>(stats);  // [12], then the start and sequence
-  long long total = 0, u0 = 0, u1 = 0;
-  int runs = 1;
-  for (int pass = 0; pass < 2; pass++) {  // the total, then the sequence of u0
-    long long base = 0;
-    for (int b0 = 0; b0 < nb; b0 += kTileThreads) {
-      TilePos t;
-      long long n = 0;
-      if (b0 + tid < nb) {
-        const int nrt = tile_seq(p, t, b0 + tid, min_past, TT, align);
-        if (nrt) n = tile_sum(p, t, nrt, TT, align, EX) * G;
-      }
-      long long x = n;
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(~0u, x, o);
-        if (lane >= o) x += y;
-      }
-      if (lane == 31) s_scan[warp] = x;
-      __syncthreads();
-      long long all = 0, before = 0;
-      for (int i = 0; i < kTileThreads / 32; i++) {
-        if (i < warp) before += s_scan[i];
-        all += s_scan[i];
-      }
-      if (pass == 1) {
-        const long long start = base + before + x - n;
-        if (n && start <= u0 && u0 < start + n) {
-          s_scan[16] = start;
-          s_scan[17] = b0 + tid;
-        }
-      }
-      base += all;
-      __syncthreads();
-    }
-    if (pass == 0) {
-      total = base;
-      if (total == 0) return;
-      runs = (int)min((long long)gridDim.x, max(1ll, total / KB));  // a run holds a block at least
-      if ((int)blockIdx.x >= runs) return;
-      u0 = total * blockIdx.x / runs;
-      u1 = total * (blockIdx.x + 1) / runs;
-    }
-  }
-  // the segment and block of u0; each role walks the list from here
-  TilePos cur;
-  long long seg;  // place of block 0 of the segment
-  int k0;
-  {
-    const long long off = u0 - s_scan[16];
-    tile_seq(p, cur, (int)s_scan[17], min_past, TT, align);
-    int lo = 0, hi = cur.nrt;  // the last row tile that starts at or before off
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (tile_sum(p, cur, mid, TT, align, EX) * G <= off)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    tile_segment<KB>(p, cur, lo, 0, TT, align);
-    const long long rem = off - tile_sum(p, cur, lo, TT, align, EX) * G, each = cur.len + EX;
-    cur.g = (int)(rem / each);
-    const long long in = rem - cur.g * each - EX;
-    seg = u0 - in;
-    k0 = in <= 0 ? 0 : (int)((in + KB - 1) / KB);
-  }
-  // to the next segment with a block in this run; false: none
-  auto next = [&](TilePos& s, long long& at, int& first) {
-    for (;;) {
-      at += s.len + EX;
-      if (at >= u1) return false;
-      first = 0;
-      if (s.g + 1 < G) {
-        tile_segment<KB>(p, s, s.rt, s.g + 1, TT, align);
-        return true;
-      }
-      if (s.rt + 1 < s.nrt) {
-        tile_segment<KB>(p, s, s.rt + 1, 0, TT, align);
-        return true;
-      }
-      int b = s.b + 1;
-      while (b < nb && !tile_seq(p, s, b, min_past, TT, align)) b++;
-      if (b >= nb) return false;
-      tile_segment<KB>(p, s, 0, 0, TT, align);
-      return true;
-    }
-  };
-  auto blocks = [&](const TilePos& s, long long at, int first) {
-    return (int)min((long long)s.nt, (u1 - at + KB - 1) / KB) - first;
-  };
-  if (seg + (long long)k0 * KB >= u1 || k0 >= cur.nt) {  // no block of this segment in the run
-    if (!next(cur, seg, k0)) return;
-  }
-  __syncthreads();  // s_scan has been read
+  TileRun<KB, EX> run;
+  if (!run.plan(p, TT, align, stats)) return;
+  const long long total = run.total;
+  const int runs = run.runs;
+  // the segment and its first block here; each role walks the list from here
+  TilePos cur = run.cur;
+  long long seg = run.seg;  // place of block 0 of the segment
+  int k0 = run.k0;
+  auto next = [&](TilePos& s, long long& at, int& first) { return run.next(p, s, at, first); };
+  auto blocks = [&](const TilePos& s, long long at, int first) { return run.blocks(s, at, first); };
 
   if (tid == 0) {
     for (int i = 0; i < NK; i++) mbar_init(kfull + i, rows_tma ? 1 : 3), mbar_init(kempty + i, 1);
@@ -652,17 +496,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         pos = all_hi = all_lo = INT_MAX / 2;
         if (a.window) {
           all_hi = -1;  // rows of different sequences: look at each
-          if (has) {
-            int lo = 0, hi = c.batch;
-            while (lo < hi) {
-              const int mid = (lo + hi) >> 1;
-              if (c.cu[mid + 1] <= tok)
-                lo = mid + 1;
-              else
-                hi = mid;
-            }
-            if (lo < c.batch) pos = c.past[lo] + tok - c.cu[lo];
-          }
+          if (has) pos = prefix_position(c, tok);
         }
       } else if (has) {
         pos = cur.past + tok;
@@ -910,10 +744,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       bar_sync(1, 256);
       const bool whole = n == cur.nt;
       const int slot = 2 * blockIdx.x + (k0 ? 0 : 1);
-      auto place = [&](int r) {
-        const int t = p.group_div.div(r);
-        return (int64_t)(cur.row0 + tok0 + t) * a.heads + cur.g * a.group + r - t * a.group;
-      };
       auto write_row = [&](int64_t to, float M, float L, const float (&v)[DP / 32]) {
         const float2 f = paged_row_scale(p, to, M, L);
         float* dst = (p.prefix ? p.pre_o : a.out) + to * D;
@@ -938,7 +768,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           for (int x = 0; x < NX; x++) p.part_o[to * DP + lane + 32 * x] = v[x];
           if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + to * 2) = ml;
         } else {
-          write_row(place(r), ml.x, ml.y, v);
+          write_row(tile_place(p, cur, TT, r), ml.x, ml.y, v);
         }
       }
       if (!whole) {
@@ -949,34 +779,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (tid == 0) *s_last = atom_add_acq_rel_gpu(p.tickets + c0, 1u) == (unsigned)(np - 1);
         bar_sync(1, 256);
         if (*s_last) {
-          for (int r = warp; r < rows_here; r += 8) {
-            auto piece = [&](int i) {
-              return (int64_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * 128 + r;
-            };
-            float M = -INFINITY;
-            for (int i = lane; i < np; i += 32) M = fmaxf(M, __ldcg(p.part_ml + piece(i) * 2));
-            for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, x));
-            const float mb = M == -INFINITY ? 0.f : M;
-            float L = 0.f, v[DP / 32];
-#pragma unroll
-            for (int x = 0; x < DP / 32; x++) v[x] = 0.f;
-            for (int i0 = 0; i0 < np; i0 += 32) {
-              float2 q = make_float2(-INFINITY, 0.f);
-              if (i0 + lane < np)
-                q = __ldcg(reinterpret_cast<const float2*>(p.part_ml + piece(i0 + lane) * 2));
-              const float f = ex2(q.x - mb);
-              L = fmaf(f, q.y, L);
-              for (int i = 0; i < min(32, np - i0); i++) {
-                const float w = __shfl_sync(~0u, f, i);
-#pragma unroll
-                for (int x = 0; x < DP / 32; x++)
-                  if (lane + 32 * x < D)
-                    v[x] = fmaf(w, __ldcg(p.part_o + piece(i0 + i) * DP + lane + 32 * x), v[x]);
-              }
-            }
-            for (int x = 16; x; x >>= 1) L += __shfl_xor_sync(~0u, L, x);
-            write_row(place(r), M, L, v);
-          }
+          tile_join<DP>(p, cur, TT, c0, np, rows_here, warp, 8);
           if (tid == 0) p.tickets[c0] = 0u;
         }
       }
