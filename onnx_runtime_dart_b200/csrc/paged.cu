@@ -6,6 +6,7 @@
 #include <map>
 #include <memory>
 #include <mutex>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -164,6 +165,9 @@ struct AppendArgs {
   const float* sin = nullptr;
   int half = 0, interleaved = 0;
   int64_t max_pos = 0;
+  // filled by the launch
+  FastDiv page_div, piece_div;
+  int parts = 1;  // CTAs of a token
 };
 
 template <typename T>
@@ -181,36 +185,53 @@ __device__ __forceinline__ __nv_bfloat16 to_cache<__nv_bfloat16>(double x) {
   return __double2bfloat16(x);
 }
 
-// One CTA per token: every feature of the token's query, key and value heads.
+// The token's sequence, position and row offset, by one warp; b < 0: none, or left out.
+struct AppendPlace {
+  int b, pos;
+  int64_t off;
+};
+__device__ __forceinline__ AppendPlace append_place(const AppendArgs& a, int t) {
+  const PagedView& c = a.c;
+  const int b = paged_find(c, t);
+  AppendPlace r = {-1, 0, -1};
+  const PagedSeq s = b < c.batch ? paged_seq(c, b, INT_MAX, 0) : PagedSeq{0, 0, 0};
+  if (t < s.row0 || t >= s.row0 + s.count) return r;
+  r.pos = s.past + t - s.row0;
+  if (a.half && r.pos >= a.max_pos) {
+    record_error(c.err, KERR_PAGED_POSITION);
+    return r;
+  }
+  r.b = b;
+  const int pg = a.page_div.div(r.pos), page = __ldg(c.table + (int64_t)b * c.max_pages + pg);
+  if (page < 0 || page >= c.num_pages)
+    record_error(c.err, KERR_PAGED_PAGE);
+  else
+    r.off = page * c.page_elems + (int64_t)(r.pos - pg * c.page_size) * c.row_elems;
+  return r;
+}
+
+// Sequences that no token of the call reaches are checked too (one CTA).
+__device__ __forceinline__ void append_check_all(const PagedView& c) {
+  for (int b = threadIdx.x; b < c.batch; b += blockDim.x) paged_seq(c, b, INT_MAX, 0);
+}
+
+// Any strides, alignments and rotated widths: a CTA per token, a thread per pair.
 template <typename T>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256) append_any_kernel(const __grid_constant__ AppendArgs a) {
+  griddep_launch_dependents();
+  griddep_wait();
   const PagedView& c = a.c;
   const int t = blockIdx.x;
-  if (t == 0)  // sequences that no token of the call reaches are checked too
-    for (int b = threadIdx.x; b < c.batch; b += blockDim.x) paged_seq(c, b, INT_MAX, 0);
-  __shared__ int s_b, s_pos;
-  __shared__ int64_t s_off;
+  if (t == 0) append_check_all(c);
+  __shared__ AppendPlace at;
   if (threadIdx.x < 32) {
-    const int b = paged_find(c, t);
-    if (threadIdx.x == 0) {
-      s_b = -1;
-      const PagedSeq s = b < c.batch ? paged_seq(c, b, INT_MAX, 0) : PagedSeq{0, 0, 0};
-      if (t >= s.row0 && t < s.row0 + s.count) {
-        const int pos = s.past + t - s.row0;
-        if (a.half && pos >= a.max_pos) {
-          record_error(c.err, KERR_PAGED_POSITION);
-        } else {
-          s_b = b;
-          s_pos = pos;
-          s_off = paged_row(c, b, pos);
-        }
-      }
-    }
+    const AppendPlace r = append_place(a, t);
+    if (threadIdx.x == 0) at = r;
   }
   __syncthreads();
-  if (s_b < 0) return;
-  const int pos = s_pos, D = c.D, half = a.half;
-  const int64_t off = s_off;
+  if (at.b < 0) return;
+  const int pos = at.pos, D = c.D, half = a.half;
+  const int64_t off = at.off;
   const float* cs = a.cos + (int64_t)pos * half;
   const float* sn = a.sin + (int64_t)pos * half;
   const int per = D - half;  // pairs, then the features behind them
@@ -237,8 +258,7 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
     h -= a.heads;
     const bool is_v = h >= c.kv_heads;
     if (is_v) h -= c.kv_heads;
-    const float* src =
-        (is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride) + (int64_t)h * D;
+    const float* src = (is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride) + (int64_t)h * D;
     T* dst = static_cast<T*>(is_v ? c.value : c.key) + off + (int64_t)h * D;
     const double x0 = src[a0], x1 = src[a1];
     if (pair && !is_v) {
@@ -251,20 +271,121 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
   }
 }
 
-int launch_append(const AppendArgs& a, cudaStream_t st, int64_t* launches) {
-  switch (a.c.type) {
-    case ORT_CUDA_CACHE_F32:
-      append_kernel<float><<<a.c.num_tokens, 256, 0, st>>>(a);
-      break;
-    case ORT_CUDA_CACHE_F16:
-      append_kernel<__half><<<a.c.num_tokens, 256, 0, st>>>(a);
-      break;
-    default:
-      append_kernel<__nv_bfloat16><<<a.c.num_tokens, 256, 0, st>>>(a);
+// 16-byte loads: a thread takes pieces of 8 features (4 pairs, or 8 features that are
+// not rotated) of a token's heads, IT of them, and has its loads in flight while one
+// warp finds the token's place (three dependent loads).  Bound by memory: 8676 tokens
+// of 48 heads of 128 (393 MB) run at MEASURED_RATE.  RoPE in double, as the dense
+// attention's, rounded once.
+template <typename T, int IT>
+__global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ AppendArgs a) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const PagedView& c = a.c;
+  const int t = blockIdx.x / a.parts, part = blockIdx.x - t * a.parts;
+  if (blockIdx.x == 0) append_check_all(c);
+  const int D = c.D, half = a.half, ppc = D >> 3;  // pieces of a head
+  const int n = (a.heads + 2 * c.kv_heads) * ppc;
+  float x[IT][8];
+  int first[IT], second[IT], head[IT];  // features of x[0..3] and x[4..7]; -1: no piece
+#pragma unroll
+  for (int i = 0; i < IT; i++) {
+    const int e = (part * IT + i) * 128 + threadIdx.x;
+    head[i] = -1;
+    if (e >= n) continue;
+    const int h = a.piece_div.div(e), y = e - h * ppc;
+    head[i] = h;
+    const bool turned = h < a.heads + c.kv_heads && 8 * y < 2 * half;
+    if (turned && !a.interleaved) {  // (i, i + half)
+      first[i] = 4 * y, second[i] = 4 * y + half;
+    } else {
+      first[i] = 8 * y, second[i] = 8 * y + 4;
+    }
+    const float* src = h < a.heads ? a.q + t * a.q_stride + (int64_t)h * D
+                       : h < a.heads + c.kv_heads
+                           ? a.k + t * a.k_stride + (int64_t)(h - a.heads) * D
+                           : a.v + t * a.v_stride + (int64_t)(h - a.heads - c.kv_heads) * D;
+    // (not through the read-only path: Q may be rotated in place)
+    *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(src + first[i]);
+    *reinterpret_cast<float4*>(x[i] + 4) = *reinterpret_cast<const float4*>(src + second[i]);
   }
-  ORTC_CUDA(cudaGetLastError());
-  (*launches)++;
-  return ORT_CUDA_OK;
+  __shared__ AppendPlace at;
+  if (threadIdx.x < 32) {
+    const AppendPlace r = append_place(a, t);
+    if (threadIdx.x == 0) at = r;
+  }
+  __syncthreads();
+  if (at.b < 0) return;
+  const int64_t off = at.off, cs0 = (int64_t)at.pos * half;
+#pragma unroll
+  for (int i = 0; i < IT; i++) {
+    if (head[i] < 0) continue;
+    const int h = head[i];
+    const bool is_q = h < a.heads, is_v = h >= a.heads + c.kv_heads;
+    if (!is_q && off < 0) continue;
+    double y[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = x[i][e];
+    const int pair0 = a.interleaved ? first[i] >> 1 : first[i];
+    if (!is_v && pair0 < half && first[i] < 2 * half) {
+      const float4 cv = __ldg(reinterpret_cast<const float4*>(a.cos + cs0 + pair0));
+      const float4 sv = __ldg(reinterpret_cast<const float4*>(a.sin + cs0 + pair0));
+      const double cd[4] = {cv.x, cv.y, cv.z, cv.w}, sd[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        double& u = a.interleaved ? y[2 * e] : y[e];
+        double& v = a.interleaved ? y[2 * e + 1] : y[e + 4];
+        const double u0 = u, v0 = v;
+        u = u0 * cd[e] - v0 * sd[e];
+        v = v0 * cd[e] + u0 * sd[e];
+      }
+    }
+    if (is_q) {
+      float* dst = a.q_out + ((int64_t)t * a.heads + h) * D;
+      *reinterpret_cast<float4*>(dst + first[i]) =
+          make_float4((float)y[0], (float)y[1], (float)y[2], (float)y[3]);
+      *reinterpret_cast<float4*>(dst + second[i]) =
+          make_float4((float)y[4], (float)y[5], (float)y[6], (float)y[7]);
+      continue;
+    }
+    T* dst = static_cast<T*>(is_v ? c.value : c.key) + off +
+             (int64_t)(h - a.heads - (is_v ? c.kv_heads : 0)) * D;
+    __align__(16) T w[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) w[e] = to_cache<T>(y[e]);
+    using H = std::conditional_t<sizeof(T) == 4, float4, uint2>;  // four features
+    *reinterpret_cast<H*>(dst + first[i]) = *reinterpret_cast<const H*>(w);
+    *reinterpret_cast<H*>(dst + second[i]) = *reinterpret_cast<const H*>(w + 4);
+  }
+}
+
+template <typename T>
+int launch_append_type(AppendArgs& a, cudaStream_t st) {
+  const PagedView& c = a.c;
+  auto ok = [](const void* p, int64_t stride) {
+    return ((uintptr_t)p & 15) == 0 && stride % 4 == 0;
+  };
+  const bool vec = a.half % 4 == 0 && ok(a.k, a.k_stride) && ok(a.v, a.v_stride) &&
+                   ok(a.q, a.q_stride) && ok(a.q_out, 0) && ok(a.cos, 0) && ok(a.sin, 0);
+  if (!vec) return launch_overlapped(append_any_kernel<T>, c.num_tokens, 256, 0, st, a);
+  const int pieces = (a.heads + 2 * c.kv_heads) * (c.D / 8);
+  a.piece_div.set((uint32_t)(c.D / 8));
+  // one piece a thread until the CTAs fill the device, then three
+  const int it = (int64_t)c.num_tokens * pieces > 148 * 2048 ? 3 : 1;
+  a.parts = (pieces + 128 * it - 1) / (128 * it);
+  ORTC_CHECK((int64_t)c.num_tokens * a.parts <= INT_MAX, ORT_CUDA_ERR_INVALID_ARG,
+             "paged append: sizes too large");
+  const unsigned grid = (unsigned)(c.num_tokens * a.parts);
+  return it == 3 ? launch_overlapped(append_kernel<T, 3>, grid, 128, 0, st, a)
+                 : launch_overlapped(append_kernel<T, 1>, grid, 128, 0, st, a);
+}
+
+int launch_append(AppendArgs& a, cudaStream_t st, int64_t* launches) {
+  a.page_div.set((uint32_t)a.c.page_size);
+  const int rc = a.c.type == ORT_CUDA_CACHE_F32   ? launch_append_type<float>(a, st)
+                 : a.c.type == ORT_CUDA_CACHE_F16 ? launch_append_type<__half>(a, st)
+                                                  : launch_append_type<__nv_bfloat16>(a, st);
+  if (rc == ORT_CUDA_OK) (*launches)++;
+  return rc;
 }
 
 // Checks what the host can see of a cache and fills the kernels' view.

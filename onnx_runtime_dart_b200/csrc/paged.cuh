@@ -56,16 +56,42 @@ __device__ __forceinline__ int paged_find(const PagedView& v, int t) {
   return v.batch;
 }
 
-// Offset in elements of position `pos` of sequence b (KV head 0) in the key
-// and value pages, -1 when its page is outside the cache.
-__device__ __forceinline__ int64_t paged_row(const PagedView& v, int b, int pos) {
-  const int pg = pos / v.page_size;
-  const int page = __ldg(v.table + (int64_t)b * v.max_pages + pg);
-  if (page < 0 || page >= v.num_pages) {
-    record_error(v.err, KERR_PAGED_PAGE);
-    return -1;
+// floor(x / d) for 0 <= x < 2^31.
+struct FastDiv {
+  uint32_t mul = 0, shift = 0;  // mul 0: a power of two
+  __host__ void set(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) s++;
+    if ((1ull << s) == d) {
+      mul = 0, shift = s;
+    } else {  // ceil(2^(31 + s) / d) < 2^32: exact for 31-bit x
+      mul = (uint32_t)(((1ull << (31 + s)) + d - 1) / d);
+      shift = s - 1;
+    }
   }
-  return page * v.page_elems + (int64_t)(pos - pg * v.page_size) * v.row_elems;
+  __device__ __forceinline__ int div(int x) const {
+    return mul ? (int)(__umulhi((uint32_t)x, mul) >> shift) : x >> shift;
+  }
+};
+
+// Launches with programmatic stream serialisation: the kernel may start while the
+// one before it ends (every kernel here waits, griddep_wait, before it touches
+// memory), which takes the launch's latency off a step's chain of small kernels.
+template <typename... P, typename... A>
+int launch_overlapped(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem,
+                      cudaStream_t st, const A&... args) {
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  ORTC_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return ORT_CUDA_OK;
 }
 
 struct PagedAttnArgs {

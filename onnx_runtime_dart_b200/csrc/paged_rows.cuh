@@ -40,6 +40,8 @@ __global__ void __launch_bounds__(256, 1) paged_rows_kernel(const __grid_constan
   unsigned char* ring = smem;
   uint4* qs = reinterpret_cast<uint4*>(smem + NS * C::STAGE + w * C::QW);  // this warp's
 
+  griddep_launch_dependents();
+  griddep_wait();
   TileRun<KB, C::EXTRA> run;
   if (!run.plan(p, TT, 1, s_plan)) return;
   TilePos cur = run.cur;
@@ -140,14 +142,10 @@ __global__ void __launch_bounds__(256, 1) paged_rows_kernel(const __grid_constan
       commit();
       const unsigned char* kt = ring + (i % NS) * C::STAGE;
       const unsigned there = __ballot_sync(~0u, s_ok[i % NS][lane] != 0);
-#pragma unroll 1
-      for (int y = 0; y < KB / 8; y++) {
-        const int base = cur.lo + (k0 + i) * KB + 8 * y;
-        const unsigned valid = (there >> (8 * y)) & 0xffu;
-        if (valid == 0 || base > pos_hi || (a.window && base + 7 <= pos_lo - a.window)) continue;
-        stream_step<float, DP, 16>(qs, kt + 8 * y * ROWB, kt + (KB + 8 * y) * ROWB, valid, base, fac,
-                                   pos, pos_lo, pos_hi, a.window, a.softcap > 0.f, p.t_mul, m, l, o);
-      }
+      const int base = cur.lo + (k0 + i) * KB;
+      if (there == 0 || base > pos_hi || (a.window && base + KB - 1 <= pos_lo - a.window)) continue;
+      stream_step<float, DP, 16, KB / 8>(qs, kt, kt + KB * ROWB, there, base, fac, pos, pos_lo,
+                                         pos_hi, a.window, a.softcap > 0.f, p.t_mul, m, l, o);
     }
 
     const bool whole = n == cur.nt;

@@ -36,24 +36,6 @@
 
 namespace ortc {
 
-// floor(x / d) for 0 <= x < 2^31.
-struct FastDiv {
-  uint32_t mul = 0, shift = 0;  // mul 0: a power of two
-  __host__ void set(uint32_t d) {
-    uint32_t s = 0;
-    while ((1ull << s) < d) s++;
-    if ((1ull << s) == d) {
-      mul = 0, shift = s;
-    } else {  // ceil(2^(31 + s) / d) < 2^32: exact for 31-bit x
-      mul = (uint32_t)(((1ull << (31 + s)) + d - 1) / d);
-      shift = s - 1;
-    }
-  }
-  __device__ __forceinline__ int div(int x) const {
-    return mul ? (int)(__umulhi((uint32_t)x, mul) >> shift) : x >> shift;
-  }
-};
-
 struct StreamArgs {
   PagedAttnArgs a;
   FastDiv page_div, group_div;
@@ -219,11 +201,11 @@ __device__ __forceinline__ int stream_seq(const StreamArgs& p, StreamPos& s, int
   return (s.nt + EXTRA) * s.nrt;
 }
 
-// One step of a warp: KW keys at `base` (bit r of `valid`: key r is there) in
+// One step of a warp: 8 NT keys at `base` (bit r of `valid`: key r is there) in
 // shared memory at kt, vt against its R rows, whose operands are qs, score factors
 // fac, positions pos (from pos_lo to pos_hi over the rows); m, l, o: the rows'
 // running maximum, this lane's part of the sum, output.
-template <typename T, int DP, int R>
+template <typename T, int DP, int R, int NT = StreamCfg<T, DP, R>::KW / 8>
 __device__ __forceinline__ void stream_step(const uint4* qs, const unsigned char* kt,
                                             const unsigned char* vt, unsigned valid, int base,
                                             const float (&fac)[R / 8], const int (&pos)[R / 8],
@@ -232,11 +214,11 @@ __device__ __forceinline__ void stream_step(const uint4* qs, const unsigned char
                                             float (&o)[DP / 64][8][R / 4]) {
   using C = StreamCfg<T, DP, R>;
   constexpr bool F32 = C::F32;
-  constexpr int KW = C::KW, CHP = C::CHP, KS = C::KS, PARTS = Split<T>::PARTS, NPASS = DP / 64;
+  constexpr int KW = 8 * NT, CHP = C::CHP, KS = C::KS, PARTS = Split<T>::PARTS, NPASS = DP / 64;
   constexpr int NR = R / 8;
+  constexpr unsigned kAll = ~0u >> (32 - KW);
   const int lane = threadIdx.x & 31;
   // scores
-  constexpr int NT = KW / 8;
   float s[NT][2][4];  // two chains of products each
 #pragma unroll
   for (int t = 0; t < NT; t++)
@@ -252,23 +234,28 @@ __device__ __forceinline__ void stream_step(const uint4* qs, const unsigned char
       kv[t] = *reinterpret_cast<const uint4*>(kt + (row + 8 * t) * C::ROWB +
                                               ((ch ^ ((row & 1) << 2)) << 4));
     if constexpr (F32) {
-      uint32_t kh[4], kl[4];
-      const float kx[4] = {__uint_as_float(kv[0].x), __uint_as_float(kv[0].y),
-                           __uint_as_float(kv[0].z), __uint_as_float(kv[0].w)};
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        uint32_t ww[2];
-        Split<float>::one(kx[e], ww);
-        kh[e] = ww[0], kl[e] = ww[1];
-      }
+      uint4 qa[2], ql[2];
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const uint4 qa = qs[(ks + e) * 32 + lane];
-        mma_1688(s[0][e], qa, kh[2 * e], kh[2 * e + 1]);
-        mma_1688(s[0][e], qa, kl[2 * e], kl[2 * e + 1]);
-        if (R == 16) {
-          const uint4 ql = qs[(KS + ks + e) * 32 + lane];
-          mma_1688(s[0][e], ql, kh[2 * e], kh[2 * e + 1]);
+        qa[e] = qs[(ks + e) * 32 + lane];
+        if (R == 16) ql[e] = qs[(KS + ks + e) * 32 + lane];
+      }
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        uint32_t kh[4], kl[4];
+        const float kx[4] = {__uint_as_float(kv[t].x), __uint_as_float(kv[t].y),
+                             __uint_as_float(kv[t].z), __uint_as_float(kv[t].w)};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          uint32_t ww[2];
+          Split<float>::one(kx[e], ww);
+          kh[e] = ww[0], kl[e] = ww[1];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          mma_1688(s[t][e], qa[e], kl[2 * e], kl[2 * e + 1]);
+          if (R == 16) mma_1688(s[t][e], ql[e], kh[2 * e], kh[2 * e + 1]);
+          mma_1688(s[t][e], qa[e], kh[2 * e], kh[2 * e + 1]);
         }
       }
     } else {
@@ -285,7 +272,7 @@ __device__ __forceinline__ void stream_step(const uint4* qs, const unsigned char
   }
 
   // softmax weights; rows (lane / 4) + 8 rr, keys base + 8 t + 2 cl + e
-  const bool full = valid == (1u << KW) - 1 && base + KW - 1 <= pos_lo &&
+  const bool full = valid == kAll && base + KW - 1 <= pos_lo &&
                     (!window || base > pos_hi - window);
   float pr[NR][NT][2];
 #pragma unroll
@@ -412,40 +399,46 @@ __device__ __forceinline__ void stream_step(const uint4* qs, const unsigned char
     }
   };
   if constexpr (F32) {
-    uint4 pa[2];
-    {
+    uint4 pa[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
       uint32_t w0[2], w1[2];
-      Split<float>::one(pr[0][0][0], w0);
-      Split<float>::one(pr[0][0][1], w1);
+      Split<float>::one(pr[0][t][0], w0);
+      Split<float>::one(pr[0][t][1], w1);
       if (R == 8) {
-        pa[0] = make_uint4(w0[0], w0[1], w1[0], w1[1]);
+        pa[t][0] = make_uint4(w0[0], w0[1], w1[0], w1[1]);
       } else {
         uint32_t y0[2], y1[2];
-        Split<float>::one(pr[NR - 1][0][0], y0);
-        Split<float>::one(pr[NR - 1][0][1], y1);
-        pa[0] = make_uint4(w0[0], y0[0], w1[0], y1[0]);
-        pa[1] = make_uint4(w0[1], y0[1], w1[1], y1[1]);
+        Split<float>::one(pr[NR - 1][t][0], y0);
+        Split<float>::one(pr[NR - 1][t][1], y1);
+        pa[t][0] = make_uint4(w0[0], y0[0], w1[0], y1[0]);
+        pa[t][1] = make_uint4(w0[1], y0[1], w1[1], y1[1]);
       }
     }
 #pragma unroll
     for (int x = 0; x < DP / 32; x++) {
       const int ch = row + 8 * x;
-      const uint4 v0 = *reinterpret_cast<const uint4*>(vt + (2 * cl) * C::ROWB +
-                                                       ((ch ^ (cl << 1)) << 4));
-      const uint4 v1 = *reinterpret_cast<const uint4*>(vt + (2 * cl + 1) * C::ROWB +
-                                                       ((ch ^ (cl << 1)) << 4));
-      const uint32_t a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
+      float d[4][4];
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        uint32_t h0[2], h1[2];
-        Split<float>::one(__uint_as_float(a0[e]), h0);
-        Split<float>::one(__uint_as_float(a1[e]), h1);
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
-        mma_1688(d, pa[0], h0[0], h1[0]);
-        mma_1688(d, pa[0], h0[1], h1[1]);
-        if (R == 16) mma_1688(d, pa[1], h0[0], h1[0]);
-        add(o[x >> 1][(x & 1) * 4 + e], d);
+      for (int e = 0; e < 4; e++) d[e][0] = d[e][1] = d[e][2] = d[e][3] = 0.f;
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        const unsigned char* vr = vt + (8 * t + 2 * cl) * C::ROWB + ((ch ^ (cl << 1)) << 4);
+        const uint4 v0 = *reinterpret_cast<const uint4*>(vr);
+        const uint4 v1 = *reinterpret_cast<const uint4*>(vr + C::ROWB);
+        const uint32_t a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          uint32_t h0[2], h1[2];
+          Split<float>::one(__uint_as_float(a0[e]), h0);
+          Split<float>::one(__uint_as_float(a1[e]), h1);
+          mma_1688(d[e], pa[t][0], h0[1], h1[1]);
+          if (R == 16) mma_1688(d[e], pa[t][1], h0[0], h1[0]);
+          mma_1688(d[e], pa[t][0], h0[0], h1[0]);
+        }
       }
+#pragma unroll
+      for (int e = 0; e < 4; e++) add(o[x >> 1][(x & 1) * 4 + e], d[e]);
     }
   } else {
     uint4 pa[C::QP];
@@ -545,6 +538,9 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
   const PagedView& c = a.c;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int D = c.D, G = c.kv_heads, nb = p.prefix ? 1 : c.batch;
+
+  griddep_launch_dependents();
+  griddep_wait();
 
   // ---- this CTA's run of tiles
   int min_past = 0;

@@ -160,6 +160,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int D = c.D, TT = 128 / a.group;
   const int rows_tma = args.tma_rows, align = max(1, rows_tma);
 
+  griddep_launch_dependents();
+  griddep_wait();
   // ---- this CTA's run
   TileRun<KB, EX> run;
   if (!run.plan(p, TT, align, stats)) return;

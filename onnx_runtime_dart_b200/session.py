@@ -117,7 +117,7 @@ class PagedKVCache:
                              "[batch + 1] and past_lens [batch]")
         self.key, self.value = key, value
         self.block_table, self.cu_seqlens, self.past_lens = block_table, cu_seqlens, past_lens
-        self.batch, self.device = batch, key.device
+        self.batch, self.device, self.index = batch, key.device, key.get_device()
         self.kv_heads, self.head_size = int(key.shape[2]), int(key.shape[3])
         self.struct = _lib.PagedCacheStruct(
             key.data_ptr(), value.data_ptr(), block_table.data_ptr(), cu_seqlens.data_ptr(),
@@ -129,11 +129,12 @@ class PagedKVCache:
         """(tensor, row stride) of a float32 activation of `width` features a
         token: rows may lie apart (a slice of a fused projection's output),
         anything else is made contiguous."""
-        if x.device != self.device or not x.is_floating_point():
+        if x.get_device() != self.index or not x.is_floating_point():
             raise ValueError(f"{name} must be a float tensor on {self.device}")
-        if x.ndim < 2 or x.numel() != x.shape[0] * width:
+        shape = x.shape
+        if len(shape) < 2 or x.numel() != shape[0] * width:
             raise ValueError(f"{name} must be [tokens, {width}] (or [tokens, heads, "
-                             f"{self.head_size}]), got {tuple(x.shape)}")
+                             f"{self.head_size}]), got {tuple(shape)}")
         if x.element_size() != 4:
             x = x.float()
         if x.is_contiguous():
@@ -648,17 +649,18 @@ class CudaSession:
 
     # -- paged KV cache ------------------------------------------------------
     def _paged_stream(self, cache: "PagedKVCache"):
-        """Where a paged call runs: on torch's current stream, or, after
-        set_stream(), with that stream current for torch too, so that what the
-        call allocates and converts belongs to it."""
-        import contextlib
+        """The stream of a paged call: None, torch's current stream; or, after
+        set_stream(), a context with that stream current for torch too, so that
+        what the call allocates and converts belongs to it."""
         import torch
-        if cache.device.index != self.device:
+        if cache.index != self.device:
             raise ValueError(f"PagedKVCache is on {cache.device}, the session on cuda:"
                              f"{self.device}")
         if not self._explicit_stream:
-            self._follow_torch_stream()
-            return contextlib.nullcontext()
+            cur = torch._C._cuda_getCurrentRawStream(self.device)
+            if cur != self._followed:
+                self._follow_torch_stream()
+            return None
         if self._stream_ptr in (0, 1):
             return torch.cuda.stream(torch.cuda.default_stream(cache.device))
         return torch.cuda.stream(torch.cuda.ExternalStream(self._stream_ptr, cache.device))
@@ -668,7 +670,7 @@ class CudaSession:
         """The fp32 output of a paged call: `out` checked, or a new tensor."""
         if out is None:
             import torch
-            return torch.empty(like.shape, dtype=torch.float32, device=like.device)
+            return torch.empty_like(like, memory_format=torch.contiguous_format)
         if out.shape != like.shape or out.element_size() != 4 or not out.is_floating_point() or \
                 out.device != like.device or not out.is_contiguous():
             raise ValueError(f"{name} must be a contiguous float32 tensor like the queries")
@@ -681,38 +683,47 @@ class CudaSession:
         the paged cache (ort_cuda_paged_kv_append), with RoPE of the keys and of
         the queries ``q`` when cos/sin caches are given.  Returns the rotated
         queries (``q_out``, which may be ``q`` itself), or None without ``q``."""
+        on = self._paged_stream(cache)
+        if on is not None:
+            with on:
+                return self._paged_kv_append(cache, k, v, q, num_heads, cos_cache, sin_cache,
+                                             rotary_interleaved, q_out)
+        return self._paged_kv_append(cache, k, v, q, num_heads, cos_cache, sin_cache,
+                                     rotary_interleaved, q_out)
+
+    def _paged_kv_append(self, cache, k, v, q, num_heads, cos_cache, sin_cache,
+                         rotary_interleaved, q_out):
         width = cache.kv_heads * cache.head_size
-        with self._paged_stream(cache):
-            k, ks = cache.rows("k", k, width)
-            v, vs = cache.rows("v", v, width)
-            n = int(k.shape[0])
-            if int(v.shape[0]) != n or (q is not None and int(q.shape[0]) != n):
-                raise ValueError("paged_kv_append: q, k and v need the same number of tokens")
-            qp = qs = op = 0
-            if q is not None:
-                rows, qs = cache.rows("q", q, num_heads * cache.head_size)
-                if q_out is q and rows is not q:
-                    raise ValueError("paged_kv_append: only contiguous float32 queries are "
-                                     "rotated in place")
-                q_out = self._paged_out("q_out", q_out, rows)
-                qp, op = rows.data_ptr(), q_out.data_ptr()
-            elif q_out is not None:
-                raise ValueError("paged_kv_append: q_out without q")
-            cp = sp = half = max_pos = 0
-            if (cos_cache is None) != (sin_cache is None):
-                raise ValueError("paged_kv_append: give both cos and sin caches or neither")
-            if cos_cache is not None:
-                for t in (cos_cache, sin_cache):
-                    if t.device != cache.device or t.element_size() != 4 or \
-                            not t.is_floating_point() or not t.is_contiguous() or t.ndim != 2 or \
-                            t.shape != cos_cache.shape:
-                        raise ValueError("paged_kv_append: cos/sin caches must be contiguous "
-                                         "float32 [max_pos, rotary_half] CUDA tensors")
-                cp, sp = cos_cache.data_ptr(), sin_cache.data_ptr()
-                max_pos, half = cos_cache.shape
-            rc = _lib.load().ort_cuda_paged_kv_append(
-                self.handle, cache.ref, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, n, num_heads,
-                cp, sp, half, max_pos, op, _lib.ROTARY_INTERLEAVED if rotary_interleaved else 0)
+        k, ks = cache.rows("k", k, width)
+        v, vs = cache.rows("v", v, width)
+        n = int(k.shape[0])
+        if int(v.shape[0]) != n or (q is not None and int(q.shape[0]) != n):
+            raise ValueError("paged_kv_append: q, k and v need the same number of tokens")
+        qp = qs = op = 0
+        if q is not None:
+            rows, qs = cache.rows("q", q, num_heads * cache.head_size)
+            if q_out is q and rows is not q:
+                raise ValueError("paged_kv_append: only contiguous float32 queries are "
+                                 "rotated in place")
+            q_out = self._paged_out("q_out", q_out, rows)
+            qp, op = rows.data_ptr(), q_out.data_ptr()
+        elif q_out is not None:
+            raise ValueError("paged_kv_append: q_out without q")
+        cp = sp = half = max_pos = 0
+        if (cos_cache is None) != (sin_cache is None):
+            raise ValueError("paged_kv_append: give both cos and sin caches or neither")
+        if cos_cache is not None:
+            for t in (cos_cache, sin_cache):
+                if t.get_device() != cache.index or t.element_size() != 4 or \
+                        not t.is_floating_point() or not t.is_contiguous() or t.ndim != 2 or \
+                        t.shape != cos_cache.shape:
+                    raise ValueError("paged_kv_append: cos/sin caches must be contiguous "
+                                     "float32 [max_pos, rotary_half] CUDA tensors")
+            cp, sp = cos_cache.data_ptr(), sin_cache.data_ptr()
+            max_pos, half = cos_cache.shape
+        rc = _lib.load().ort_cuda_paged_kv_append(
+            self.handle, cache.ref, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, n, num_heads,
+            cp, sp, half, max_pos, op, _lib.ROTARY_INTERLEAVED if rotary_interleaved else 0)
         if rc:
             check(rc, "ort_cuda_paged_kv_append")
         return q_out
@@ -728,14 +739,23 @@ class CudaSession:
         tokens of any one sequence (default: the tokens of the call);
         ``shared_len``: that many first positions are the same in every
         sequence and are read once, through the block table's first row."""
-        with self._paged_stream(cache):
-            q, qs = cache.rows("q", q, num_heads * cache.head_size)
-            out = self._paged_out("out", out, q)
-            n = int(q.shape[0])
-            rc = _lib.load().ort_cuda_paged_attention(
-                self.handle, cache.ref, q.data_ptr(), qs, n, n if max_seq is None else max_seq,
-                num_heads, 0.0 if scale is None else scale, softcap, local_window_size,
-                shared_len, out.data_ptr(), 0)
+        on = self._paged_stream(cache)
+        if on is not None:
+            with on:
+                return self._paged_attention(cache, q, num_heads, max_seq, scale, softcap,
+                                             local_window_size, shared_len, out)
+        return self._paged_attention(cache, q, num_heads, max_seq, scale, softcap,
+                                     local_window_size, shared_len, out)
+
+    def _paged_attention(self, cache, q, num_heads, max_seq, scale, softcap, local_window_size,
+                         shared_len, out):
+        q, qs = cache.rows("q", q, num_heads * cache.head_size)
+        out = self._paged_out("out", out, q)
+        n = int(q.shape[0])
+        rc = _lib.load().ort_cuda_paged_attention(
+            self.handle, cache.ref, q.data_ptr(), qs, n, n if max_seq is None else max_seq,
+            num_heads, 0.0 if scale is None else scale, softcap, local_window_size,
+            shared_len, out.data_ptr(), 0)
         if rc:
             check(rc, "ort_cuda_paged_attention")
         return out
