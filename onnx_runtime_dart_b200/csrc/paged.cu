@@ -170,19 +170,43 @@ struct AppendArgs {
   int parts = 1;  // CTAs of a token
 };
 
+// a b - c d (or + c d), as computed in double and rounded to fp32: the products as
+// pairs of floats (exact), their sum with its error.  About 13 fp32 instructions in
+// place of 4 conversions to and from double, which run at an eighth of the rate.
+// `odd`: rounded to odd instead, so that rounding on to 16 bits rounds once.
+template <bool PLUS, bool ODD>
+__device__ __forceinline__ float rope_sum(float a, float b, float c, float d) {
+  const float p = __fmul_rn(a, b), pe = __fmaf_rn(a, b, -p);
+  if (PLUS) c = -c;
+  const float q = __fmul_rn(c, d), qe = __fmaf_rn(c, d, -q);
+  const float s = __fsub_rn(p, q), z = __fsub_rn(s, p);
+  const float e = __fsub_rn(__fsub_rn(p, __fsub_rn(s, z)), __fadd_rn(q, z));
+  const float t = __fadd_rn(e, __fsub_rn(pe, qe));
+  float r = __fadd_rn(s, t);
+  if (!(t == t)) return s;  // infinities and NaN
+  if (ODD) {
+    const float rest = __fsub_rn(t, __fsub_rn(r, s));
+    const int u = __float_as_int(r);
+    // an even r that is not exact: its neighbour on the side of the rest
+    if (rest != 0.f && !(u & 1) && r != 0.f)
+      r = __int_as_float((rest > 0.f) == (r > 0.f) ? u + 1 : u - 1);
+  }
+  return r;
+}
+
 template <typename T>
-__device__ __forceinline__ T to_cache(double x);
+__device__ __forceinline__ T to_cache(float x);
 template <>
-__device__ __forceinline__ float to_cache<float>(double x) {
-  return (float)x;
+__device__ __forceinline__ float to_cache<float>(float x) {
+  return x;
 }
 template <>
-__device__ __forceinline__ __half to_cache<__half>(double x) {
-  return __double2half(x);
+__device__ __forceinline__ __half to_cache<__half>(float x) {
+  return __float2half_rn(x);
 }
 template <>
-__device__ __forceinline__ __nv_bfloat16 to_cache<__nv_bfloat16>(double x) {
-  return __double2bfloat16(x);
+__device__ __forceinline__ __nv_bfloat16 to_cache<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
 }
 
 // The token's sequence, position and row offset, by one warp; b < 0: none, or left out.
@@ -245,12 +269,12 @@ __global__ void __launch_bounds__(256) append_any_kernel(const __grid_constant__
     if (h < a.heads) {
       const float* src = a.q + t * a.q_stride + (int64_t)h * D;
       float* dst = a.q_out + ((int64_t)t * a.heads + h) * D;
-      const double x0 = src[a0], x1 = src[a1];
+      const float x0 = src[a0], x1 = src[a1];
       if (pair) {
-        dst[a0] = (float)(x0 * cs[i] - x1 * sn[i]);
-        dst[a1] = (float)(x1 * cs[i] + x0 * sn[i]);
+        dst[a0] = rope_sum<false, false>(x0, cs[i], x1, sn[i]);
+        dst[a1] = rope_sum<true, false>(x1, cs[i], x0, sn[i]);
       } else {
-        dst[a0] = (float)x0;
+        dst[a0] = x0;
       }
       continue;
     }
@@ -260,10 +284,11 @@ __global__ void __launch_bounds__(256) append_any_kernel(const __grid_constant__
     if (is_v) h -= c.kv_heads;
     const float* src = (is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride) + (int64_t)h * D;
     T* dst = static_cast<T*>(is_v ? c.value : c.key) + off + (int64_t)h * D;
-    const double x0 = src[a0], x1 = src[a1];
+    constexpr bool odd = sizeof(T) == 2;
+    const float x0 = src[a0], x1 = src[a1];
     if (pair && !is_v) {
-      dst[a0] = to_cache<T>(x0 * cs[i] - x1 * sn[i]);
-      dst[a1] = to_cache<T>(x1 * cs[i] + x0 * sn[i]);
+      dst[a0] = to_cache<T>(rope_sum<false, odd>(x0, cs[i], x1, sn[i]));
+      dst[a1] = to_cache<T>(rope_sum<true, odd>(x1, cs[i], x0, sn[i]));
     } else {
       dst[a0] = to_cache<T>(x0);
       if (pair) dst[a1] = to_cache<T>(x1);
@@ -274,10 +299,10 @@ __global__ void __launch_bounds__(256) append_any_kernel(const __grid_constant__
 // 16-byte loads: a thread takes pieces of 8 features (4 pairs, or 8 features that are
 // not rotated) of a token's heads, IT of them, and has its loads in flight while one
 // warp finds the token's place (three dependent loads).  Bound by memory: 8676 tokens
-// of 48 heads of 128 (393 MB) run at MEASURED_RATE.  RoPE in double, as the dense
-// attention's, rounded once.
+// of 48 heads of 128 (393 MB) run at MEASURED_RATE.  RoPE as in
+// double, like the dense attention's, rounded once.
 template <typename T, int IT>
-__global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(128, 8) append_kernel(const __grid_constant__ AppendArgs a) {
   griddep_launch_dependents();
   griddep_wait();
   const PagedView& c = a.c;
@@ -322,29 +347,33 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ App
     const int h = head[i];
     const bool is_q = h < a.heads, is_v = h >= a.heads + c.kv_heads;
     if (!is_q && off < 0) continue;
-    double y[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) y[e] = x[i][e];
+    float(&y)[8] = x[i];
     const int pair0 = a.interleaved ? first[i] >> 1 : first[i];
     if (!is_v && pair0 < half && first[i] < 2 * half) {
       const float4 cv = __ldg(reinterpret_cast<const float4*>(a.cos + cs0 + pair0));
       const float4 sv = __ldg(reinterpret_cast<const float4*>(a.sin + cs0 + pair0));
-      const double cd[4] = {cv.x, cv.y, cv.z, cv.w}, sd[4] = {sv.x, sv.y, sv.z, sv.w};
+      const float cd[4] = {cv.x, cv.y, cv.z, cv.w}, sd[4] = {sv.x, sv.y, sv.z, sv.w};
+      auto turn = [&](auto odd) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        double& u = a.interleaved ? y[2 * e] : y[e];
-        double& v = a.interleaved ? y[2 * e + 1] : y[e + 4];
-        const double u0 = u, v0 = v;
-        u = u0 * cd[e] - v0 * sd[e];
-        v = v0 * cd[e] + u0 * sd[e];
-      }
+        for (int e = 0; e < 4; e++) {
+          const float u = a.interleaved ? y[2 * e] : y[e], v = a.interleaved ? y[2 * e + 1] : y[e + 4];
+          const float nu = rope_sum<false, odd>(u, cd[e], v, sd[e]);
+          const float nv = rope_sum<true, odd>(v, cd[e], u, sd[e]);
+          if (a.interleaved)
+            y[2 * e] = nu, y[2 * e + 1] = nv;
+          else
+            y[e] = nu, y[e + 4] = nv;
+        }
+      };
+      if (is_q || sizeof(T) == 4)
+        turn(std::false_type());
+      else
+        turn(std::true_type());
     }
     if (is_q) {
       float* dst = a.q_out + ((int64_t)t * a.heads + h) * D;
-      *reinterpret_cast<float4*>(dst + first[i]) =
-          make_float4((float)y[0], (float)y[1], (float)y[2], (float)y[3]);
-      *reinterpret_cast<float4*>(dst + second[i]) =
-          make_float4((float)y[4], (float)y[5], (float)y[6], (float)y[7]);
+      *reinterpret_cast<float4*>(dst + first[i]) = make_float4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<float4*>(dst + second[i]) = make_float4(y[4], y[5], y[6], y[7]);
       continue;
     }
     T* dst = static_cast<T*>(is_v ? c.value : c.key) + off +
