@@ -74,26 +74,6 @@ struct FastDiv {
   }
 };
 
-// Launches with programmatic stream serialisation: the kernel may start while the
-// one before it ends (every kernel here waits, griddep_wait, before it touches
-// memory), which takes the launch's latency off a step's chain of small kernels.
-template <typename... P, typename... A>
-int launch_overlapped(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem,
-                      cudaStream_t st, const A&... args) {
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  ORTC_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
-  return ORT_CUDA_OK;
-}
-
 struct PagedAttnArgs {
   PagedView c;
   const float* q = nullptr;

@@ -41,7 +41,9 @@ int launch_stream_one(const StreamArgs& p, int grid, cudaStream_t st) {
   static std::atomic<unsigned long long> attr_set{0};  // per device
   const int rc = set_smem(paged_stream_kernel<T, DP, R>, C::SMEM, attr_set);
   if (rc) return rc;
-  return launch_overlapped(paged_stream_kernel<T, DP, R>, grid, 256, C::SMEM, st, p);
+  paged_stream_kernel<T, DP, R><<<grid, 256, C::SMEM, st>>>(p);
+  ORTC_CUDA(cudaGetLastError());
+  return ORT_CUDA_OK;
 }
 
 template <typename T>
@@ -80,7 +82,9 @@ int launch_tile_cap(const TileArgs& p, int grid, cudaStream_t st) {
   }
   const int rc = set_smem(paged_tile_kernel<T, DP, CAP>, C::SMEM, attr_set);
   if (rc) return rc;
-  return launch_overlapped(paged_tile_kernel<T, DP, CAP>, grid, kTileThreads, C::SMEM, st, p);
+  paged_tile_kernel<T, DP, CAP><<<grid, kTileThreads, C::SMEM, st>>>(p);
+  ORTC_CUDA(cudaGetLastError());
+  return ORT_CUDA_OK;
 }
 
 template <typename T, int DP>
@@ -94,7 +98,9 @@ int launch_rows(const StreamArgs& p, int grid, cudaStream_t st) {
   static std::atomic<unsigned long long> attr_set{0};
   const int rc = set_smem(paged_rows_kernel<DP>, RowsCfg<DP>::SMEM, attr_set);
   if (rc) return rc;
-  return launch_overlapped(paged_rows_kernel<DP>, grid, 256, RowsCfg<DP>::SMEM, st, p);
+  paged_rows_kernel<DP><<<grid, 256, RowsCfg<DP>::SMEM, st>>>(p);
+  ORTC_CUDA(cudaGetLastError());
+  return ORT_CUDA_OK;
 }
 
 int launch_tile(const StreamArgs& s, int grid, cudaStream_t st, int64_t* launches) {

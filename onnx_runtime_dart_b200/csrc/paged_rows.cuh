@@ -40,8 +40,6 @@ __global__ void __launch_bounds__(256, 1) paged_rows_kernel(const __grid_constan
   unsigned char* ring = smem;
   uint4* qs = reinterpret_cast<uint4*>(smem + NS * C::STAGE + w * C::QW);  // this warp's
 
-  griddep_launch_dependents();
-  griddep_wait();
   TileRun<KB, C::EXTRA> run;
   if (!run.plan(p, TT, 1, s_plan)) return;
   TilePos cur = run.cur;

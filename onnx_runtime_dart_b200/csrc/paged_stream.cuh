@@ -539,9 +539,6 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int D = c.D, G = c.kv_heads, nb = p.prefix ? 1 : c.batch;
 
-  griddep_launch_dependents();
-  griddep_wait();
-
   // ---- this CTA's run of tiles
   int min_past = 0;
   if (p.prefix && a.window) {

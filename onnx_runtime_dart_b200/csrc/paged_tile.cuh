@@ -47,10 +47,10 @@ struct TileCfg {
   static constexpr int NK = PARTS == 2 && DP == 128 ? 3 : 4;  // ring stages of keys
   static constexpr int NV = PARTS == 2 && DP == 128 ? 2 : 4;  // and of values
   static constexpr int DATA = QB + (NK + NV) * STAGE;
-  // What a segment's start and end cost, in keys: a 4096-token fp16 prompt took 690,
-  // 445, 391, 368, 377 us at 3, 6, 8, 10, 12 blocks, a mixed bf16 step 240, 244, 263
-  // us at 6, 8, 12 (12, 16, 24 half blocks), a shared prefix 159, 151, 151 us at 3, 6, 10.
-  static constexpr int EXTRA = 8 * KB;
+  // What a segment's start and end cost, in keys (its q operands, the first block's
+  // latency, the output): a 4096-token fp16 prompt took 462, 389, 352, 355 us at 6,
+  // 8, 10, 12 blocks, a mixed bf16 step 210 to 220 us at 6 to 12, a shared prefix 111.
+  static constexpr int EXTRA = (PARTS == 2 ? 10 : 8) * KB;
   // data, (max, sum) of 128 rows by both warpgroups, block validity, barriers
   static constexpr int SMEM = DATA + 2 * 128 * 8 + 8 * 16 + 256;
   static_assert(2 * SREG + 2 * DP <= 512, "TMEM");
@@ -160,8 +160,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int D = c.D, TT = 128 / a.group;
   const int rows_tma = args.tma_rows, align = max(1, rows_tma);
 
-  griddep_launch_dependents();
-  griddep_wait();
   // ---- this CTA's run
   TileRun<KB, EX> run;
   if (!run.plan(p, TT, align, stats)) return;
@@ -425,32 +423,27 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       __syncwarp();
       tc_fence_after();
     };
-    // q rows: warp w loads rows 16 w .. 16 w + 15 of a segment's tile, a 16-byte
-    // piece a lane
-    constexpr int LPR = DP / 4, RPI = 32 / LPR, NQ = 16 / RPI;  // lanes a row, rows a step, steps
-    auto load_q = [&](const TilePos& s, float4 (&q4)[NQ]) {
+    // q rows: warp w brings rows 16 w .. 16 w + 15 of a segment's tile, a 16-byte piece
+    // a lane, four steps at a time with the next four on their way (the loop is rolled:
+    // straight-line code for all rows, run once a segment, waits for its instructions)
+    constexpr int LPR = DP / 4, RPI = 32 / LPR, NQ = 16 / RPI, QS = 4;  // lanes a row, rows a step, steps
+    auto load_q = [&](const TilePos& s, int i0, float4 (&q4)[QS]) {
       const int t0 = s.rt * TT, rows = min(TT, s.count - t0) * a.group;
       const int f = (lane & (LPR - 1)) * 4;
       const float* base = a.q + (int64_t)(s.row0 + t0) * a.q_stride + (int64_t)(s.g * a.group) * D;
-      const float* src[NQ];
 #pragma unroll
-      for (int i = 0; i < NQ; i++) {  // rows and features that are not there: the first
-        const int r0 = warp * 16 + i * RPI + lane / LPR, r = r0 < rows ? r0 : 0;
-        const int t = p.group_div.div(r);
-        src[i] = base + (int64_t)t * a.q_stride + (int64_t)(r - t * a.group) * D + (f < D ? f : 0);
+      for (int i = 0; i < QS; i++) {
+        const int r = warp * 16 + (i0 + i) * RPI + lane / LPR;
+        q4[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < rows && f < D) {
+          const int t = p.group_div.div(r);
+          const float* src = base + (int64_t)t * a.q_stride + (int64_t)(r - t * a.group) * D + f;
+          if (p.q_vec)
+            q4[i] = __ldg(reinterpret_cast<const float4*>(src));
+          else
+            q4[i] = make_float4(__ldg(src), __ldg(src + 1), __ldg(src + 2), __ldg(src + 3));
+        }
       }
-      if (p.q_vec) {
-#pragma unroll
-        for (int i = 0; i < NQ; i++) q4[i] = __ldg(reinterpret_cast<const float4*>(src[i]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < NQ; i++)
-          q4[i] =
-              make_float4(__ldg(src[i]), __ldg(src[i] + 1), __ldg(src[i] + 2), __ldg(src[i] + 3));
-      }
-#pragma unroll
-      for (int i = 0; i < NQ; i++)
-        if (warp * 16 + i * RPI + lane / LPR >= rows || f >= D) q4[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     };
     for (;;) {
       const int n = blocks(cur, seg, k0);
@@ -458,35 +451,41 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const bool has = row < rows_here;
       const int tok = tok0 + (has ? p.group_div.div(row) : 0);
       // the parts of the q tile
-      float4 q4[NQ];
-      load_q(cur, q4);
+      float4 q4[QS];
+      load_q(cur, 0, q4);
+#pragma unroll 1
+      for (int i0 = 0; i0 < NQ; i0 += QS) {
+        float4 nq[QS];
+        load_q(cur, min(i0 + QS, NQ - QS), nq);
 #pragma unroll
-      for (int i = 0; i < NQ; i++) {
-        const int r = warp * 16 + i * RPI + lane / LPR, ch = (lane & (LPR - 1)) >> 1;
-        float fr = p.t_scale, up = 1.f;
-        if constexpr (PARTS == 2) {  // the row's largest value into [2^13, 2^14)
-          float mx = fmaxf(fmaxf(fabsf(q4[i].x), fabsf(q4[i].y)),
-                           fmaxf(fabsf(q4[i].z), fabsf(q4[i].w)));
-          if (LPR == 32) {
-            mx = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(mx)));
-          } else {
+        for (int i = 0; i < QS; i++) {
+          const int r = warp * 16 + (i0 + i) * RPI + lane / LPR, ch = (lane & (LPR - 1)) >> 1;
+          float fr = p.t_scale, up = 1.f;
+          if constexpr (PARTS == 2) {  // the row's largest value into [2^13, 2^14)
+            float mx = fmaxf(fmaxf(fabsf(q4[i].x), fabsf(q4[i].y)),
+                             fmaxf(fabsf(q4[i].z), fabsf(q4[i].w)));
+            if (LPR == 32) {
+              mx = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(mx)));
+            } else {
 #pragma unroll
-            for (int x = LPR / 2; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, x));
+              for (int x = LPR / 2; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, x));
+            }
+            int ex = (int)(__float_as_uint(mx) >> 23) - 127;
+            ex = max(-100, min(ex, 126));
+            up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
+            fr *= __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
           }
-          int ex = (int)(__float_as_uint(mx) >> 23) - 127;
-          ex = max(-100, min(ex, 126));
-          up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
-          fr *= __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
-        }
-        uint32_t w0[PARTS], w1[PARTS];
-        Split<T>::pair(q4[i].x * up, q4[i].y * up, w0);
-        Split<T>::pair(q4[i].z * up, q4[i].w * up, w1);
+          uint32_t w0[PARTS], w1[PARTS];
+          Split<T>::pair(q4[i].x * up, q4[i].y * up, w0);
+          Split<T>::pair(q4[i].z * up, q4[i].w * up, w1);
 #pragma unroll
-        for (int pt = 0; pt < PARTS; pt++)
-          *reinterpret_cast<uint2*>(qs + pt * C::QPART + (ch >> 3) * 16384 + r * 128 +
-                                    (((ch & 7) ^ (r & 7)) << 4) + (lane & 1) * 8) =
-              make_uint2(w0[pt], w1[pt]);
-        if ((lane & (LPR - 1)) == 0) stats[r].x = fr;
+          for (int pt = 0; pt < PARTS; pt++)
+            *reinterpret_cast<uint2*>(qs + pt * C::QPART + (ch >> 3) * 16384 + r * 128 +
+                                      (((ch & 7) ^ (r & 7)) << 4) + (lane & 1) * 8) =
+                make_uint2(w0[pt], w1[pt]);
+          if ((lane & (LPR - 1)) == 0) stats[r].x = fr;
+          q4[i] = nq[i];
+        }
       }
       fence_proxy_async_smem();
       mbar_arrive(qfull);
@@ -758,7 +757,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (p.prefix && lane == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * to) = make_float2(M, L);
       };
       constexpr int NX = DP / 32;
-#pragma unroll 4
+#pragma unroll 2
       for (int r = warp; r < rows_here; r += 8) {
         const float2 ml = stats[r];
         float v[NX];
