@@ -48,8 +48,8 @@ struct TileCfg {
   static constexpr int NV = PARTS == 2 && DP == 128 ? 2 : 4;  // and of values
   static constexpr int DATA = QB + (NK + NV) * STAGE;
   // What a segment's start and end cost, in keys (its q operands, the first block's
-  // latency, the output): a 4096-token fp16 prompt took 462, 389, 352, 355 us at 6,
-  // 8, 10, 12 blocks, a mixed bf16 step 210 to 220 us at 6 to 12, a shared prefix 111.
+  // latency, the output): a 4096-token fp16 prompt took 383, 345, 340 us at 6, 8, 10
+  // blocks, a mixed bf16 step 219, 210, 210, a shared prefix 115, 112, 112.
   static constexpr int EXTRA = (PARTS == 2 ? 10 : 8) * KB;
   // data, (max, sum) of 128 rows by both warpgroups, block validity, barriers
   static constexpr int SMEM = DATA + 2 * 128 * 8 + 8 * 16 + 256;
@@ -128,9 +128,10 @@ __device__ __forceinline__ void split2(uint64_t x, uint32_t (&w)[Split<T>::PARTS
   }
 }
 
-// tile_warp_regs: registers per thread after the split; they draw on what the
-// block was launched with (kTileRegs a thread), which launch_tile checks.
-constexpr int kTileThreads = 384, kTileSoftRegs = 216, kTileLoadRegs = 72, kTileRegs = 168;
+// Registers a thread after the split; they draw on what the block was launched with
+// (kTileRegs a thread), which launch_tile_cap checks.  A softmax thread holds its row's
+// output (128); 208, 216, 224, 232 for it: a mixed bf16 step 224, 210, 205, 205 us.
+constexpr int kTileThreads = 384, kTileSoftRegs = 232, kTileLoadRegs = 40, kTileRegs = 168;
 static_assert(256 * kTileSoftRegs + 128 * kTileLoadRegs <= kTileThreads * kTileRegs, "registers");
 
 template <typename T, int DP, bool CAP>
@@ -445,18 +446,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
       }
     };
+    float4 q4[QS];
+    load_q(cur, 0, q4);
     for (;;) {
       const int n = blocks(cur, seg, k0);
       const int tok0 = cur.rt * TT, rows_here = min(TT, cur.count - tok0) * a.group;
       const bool has = row < rows_here;
       const int tok = tok0 + (has ? p.group_div.div(row) : 0);
       // the parts of the q tile
-      float4 q4[QS];
-      load_q(cur, 0, q4);
 #pragma unroll 1
       for (int i0 = 0; i0 < NQ; i0 += QS) {
         float4 nq[QS];
-        load_q(cur, min(i0 + QS, NQ - QS), nq);
+        if (i0 + QS < NQ) load_q(cur, i0 + QS, nq);
 #pragma unroll
         for (int i = 0; i < QS; i++) {
           const int r = warp * 16 + (i0 + i) * RPI + lane / LPR, ch = (lane & (LPR - 1)) >> 1;
@@ -484,7 +485,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                       (((ch & 7) ^ (r & 7)) << 4) + (lane & 1) * 8) =
                 make_uint2(w0[pt], w1[pt]);
           if ((lane & (LPR - 1)) == 0) stats[r].x = fr;
-          q4[i] = nq[i];
+          if (NQ > QS) q4[i] = nq[i];
         }
       }
       fence_proxy_async_smem();
@@ -628,16 +629,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             tmem_st8(ts + KB + 8 * st, make_uint4(w2[0], w2[1], w2[2], w2[3]),
                      make_uint4(w2[4], w2[5], w2[6], w2[7]));
         };
-        if (full) {  // the next scores on their way from TMEM meanwhile
-          uint32_t ra[16], rb[16];
-          tmem_ld16(ts, ra);
+        if (full) {
 #pragma unroll 1
           for (int i = 0; i < KB / 32; i++) {
-            tmem_ld_wait();
+            uint32_t ra[16], rb[16];
+            tmem_ld16(ts + 32 * i, ra);
             tmem_ld16(ts + 32 * i + 16, rb);
-            weigh(std::false_type(), 2 * i, ra, 0u);
             tmem_ld_wait();
-            if (i + 1 < KB / 32) tmem_ld16(ts + 32 * i + 32, ra);
+            weigh(std::false_type(), 2 * i, ra, 0u);
             weigh(std::false_type(), 2 * i + 1, rb, 0u);
           }
         } else {
@@ -739,39 +738,48 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       else
         join(H1(), mine, theirs);
       bar_sync(1, 256);
-      // (stats[0..127] becomes the joined pair; a thread reads only its own row's
-      // other half above, so the second half of the array is no longer needed)
-      if (wg == 0) stats[row] = make_float2(M, l * mine + s2.y * theirs);
-      bar_sync(1, 256);
       const bool whole = n == cur.nt;
       const int slot = 2 * blockIdx.x + (k0 ? 0 : 1);
-      auto write_row = [&](int64_t to, float M, float L, const float (&v)[DP / 32]) {
-        const float2 f = paged_row_scale(p, to, M, L);
-        float* dst = (p.prefix ? p.pre_o : a.out) + to * D;
-        const float* pre = p.pre_o + to * D;
-#pragma unroll
-        for (int x = 0; x < DP / 32; x++) {
-          const int d = lane + 32 * x;
-          if (d < D) dst[d] = p.prefix || !a.shared ? v[x] * f.x : fmaf(v[x], f.x, pre[d] * f.y);
-        }
-        if (p.prefix && lane == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * to) = make_float2(M, L);
-      };
-      constexpr int NX = DP / 32;
-#pragma unroll 2
-      for (int r = warp; r < rows_here; r += 8) {
-        const float2 ml = stats[r];
-        float v[NX];
-#pragma unroll
-        for (int x = 0; x < NX; x++) v[x] = at(lane + 32 * x, r);
-        if (!whole) {
-          const int64_t to = (int64_t)slot * 128 + r;
-#pragma unroll
-          for (int x = 0; x < NX; x++) p.part_o[to * DP + lane + 32 * x] = v[x];
-          if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + to * 2) = ml;
-        } else {
-          write_row(tile_place(p, cur, TT, r), ml.x, ml.y, v);
-        }
+      if (wg == 0) {  // the row's place and factors, over the states (read above)
+        const float L = l * mine + s2.y * theirs;
+        const int64_t to = whole ? tile_place(p, cur, TT, has ? row : 0) : (int64_t)slot * 128 + row;
+        float2 f = make_float2(1.f, 0.f);
+        if (has && (!whole || p.prefix))
+          *reinterpret_cast<float2*>((whole ? p.pre_ml : p.part_ml) + 2 * to) = make_float2(M, L);
+        else if (has)
+          f = paged_row_scale(p, to, M, L);
+        stats[row] = f;
+        reinterpret_cast<int64_t*>(stats + 128)[row] = to * (whole ? D : DP);
       }
+      // the next segment's first q rows come while this one's are written
+      TilePos nx = cur;
+      long long nseg = seg;
+      int nk0 = k0;
+      const bool more = next(nx, nseg, nk0);
+      if (more) load_q(nx, 0, q4);
+      bar_sync(1, 256);
+      auto write = [&](auto add) {
+        float* dst = whole ? (p.prefix ? p.pre_o : a.out) : p.part_o;
+#pragma unroll 4
+        for (int r = warp; r < rows_here; r += 8) {
+          const float2 f = stats[r];
+          const int64_t to = reinterpret_cast<const int64_t*>(stats + 128)[r];
+          float v[DP / 32];
+#pragma unroll
+          for (int x = 0; x < DP / 32; x++) v[x] = at(lane + 32 * x, r) * f.x;
+#pragma unroll
+          for (int x = 0; x < DP / 32; x++) {
+            const int d = lane + 32 * x;
+            if (d >= D) continue;
+            if (add) v[x] = fmaf(p.pre_o[to + d], f.y, v[x]);
+            dst[to + d] = v[x];
+          }
+        }
+      };
+      if (whole && !p.prefix && a.shared)
+        write(std::true_type());
+      else
+        write(std::false_type());
       if (!whole) {
         const int c0 = (int)(((seg + 1) * runs - 1) / total);
         const int c1 = (int)(((seg + (long long)(cur.nt - 1) * KB + 1) * runs - 1) / total);
@@ -785,7 +793,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
       }
       bar_sync(1, 256);  // the staged output has been read
-      if (!next(cur, seg, k0)) break;
+      if (!more) break;
+      cur = nx, seg = nseg, k0 = nk0;
     }
   }
   tc_fence_before();
