@@ -458,7 +458,7 @@ typedef struct ort_cuda_paged_cache {
  * rows k_stride and v_stride floats apart (slices of a fused projection's
  * output need no copy), Q [num_tokens, num_heads * head_size] with row stride
  * q_stride, or NULL with Q_out NULL; Q_out is contiguous and may be Q itself
- * when q_stride is its row length.  cos/sin caches [max_pos, rotary_half] as
+ * when q_stride is its row length (else it may not overlap Q, K or V).  cos/sin caches [max_pos, rotary_half] as
  * for ort_cuda_group_query_attention (ORT_CUDA_ROTARY_INTERLEAVED for (2i, 2i + 1)
  * pairs; a position >= max_pos is not rotated but left out, and reported as
  * above), or both NULL: no rotation.  The rows of one call must be distinct
@@ -479,17 +479,19 @@ ORT_CUDA_API int ort_cuda_paged_kv_append(ort_cuda_session* s, const ort_cuda_pa
  * are scale * q.k (scale <= 0: 1/sqrt(head_size)) and, with softcap > 0,
  * softcap * tanh(score / softcap).  Q [num_tokens, num_heads * head_size] fp32
  * with row stride q_stride; out [num_tokens, num_heads * head_size] fp32,
- * contiguous.  Query head h reads KV head h / (num_heads / kv_num_heads).
+ * contiguous, apart from Q.  Query head h reads KV head h / (num_heads / kv_num_heads).
  *   max_seq     bound of the tokens of any one sequence of the call (a
  *               sequence with more is left out and reported)
  *   shared_len  > 0: the first shared_len positions of every sequence hold
  *               the same tokens, and are read through the first row of the
- *               block table, once for the whole batch; every past_lens[b]
- *               of a sequence with tokens must be at least shared_len
+ *               block table (whether or not its sequence has tokens in this
+ *               call), once for the whole batch; every past_lens[b] of a
+ *               sequence with tokens must be at least shared_len
  * fp32 results whatever the cache's type: products, softmax statistics and
  * sums keep 22 bits or more.  Device pointers only; stream-ordered.  A call
  * uses a workspace of its stream (or of the graph being captured), so calls
- * on different streams may run at the same time. */
+ * on different streams may run at the same time; the session must outlive the
+ * graphs that were captured with its calls. */
 ORT_CUDA_API int ort_cuda_paged_attention(ort_cuda_session* s, const ort_cuda_paged_cache* cache,
                                           const float* Q, int64_t q_stride, int64_t num_tokens,
                                           int64_t max_seq, int num_heads, double scale,

@@ -422,6 +422,11 @@ int launch_append(AppendArgs& a, cudaStream_t st, int64_t* launches) {
   return rc;
 }
 
+// Whether two ranges of floats share one.
+bool overlap(const float* a, int64_t an, const float* b, int64_t bn) {
+  return a && b && a < b + bn && b < a + an;
+}
+
 // Checks what the host can see of a cache and fills the kernels' view.
 int paged_view(ort_cuda_session* s, const ort_cuda_paged_cache* c, int64_t num_tokens, int flags,
                PagedView* v) {
@@ -483,8 +488,15 @@ ORT_CUDA_API int ort_cuda_paged_kv_append(ort_cuda_session* s, const ort_cuda_pa
                     num_heads <= INT_MAX / D && q_stride >= num_heads * D),
              ORT_CUDA_ERR_INVALID_ARG,
              "paged append: need num_heads a multiple of kv_num_heads and q_stride >= its row");
-  ORTC_CHECK(Q != Q_out || !Q || q_stride == num_heads * D, ORT_CUDA_ERR_INVALID_ARG,
-             "paged append: Q_out may be Q only when Q is contiguous");
+  const int64_t rows = std::max<int64_t>(num_tokens - 1, 0), qn = num_heads * D;
+  ORTC_CHECK(!Q || num_tokens == 0 ||
+                 (Q == Q_out ? q_stride == qn : !overlap(Q_out, (rows + 1) * qn, Q, rows * q_stride + qn)),
+             ORT_CUDA_ERR_INVALID_ARG,
+             "paged append: Q_out may be Q only when Q is contiguous, and not overlap it else");
+  ORTC_CHECK(!Q || num_tokens == 0 ||
+                 (!overlap(Q_out, (rows + 1) * qn, K, rows * k_stride + row) &&
+                  !overlap(Q_out, (rows + 1) * qn, V, rows * v_stride + row)),
+             ORT_CUDA_ERR_INVALID_ARG, "paged append: Q_out overlaps K or V");
   ORTC_CHECK(k_stride >= row && v_stride >= row, ORT_CUDA_ERR_INVALID_ARG,
              "paged append: k_stride and v_stride must be at least a row");
   ORTC_CHECK((cos_cache == nullptr) == (sin_cache == nullptr), ORT_CUDA_ERR_INVALID_ARG,
@@ -530,6 +542,8 @@ ORT_CUDA_API int ort_cuda_paged_attention(ort_cuda_session* s, const ort_cuda_pa
   ORTC_CHECK(Q && out, ORT_CUDA_ERR_INVALID_ARG, "NULL argument");
   ORTC_CHECK(num_tokens * num_heads <= INT_MAX, ORT_CUDA_ERR_INVALID_ARG,
              "paged attention: sizes too large");
+  ORTC_CHECK(!overlap(out, num_tokens * num_heads * D, Q, (num_tokens - 1) * q_stride + num_heads * D),
+             ORT_CUDA_ERR_INVALID_ARG, "paged attention: out overlaps Q");
   a.q = Q, a.q_stride = q_stride, a.out = out;
   a.heads = num_heads, a.group = num_heads / cache->kv_num_heads;
   a.max_seq = (int)std::min<int64_t>(max_seq, num_tokens);

@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const uint32_t ring = smem_u32(is_k ? ks : vs);
         const CUtensorMap* map = is_k ? &args.key : &args.value;
         if (lane == 0) prefetch_tensormap(map);
-        int cnt = 0;
+        int cnt = 0, issued = 0;
         for (;;) {
           const int n = blocks(cur, seg, k0);
 #pragma unroll 1
@@ -299,6 +299,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               __syncwarp();
             }
             if (!dead) {
+              issued = cnt + 1;
               if (lane == 0)
                 mbar_arrive_expect_tx(full + st,
                                       (uint32_t)(__popc(there) * rows_tma * 128 * (DP / 64)));
@@ -313,11 +314,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
           if (!next(cur, seg, k0)) break;
         }
-        // the last stages have landed before the block's memory is given up: every
-        // one is waited for by the MMA warp (unless a wait ran out)
-        if (dead)
-          for (int i = max(0, cnt - NS); i < cnt; i++)
-            if (!mbar_wait(full + i % NS, (i / NS) & 1)) record_error(c.err, KERR_WAIT_DRAIN);
+        // the last copies have landed before the block's memory is given up
+        for (int i = max(0, issued - NS); i < issued; i++)
+          if (!mbar_wait(full + i % NS, (i / NS) & 1)) record_error(c.err, KERR_WAIT_DRAIN);
       }
     } else {
       // ---- loaders: the stages in the order the MMA warp takes them (K0, K1, V0,

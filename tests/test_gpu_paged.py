@@ -114,6 +114,50 @@ def test_attention_shared_prefix(sess, shared, shape, window, softcap, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("new,past", [([1], 900), ([1, 0, 2], 70), ([40], 30), ([1, 33, 1], 200)])
+def test_attention_many_sequences(sess, new, past, dtype):
+    """More sequences than a block has threads: the list is found in two passes."""
+    batch = 700
+    new = [new[b % len(new)] for b in range(batch)]
+    past = [(b * 37) % past for b in range(batch)]
+    s = ref.make(16, dtype, new, past, 8, 2, 64, 16)
+    want = ref.attention(s, new, past, 8)
+    near(want, run(sess, s, 8, new))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("window", [0, 700])
+def test_attention_long_prompt(sess, window, dtype):
+    """Many tiles of rows per run, long and short ones, on every kind of page."""
+    for page in (16, 12):
+        new, past = [2600, 500], [0, 1300]
+        s = ref.make(17, dtype, new, past, 8, 2, 128, page)
+        want = ref.attention(s, new, past, 8, window=window)
+        near(want, run(sess, s, 8, new, local_window_size=window))
+
+
+def test_attention_of_drawn_batches(sess):
+    """Ragged batches of all kinds, drawn from a seed."""
+    import random
+    for seed in range(40):
+        r = random.Random(seed)
+        heads, G = r.choice([(8, 8), (8, 2), (16, 1), (12, 4), (7, 1), (32, 8)])
+        head, page = r.choice([64, 128, 96, 72]), r.choice([16, 8, 64, 24, 11, 1, 48])
+        batch = r.choice([1, 2, 5, 17, 60])
+        most = r.choice([1, 1, 4, 30, 200])
+        new = [r.randint(0, most) for _ in range(batch)]
+        new[r.randrange(batch)] = most
+        shared = r.choice([0, 0, r.randint(1, 500)])
+        past = [shared + int(10 ** r.uniform(0, 3.3)) for _ in range(batch)]
+        window = r.choice([0, 0, r.randint(1, 600)])
+        softcap = r.choice([0.0, 0.0, 10.0])
+        s = ref.make(seed, r.choice([F32, F16, BF16]), new, past, heads, G, head, page, shared)
+        want = ref.attention(s, new, past, heads, None, softcap, window)
+        near(want, run(sess, s, heads, new, softcap=softcap, local_window_size=window,
+                       shared_len=shared))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_attention_large_and_small_values(sess, dtype):
     """Queries over ten orders of magnitude, sharp and flat rows."""
     new, past, heads = [6, 140], [90, 0], 8
@@ -372,6 +416,9 @@ def test_refusals(sess):
                  lambda: sess.paged_attention(h, q, 8, shared_len=10 ** 6),
                  lambda: sess.paged_attention(h, q, 8, scale=math.inf),
                  lambda: sess.paged_attention(h, q, 8, softcap=math.nan),
+                 lambda: sess.paged_attention(h, q, 8, out=q),
+                 lambda: sess.paged_kv_append(h, q[:, :128].contiguous(), kv, q=q, num_heads=8,
+                                              q_out=torch.empty(2, 513, device="cuda")[:, 1:]),
                  lambda: sess.paged_attention(h, q, 8, out=q.half()),
                  lambda: sess.paged_attention(h, q, 8, out=q[:1]),
                  lambda: sess.paged_kv_append(h, kv, kv[:1]),
@@ -388,6 +435,11 @@ def test_refusals(sess):
                  lambda: PagedKVCache(s["key"].cpu(), s["value"], s["table"], s["cu"], s["past"])):
         with pytest.raises(ValueError):
             call()
+    both = torch.zeros((3, 512), device="cuda")
+    with pytest.raises(ValueError, match="overlap"):  # shifted by a row
+        sess.paged_kv_append(h, kv, kv, q=both[:2], num_heads=8, q_out=both[1:])
+    with pytest.raises(ValueError, match="overlaps K"):
+        sess.paged_kv_append(h, both[0, :256].view(2, 128), kv, q=q, num_heads=8, q_out=both[:2])
     for head in (136, 12):
         odd = ref.make(15, F16, [2], [5], 2, 1, head, 16)
         with pytest.raises(UnsupportedError):
