@@ -22,8 +22,6 @@ namespace ortc {
 // replayed at once, never share one.  A graph's workspace is handed back when
 // the graph and everything instantiated from it are gone (a CUDA user object),
 // and is reused by later captures.  The first kTicketBytes are zero between calls.
-constexpr size_t kTicketBytes = 4096;
-
 struct PagedScratch {
   struct Buf {
     void* p = nullptr;
@@ -297,9 +295,9 @@ __global__ void __launch_bounds__(256) append_any_kernel(const __grid_constant__
 // 16-byte loads: a thread takes pieces of 8 features (4 pairs, or 8 features that are
 // not rotated) of a token's heads, IT of them, and has its loads in flight while one
 // warp finds the token's place (three dependent loads).  Bound by memory: 8676 tokens
-// of 48 heads of 128 (393 MB) take
-// 83 us, 4.75 TB/s, 0.73 of the copy.  RoPE as in
-// double, like the dense attention's, rounded once.
+// of 48 heads of
+// 128 (393 MB) take 83 us, 4.75 TB/s, 0.73 of the copy (90, 107 us with two pieces, one).
+// RoPE as in double, like the dense attention's, rounded once.
 template <typename T, int IT>
 __global__ void __launch_bounds__(128, 8) append_kernel(const __grid_constant__ AppendArgs a) {
   const PagedView& c = a.c;

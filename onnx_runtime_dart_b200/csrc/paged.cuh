@@ -74,6 +74,9 @@ struct FastDiv {
   }
 };
 
+// The first bytes of a workspace, zero between calls.
+constexpr size_t kTicketBytes = 4096;
+
 struct PagedAttnArgs {
   PagedView c;
   const float* q = nullptr;

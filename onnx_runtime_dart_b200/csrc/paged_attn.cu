@@ -9,7 +9,6 @@
 namespace ortc {
 namespace {
 
-constexpr size_t kTicketBytes = 4096;  // kept zero between calls (csrc/paged.cu)
 size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // Query rows of a sequence and KV head up to which the stream kernel takes it.
