@@ -11,8 +11,17 @@ namespace {
 
 size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Query rows of a sequence and KV head up to which the stream kernel takes it.
-constexpr int kStreamRows = 64;
+// Query rows of a sequence and KV head up to which the stream kernel takes it.  The
+// tiles win from 33 to 64 rows where their segments fill the device (16-bit pages, 8
+// sequences of 8 KV heads over 2000 to 4000 keys, 64 rows: 58 us against 84, 32 rows: 53
+// against 49) and lose where few do (1 sequence, 64 rows: 36 against 22); over fp32
+// pages the stream wins to 64 rows either way (276 against 211, 68 against 38; 128 rows:
+// 324 against 408).
+// A shared prefix is one sequence.
+int stream_limit(const PagedAttnArgs& a, int sequences) {
+  const bool many = (int64_t)sequences * a.c.kv_heads > 16;
+  return a.c.type != ORT_CUDA_CACHE_F32 && many ? 32 : 64;
+}
 
 // Rows of one MMA tile of the stream kernel: 8 when no sequence can have more
 // (a row's parts then share an MMA), else 16.
@@ -138,10 +147,10 @@ int launch_tile(const StreamArgs& s, int grid, cudaStream_t st, int64_t* launche
 
 // Whether the sequences' own keys, and the shared prefix, may need tiles of 128 rows.
 bool tile_main(const PagedAttnArgs& a) {
-  return tile_ok(a) && (int64_t)a.max_seq * a.group > kStreamRows;
+  return tile_ok(a) && (int64_t)a.max_seq * a.group > stream_limit(a, a.c.batch);
 }
 bool tile_prefix(const PagedAttnArgs& a) {
-  return tile_ok(a) && a.shared && (int64_t)a.c.num_tokens * a.group > kStreamRows;
+  return tile_ok(a) && a.shared && (int64_t)a.c.num_tokens * a.group > stream_limit(a, 1);
 }
 size_t piece_rows(const PagedAttnArgs& a) { return tile_main(a) || tile_prefix(a) ? 128 : 16; }
 
@@ -191,7 +200,7 @@ int launch_paged_attention(const PagedAttnArgs& a, void* scratch, int sm_count, 
                              launches);
     if (rc) return rc;
   }
-  p.max_rows = tile_ok(a) ? kStreamRows : INT_MAX;
+  p.max_rows = tile_ok(a) ? stream_limit(a, a.c.batch) : INT_MAX;
   if (tile_main(a)) {
     rc = launch_tile(p, sm_count, st, launches);
     if (rc) return rc;
