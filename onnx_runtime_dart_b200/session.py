@@ -118,6 +118,7 @@ class PagedKVCache:
         self.key, self.value = key, value
         self.block_table, self.cu_seqlens, self.past_lens = block_table, cu_seqlens, past_lens
         self.batch, self.device, self.index = batch, key.device, key.get_device()
+        self._torch = torch
         self.kv_heads, self.head_size = int(key.shape[2]), int(key.shape[3])
         self.struct = _lib.PagedCacheStruct(
             key.data_ptr(), value.data_ptr(), block_table.data_ptr(), cu_seqlens.data_ptr(),
@@ -129,6 +130,9 @@ class PagedKVCache:
         """(tensor, row stride) of a float32 activation of `width` features a
         token: rows may lie apart (a slice of a fused projection's output),
         anything else is made contiguous."""
+        if x.dtype is self._torch.float32 and x.ndim == 2 and x.shape[1] == width and \
+                x.is_contiguous() and x.get_device() == self.index:
+            return x, width
         if x.get_device() != self.index or not x.is_floating_point():
             raise ValueError(f"{name} must be a float tensor on {self.device}")
         shape = x.shape
@@ -652,7 +656,7 @@ class CudaSession:
         """The stream of a paged call: None, torch's current stream; or, after
         set_stream(), a context with that stream current for torch too, so that
         what the call allocates and converts belongs to it."""
-        import torch
+        torch = cache._torch
         if cache.index != self.device:
             raise ValueError(f"PagedKVCache is on {cache.device}, the session on cuda:"
                              f"{self.device}")
@@ -666,10 +670,10 @@ class CudaSession:
         return torch.cuda.stream(torch.cuda.ExternalStream(self._stream_ptr, cache.device))
 
     @staticmethod
-    def _paged_out(name: str, out, like):
+    def _paged_out(cache, name: str, out, like):
         """The fp32 output of a paged call: `out` checked, or a new tensor."""
         if out is None:
-            import torch
+            torch = cache._torch
             return torch.empty_like(like, memory_format=torch.contiguous_format)
         if out.shape != like.shape or out.element_size() != 4 or not out.is_floating_point() or \
                 out.device != like.device or not out.is_contiguous():
@@ -696,8 +700,8 @@ class CudaSession:
         width = cache.kv_heads * cache.head_size
         k, ks = cache.rows("k", k, width)
         v, vs = cache.rows("v", v, width)
-        n = int(k.shape[0])
-        if int(v.shape[0]) != n or (q is not None and int(q.shape[0]) != n):
+        n = k.shape[0]
+        if v.shape[0] != n or (q is not None and q.shape[0] != n):
             raise ValueError("paged_kv_append: q, k and v need the same number of tokens")
         qp = qs = op = 0
         if q is not None:
@@ -705,7 +709,7 @@ class CudaSession:
             if q_out is q and rows is not q:
                 raise ValueError("paged_kv_append: only contiguous float32 queries are "
                                  "rotated in place")
-            q_out = self._paged_out("q_out", q_out, rows)
+            q_out = self._paged_out(cache, "q_out", q_out, rows)
             qp, op = rows.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("paged_kv_append: q_out without q")
@@ -713,14 +717,14 @@ class CudaSession:
         if (cos_cache is None) != (sin_cache is None):
             raise ValueError("paged_kv_append: give both cos and sin caches or neither")
         if cos_cache is not None:
+            f32, shape = cache._torch.float32, cos_cache.shape
             for t in (cos_cache, sin_cache):
-                if t.get_device() != cache.index or t.element_size() != 4 or \
-                        not t.is_floating_point() or not t.is_contiguous() or t.ndim != 2 or \
-                        t.shape != cos_cache.shape:
+                if t.dtype is not f32 or t.get_device() != cache.index or \
+                        not t.is_contiguous() or len(shape) != 2 or t.shape != shape:
                     raise ValueError("paged_kv_append: cos/sin caches must be contiguous "
                                      "float32 [max_pos, rotary_half] CUDA tensors")
             cp, sp = cos_cache.data_ptr(), sin_cache.data_ptr()
-            max_pos, half = cos_cache.shape
+            max_pos, half = shape
         rc = _lib.load().ort_cuda_paged_kv_append(
             self.handle, cache.ref, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, n, num_heads,
             cp, sp, half, max_pos, op, _lib.ROTARY_INTERLEAVED if rotary_interleaved else 0)
@@ -750,8 +754,8 @@ class CudaSession:
     def _paged_attention(self, cache, q, num_heads, max_seq, scale, softcap, local_window_size,
                          shared_len, out):
         q, qs = cache.rows("q", q, num_heads * cache.head_size)
-        out = self._paged_out("out", out, q)
-        n = int(q.shape[0])
+        out = self._paged_out(cache, "out", out, q)
+        n = q.shape[0]
         rc = _lib.load().ort_cuda_paged_attention(
             self.handle, cache.ref, q.data_ptr(), qs, n, n if max_seq is None else max_seq,
             num_heads, 0.0 if scale is None else scale, softcap, local_window_size,
