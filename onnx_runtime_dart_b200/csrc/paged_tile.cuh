@@ -10,10 +10,10 @@
 //
 // Roles: two softmax warpgroups, which take the blocks of a segment in turn
 // (one works on its block's weights while the tensor cores work for the
-// other), an MMA warp, and loaders: TMA boxes of as many tokens
-// as a power of two divides the page size, or, where that is below 8, cp.async in
-// pieces of 16 bytes by three warps (about 4000 cycles a stage of 32 KB).  A
-// warpgroup's thread owns one query row: it reads the row's scores from TMEM,
+// other), an MMA warp, and loaders: TMA boxes of as many tokens as a power of
+// two divides the page size, or, where that is below 8, cp.async in pieces of
+// 16 bytes by three warps (a 2048-token prompt on pages of 16, 24, 17 tokens:
+// 137, 152, 322 us).  A warpgroup's thread owns one query row: it reads the row's scores from TMEM,
 // writes the weights back over them as the A operand of p.v, and adds each
 // block's product, which comes in TMEM columns of its own, to its fp32 output in
 // registers (so sums over many blocks are rounded, where the tensor cores cut

@@ -130,6 +130,8 @@ class PagedKVCache:
         """(tensor, row stride) of a float32 activation of `width` features a
         token: rows may lie apart (a slice of a fused projection's output),
         anything else is made contiguous."""
+        if not isinstance(x, self._torch.Tensor):
+            raise ValueError(f"{name} must be a float tensor on {self.device}")
         if x.dtype is self._torch.float32 and x.ndim == 2 and x.shape[1] == width and \
                 x.is_contiguous() and x.get_device() == self.index:
             return x, width
@@ -1059,11 +1061,15 @@ class CudaSession:
             k, v, kc, vc, cu, past, table, cos, sin = (values[x] if x else None
                                                        for x in names[1:10])
             heads, kv = attrs["num_heads"], attrs["kv_num_heads"]
+            cache = PagedKVCache(kc, vc, table, cu, past)
             if k is None:  # q, k and v side by side
+                if not self._is_torch(a):
+                    raise ValueError("PagedAttention takes device tensors")
                 D = int(a.shape[-1]) // (heads + 2 * kv)
                 a, k, v = a.split([heads * D, kv * D, kv * D], dim=-1)
             rotary = bool(attrs.get("do_rotary", 0))
-            cache = PagedKVCache(kc, vc, table, cu, past)
+            if rotary and (cos is None or sin is None):
+                raise ValueError("PagedAttention: do_rotary needs cos and sin caches")
             q = self.paged_kv_append(cache, k, v, q=a if rotary else None, num_heads=heads,
                                      cos_cache=cos if rotary else None,
                                      sin_cache=sin if rotary else None,

@@ -417,6 +417,13 @@ def test_refusals(sess):
                  lambda: sess.paged_attention(h, q, 8, scale=math.inf),
                  lambda: sess.paged_attention(h, q, 8, softcap=math.nan),
                  lambda: sess.paged_attention(h, q, 8, out=q),
+                 lambda: sess.paged_attention(h, q.cpu().numpy(), 8),
+                 lambda: sess.paged_kv_append(h, None, kv),
+                 lambda: sess.dispatch(
+                     dict(op_type="PagedAttention", inputs=list("q__kvcpb"),
+                          attrs=dict(num_heads=8, kv_num_heads=2)),
+                     dict(zip("q_kvcpb", [q.cpu().numpy(), None, s["key"], s["value"], s["cu"],
+                                          s["past"], s["table"]]))),
                  lambda: sess.paged_kv_append(h, q[:, :128].contiguous(), kv, q=q, num_heads=8,
                                               q_out=torch.empty(2, 513, device="cuda")[:, 1:]),
                  lambda: sess.paged_attention(h, q, 8, out=q.half()),
@@ -427,6 +434,11 @@ def test_refusals(sess):
                  lambda: sess.paged_kv_append(h, kv, kv, q_out=q),
                  lambda: sess.paged_kv_append(h, kv, kv, cos_cache=kv),
                  lambda: sess.paged_kv_append(h, kv, kv, cos_cache=kv, sin_cache=kv),
+                 lambda: sess.dispatch(
+                     dict(op_type="PagedAttention", inputs=list("qxykvcpb"),
+                          attrs=dict(num_heads=8, kv_num_heads=2, do_rotary=1)),
+                     dict(q=q, x=kv, y=kv, k=s["key"], v=s["value"], c=s["cu"], p=s["past"],
+                          b=s["table"])),
                  lambda: PagedKVCache(s["key"], s["value"].float(), s["table"], s["cu"], s["past"]),
                  lambda: PagedKVCache(s["key"], s["value"], s["table"].long(), s["cu"], s["past"]),
                  lambda: PagedKVCache(s["key"], s["value"], s["table"], s["cu"][:1], s["past"]),
