@@ -23,6 +23,10 @@
 // rows, a row's hi and lo parts are rows r and r + 8 of one MMA, so the split
 // costs nothing.
 //
+// Bound by memory: 64 sequences of 100 to 8191 keys, fp16, 81 us, 5.9 TB/s (0.90 of
+// the copy); one of 131000 keys 94 us, 5.7 TB/s; bf16 with capped scores and 8 rows
+// 4.2 TB/s, by the products and tanh of two warps a scheduler.
+//
 // Operand layouts avoid shuffles and transposes: the feature order of q.k is
 // free, so a lane's 16-byte chunk of a key row serves as its B operand of two
 // MMAs; the score accumulator is, after exp2, the A operand of p.v; and a
