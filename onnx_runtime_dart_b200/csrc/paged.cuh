@@ -28,7 +28,7 @@ struct PagedSeq {
   int row0, count, past;
 };
 
-__device__ __forceinline__ PagedSeq paged_seq(const PagedView& v, int b, int max_seq, int shared) {
+__host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedView& v, int b, int max_seq, int shared) {
   const int c0 = v.cu[b], c1 = v.cu[b + 1], past = v.past[b];
   PagedSeq s = {c0, c1 - c0, past};
   if (c0 >= 0 && c1 == c0) {  // no tokens: nothing to check
@@ -39,7 +39,9 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedView& v, int b, int max
                     past >= shared &&
                     (int64_t)past + (c1 - c0) <= (int64_t)v.max_pages * v.page_size;
   if (!fits) {
+#ifdef __CUDA_ARCH__
     record_error(v.err, KERR_PAGED_LENGTH);
+#endif
     s.count = 0;
   }
   return s;

@@ -178,9 +178,12 @@ struct StreamPos {
 };
 
 // Sets the sequence of `s` and returns its length in the list per KV head
-// (0: nothing for this kernel).
+// (0: nothing for this kernel).  The length passes 32 bits where a KV head has more
+// query heads than a tile takes: 128 heads and 131072 tokens over fp32 pages are
+// 1048576 row tiles of 2050 places.
 template <int R, int TK, int EXTRA>
-__device__ __forceinline__ int stream_seq(const StreamArgs& p, StreamPos& s, int b, int min_past) {
+__host__ __device__ __forceinline__ long long stream_seq(const StreamArgs& p, StreamPos& s, int b,
+                                                         int min_past) {
   const PagedAttnArgs& a = p.a;
   s.b = b;
   if (p.prefix) {
@@ -202,7 +205,7 @@ __device__ __forceinline__ int stream_seq(const StreamArgs& p, StreamPos& s, int
   }
   s.nrt = (int)((rows + R - 1) / R);
   s.nt = max(1, (s.hi - s.lo + TK - 1) / TK);
-  return (s.nt + EXTRA) * s.nrt;
+  return (long long)(s.nt + EXTRA) * s.nrt;
 }
 
 // One step of a warp: 8 NT keys at `base` (bit r of `valid`: key r is there) in
@@ -563,7 +566,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     for (int b0 = 0; b0 < nb; b0 += 256) {
       StreamPos t;
       const long long n =
-          b0 + tid < nb ? (long long)stream_seq<R, TK, EXTRA>(p, t, b0 + tid, min_past) * G : 0;
+          b0 + tid < nb ? stream_seq<R, TK, EXTRA>(p, t, b0 + tid, min_past) * G : 0;
       long long x = n;
       for (int o = 1; o < 32; o <<= 1) {
         const long long y = __shfl_up_sync(~0u, x, o);
