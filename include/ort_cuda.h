@@ -432,11 +432,11 @@ ORT_CUDA_API int ort_cuda_rotary_embedding(ort_cuda_session* s, const float* X,
  * The structure lives on the host; every pointer in it is a device pointer.
  * Lengths and pages are read on the device when the kernels run, so a
  * recorded call follows what the caller writes there between replays.  What
- * does not fit (cu_seqlens that fall or pass num_tokens, a negative
- * past_lens, more tokens than max_pages * page_size, a page outside
+ * does not fit (cu_seqlens that pass num_tokens or cu_seqlens[batch], a
+ * negative past_lens, more tokens than max_pages * page_size, a page outside
  * [0, num_pages), ...) is never followed: the sequence, or the keys of the
- * page, are left out, and the next synchronising call returns
- * ORT_CUDA_ERR_INVALID_ARG. */
+ * page, are left out, and so are a sequence whose cu_seqlens fall and all
+ * behind it; the next synchronising call returns ORT_CUDA_ERR_INVALID_ARG. */
 #define ORT_CUDA_CACHE_F32 0
 #define ORT_CUDA_CACHE_F16 1
 #define ORT_CUDA_CACHE_BF16 2

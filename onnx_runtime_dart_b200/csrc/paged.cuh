@@ -23,7 +23,8 @@ struct PagedView {
 };
 
 // Sequence b of a call: its first token, its token count and its past; no
-// tokens when its lengths do not fit (see fits).
+// tokens when its lengths do not fit (see fits).  Callers pass no sequence behind the
+// first one whose lengths fall (paged_falls): those before it share no token.
 struct PagedSeq {
   int row0, count, past;
 };
@@ -35,8 +36,9 @@ __host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedView& v, int b
     s.count = 0;
     return s;
   }
-  const bool fits = c0 >= 0 && c0 < c1 && (b == 0 || c0 >= v.cu[b - 1]) && c1 <= v.num_tokens && c1 - c0 <= max_seq && past >= 0 &&
-                    past >= shared &&
+  // (the shared prefix is worked out for the tokens up to cu[batch])
+  const bool fits = c0 >= 0 && c0 < c1 && c1 <= v.num_tokens && c1 <= v.cu[v.batch] &&
+                    c1 - c0 <= max_seq && past >= 0 && past >= shared &&
                     (int64_t)past + (c1 - c0) <= (int64_t)v.max_pages * v.page_size;
   if (!fits) {
 #ifdef __CUDA_ARCH__
@@ -46,13 +48,20 @@ __host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedView& v, int b
   }
   return s;
 }
+__device__ __forceinline__ bool paged_falls(const PagedView& v, int b) {
+  return v.cu[b + 1] < v.cu[b];
+}
 
 // The sequence that token t belongs to: the first that ends behind t, `batch`
-// when there is none.  Whole warp; the lengths of 32 sequences a step.
+// when there is none or a sequence before it falls.  Whole warp; the lengths of 32
+// sequences a step.
 __device__ __forceinline__ int paged_find(const PagedView& v, int t) {
   const int lane = threadIdx.x & 31;
   for (int b0 = 0; b0 < v.batch; b0 += 32) {
-    const unsigned m = __ballot_sync(0xffffffffu, b0 + lane < v.batch && v.cu[b0 + lane + 1] > t);
+    const bool in = b0 + lane < v.batch;
+    const unsigned m = __ballot_sync(0xffffffffu, in && v.cu[b0 + lane + 1] > t);
+    const unsigned f = __ballot_sync(0xffffffffu, in && paged_falls(v, b0 + lane));
+    if (f && (!m || __ffs(f) < __ffs(m))) break;
     if (m) return b0 + __ffs(m) - 1;
   }
   return v.batch;

@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(256, 1) paged_rows_kernel(const __grid_constan
   using S = StreamCfg<float, DP, 16>;
   constexpr int KB = C::KB, NS = C::NS, ROWB = S::ROWB, CHP = S::CHP, KS = S::KS, E = DP / 32;
   extern __shared__ __align__(1024) unsigned char smem[];
-  __shared__ long long s_plan[18];
+  __shared__ long long s_plan[19];
   __shared__ unsigned char s_ok[NS][KB];
   __shared__ int s_last;
   const PagedAttnArgs& a = p.a;

@@ -81,15 +81,20 @@ struct TileRun {
   int k0;         // first block of cur here
   long long total, u0, u1;
   int runs, min_past, TT, align;
+  int nb;  // sequences: those before the first whose lengths fall
 
-  // False: nothing to do.  Whole CTA; scratch of 18 * 8 bytes, free again at return.
+  // False: nothing to do.  Whole CTA; scratch of 19 * 8 bytes, free again at return.
   __device__ __forceinline__ bool plan(const StreamArgs& p, int TT_, int align_, void* scratch) {
     TT = TT_, align = align_;
     const PagedAttnArgs& a = p.a;
     const PagedView& c = a.c;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nt = blockDim.x;
-    const int G = c.kv_heads, nb = p.prefix ? 1 : c.batch;
-    long long* s_scan = static_cast<long long*>(scratch);  // warps, then the start and sequence
+    const int G = c.kv_heads;
+    nb = p.prefix ? 1 : c.batch;
+    // warps, then the start and sequence of u0, the first sequence that falls
+    long long* s_scan = static_cast<long long*>(scratch);
+    int* s_falls = reinterpret_cast<int*>(s_scan + 18);
+    if (tid == 0) *s_falls = INT_MAX;
     min_past = 0;
     if (p.prefix && a.window) {
       int* s_min = static_cast<int*>(scratch);
@@ -117,7 +122,14 @@ struct TileRun {
           if (lane >= o) x += y;
         }
         if (lane == 31) s_scan[warp] = x;
-        __syncthreads();
+        const bool falls = !p.prefix && b0 + tid < nb && paged_falls(c, b0 + tid);
+        if (__syncthreads_or(falls)) {  // the list again, without what lies behind
+          if (falls) atomicMin(s_falls, b0 + tid);
+          __syncthreads();
+          nb = *s_falls;
+          base = 0, b0 = -nt;
+          continue;
+        }
         long long all = 0, before = 0;
         for (int i = 0; i < nt / 32; i++) {
           if (i < warp) before += s_scan[i];
@@ -177,7 +189,6 @@ struct TileRun {
       tile_segment<KB>(p, s, s.rt + 1, 0, TT, align);
       return true;
     }
-    const int nb = p.prefix ? 1 : p.a.c.batch;
     int b = s.b + 1;
     while (b < nb && !tile_seq(p, s, b, min_past, TT, align)) b++;
     if (b >= nb) return false;

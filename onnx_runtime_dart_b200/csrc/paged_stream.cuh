@@ -537,16 +537,18 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
   float2* wml = reinterpret_cast<float2*>(smem + C::RING + 2 * C::QB);  // [8][R]
   __shared__ long long s_scan[8];
   __shared__ long long s_u0base;
-  __shared__ int s_b0, s_min[8], s_last;
+  __shared__ int s_b0, s_min[8], s_last, s_falls;
   __shared__ float s_fac[2][R];   // score factor of a row
   __shared__ int s_pos[2][R];     // position of a row, INT_MIN: no row
 
   const PagedAttnArgs& a = p.a;
   const PagedView& c = a.c;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const int D = c.D, G = c.kv_heads, nb = p.prefix ? 1 : c.batch;
+  const int D = c.D, G = c.kv_heads;
+  int nb = p.prefix ? 1 : c.batch;  // sequences: those before the first whose lengths fall
 
   // ---- this CTA's run of tiles
+  if (tid == 0) s_falls = INT_MAX;
   int min_past = 0;
   if (p.prefix && a.window) {
     min_past = INT_MAX;
@@ -573,7 +575,14 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
         if (lane >= o) x += y;
       }
       if (lane == 31) s_scan[w] = x;
-      __syncthreads();
+      const bool falls = !p.prefix && b0 + tid < nb && paged_falls(c, b0 + tid);
+      if (__syncthreads_or(falls)) {  // the list again, without what lies behind
+        if (falls) atomicMin(&s_falls, b0 + tid);
+        __syncthreads();
+        nb = s_falls;
+        base = 0, b0 = -256;
+        continue;
+      }
       long long all = 0, before = 0;
       for (int i = 0; i < 8; i++) {
         if (i < w) before += s_scan[i];

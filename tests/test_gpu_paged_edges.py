@@ -23,3 +23,51 @@ def test_more_heads_than_a_tile_has_rows(sess, heads, new, past, window, shared,
     s = ref.make(30, dtype, new, past, heads, 1, 64, 16, shared)
     want = ref.attention(s, new, past, heads, window=window)
     near(want, run(sess, s, heads, new, local_window_size=window, shared_len=shared))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("scale", [1, 60])  # few rows, and tiles of 128
+@pytest.mark.parametrize("cu,kept", [
+    ([0, 10, 2, 5, 8], 0),    # a sequence behind the fall would share tokens 5 to 7
+    ([0, 3, 2, 5, 9], 1),
+    ([0, 3, 5, 4, 9], 2),
+    ([0, 3, 5, 9, 8], 2),     # the third passes the last length
+    ([0] * 300 + [3, 2, 5, 9], 300)])
+def test_lengths_that_fall_leave_out_what_lies_behind(sess, cu, kept, scale, dtype):
+    """Sequences before the fall keep their results; no row of another is written, and
+    nothing of them is appended."""
+    heads, G, D, past = 8, 2, 64, 50
+    batch = len(cu) - 1
+    cu = [scale * x for x in cu]
+    new = [b - a if i < kept else 0 for i, (a, b) in enumerate(zip(cu, cu[1:]))]
+    s = ref.make(31, dtype, new, [past] * batch, heads, G, D, 16, garbage=False)
+    n = 9 * scale
+    q = torch.randn((n, heads * D), device="cuda")
+    s = {**s, "q": q, "cu": torch.tensor(cu, dtype=torch.int32, device="cuda"),
+         "table": s["table"].clamp_min(0)}
+    good = sum(new)
+    want = ref.attention({**s, "q": q[:good]}, new, [past] * batch, heads)
+    for shared in (0, 16):
+        if shared:  # one prefix for all: sequence 0's first page
+            s["table"][:, 0] = s["table"][0, 0]
+            want = ref.attention({**s, "q": q[:good]}, new, [past] * batch, heads)
+        out = torch.full_like(q, 7.0)
+        run(sess, s, heads, new, checked=False, out=out, max_seq=n, shared_len=shared)
+        if good:
+            near(want, out[:good])
+        assert (out[good:] == 7.0).all()
+        reported(sess, "cu_seqlens")
+    kv = torch.randn((n, G * D), device="cuda")
+    key, value = s["key"].clone(), s["value"].clone()
+    out = torch.full_like(q, 7.0)
+    sess.paged_kv_append(handle(s), kv, kv, q=q, num_heads=heads, q_out=out)
+    reported(sess, "cu_seqlens")
+    assert torch.equal(out[:good], q[:good]) and (out[good:] == 7.0).all()
+    row = 0
+    for b, m in enumerate(new):
+        pos = torch.arange(past, past + m)
+        where = (s["table"][b].cpu()[pos // 16].long(), pos % 16)
+        for cache in (key, value):
+            cache[where] = kv[row:row + m].view(m, G, D).to(dtype)
+        row += m
+    assert torch.equal(key, s["key"]) and torch.equal(value, s["value"])
