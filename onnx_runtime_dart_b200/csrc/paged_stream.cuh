@@ -34,6 +34,8 @@
 // with byte permutes, its B operand of eight MMAs.
 #pragma once
 
+#include <type_traits>
+
 #include <cuda_bf16.h>
 
 #include "paged.cuh"
@@ -146,6 +148,15 @@ struct Split<float> {
   }
 };
 
+// The base of a row's weights exp2(score - base), from its largest score; what a row
+// keeps as its maximum.  fp16: 15 below it, so that the weights' low parts keep their
+// bits, rounded up, so that none passes 2^15 however large the scores are (a score of
+// 2^24 less 15, rounded to nearest, may be 16 below it, and 2^16 is no fp16 number).
+template <typename T>
+__device__ __forceinline__ float row_base(float mx) {
+  return std::is_same<T, __half>::value ? __fadd_ru(mx, -15.f) : mx;
+}
+
 template <typename T, int DP, int R>
 struct StreamCfg {
   static constexpr bool F32 = sizeof(T) == 4;
@@ -211,7 +222,7 @@ __host__ __device__ __forceinline__ long long stream_seq(const StreamArgs& p, St
 // One step of a warp: 8 NT keys at `base` (bit r of `valid`: key r is there) in
 // shared memory at kt, vt against its R rows, whose operands are qs, score factors
 // fac, positions pos (from pos_lo to pos_hi over the rows); m, l, o: the rows'
-// running maximum, this lane's part of the sum, output.
+// running maximum (row_base), this lane's part of the sum, output.
 template <typename T, int DP, int R, int NT = StreamCfg<T, DP, R>::KW / 8>
 __device__ __forceinline__ void stream_step(const uint4* qs, const unsigned char* kt,
                                             const unsigned char* vt, unsigned valid, int base,
@@ -292,7 +303,7 @@ __device__ __forceinline__ void stream_step(const uint4* qs, const unsigned char
         if (R == 8) x += s[t][0][e + 2] + s[t][1][e + 2];
         x *= fac[rr];
         if (softcap) x = tanhf(x);
-        pr[rr][t][e] = x * t_mul;
+        pr[rr][t][e] = __fmul_rn(x, t_mul);  // not fused with the subtraction of the base below
       }
   if (!full) {
 #pragma unroll
@@ -309,22 +320,21 @@ __device__ __forceinline__ void stream_step(const uint4* qs, const unsigned char
   float corr[NR];
 #pragma unroll
   for (int rr = 0; rr < NR; rr++) {
-    float mx = m[rr];
+    float mx = -INFINITY;
 #pragma unroll
     for (int t = 0; t < NT; t++) mx = fmaxf(mx, fmaxf(pr[rr][t][0], pr[rr][t][1]));
     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+    mx = fmaxf(m[rr], row_base<T>(mx));
     const float mb = mx == -INFINITY ? 0.f : mx;
     corr[rr] = ex2(m[rr] - mb);
     m[rr] = mx;
-    // p scaled by 2^15 for fp16: its low part then keeps its bits
-    const float sub = PARTS == 2 && !F32 ? mb - 15.f : mb;
     float sum = 0.f;
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        pr[rr][t][e] = ex2(pr[rr][t][e] - sub);
+        pr[rr][t][e] = ex2(pr[rr][t][e] - mb);
         sum += pr[rr][t][e];
       }
     l[rr] = l[rr] * corr[rr] + sum;

@@ -554,9 +554,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
         }
         mx = fmaxf(mx, mx2);
-        if (mx != -INFINITY) mx = CAP ? tanhf(mx * fac) * p.t_mul : mx * cmul;
-        const float mn = fmaxf(m, mx), mb = mn == -INFINITY ? 0.f : mn;
-        const float corr = ex2(m - mb), sub = PARTS == 2 ? mb - 15.f : mb;
+        if (mx != -INFINITY) mx = CAP ? __fmul_rn(tanhf(mx * fac), p.t_mul) : __fmul_rn(mx, cmul);
+        const float mn = fmaxf(m, row_base<T>(mx)), sub = mn == -INFINITY ? 0.f : mn;
+        const float corr = ex2(m - sub);
         m = mn;
 
         // values only some rows see: an infinity or NaN among them must not reach
@@ -592,7 +592,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
         // weights, over the scores
         uint64_t sums[2] = {0, 0};
-        const uint64_t cmul2 = pack2(cmul, cmul), sub2 = pack2(-sub, -sub);
+        // The fused product is not rounded as the maximum's was, which below 2^20 is no
+        // more than 2^-5 apart.  Where the base is larger, scores are rounded like it.
+        const bool big = !CAP && fabsf(m) >= 1048576.f;
+        const uint64_t cmul2 = big ? pack2(1.f, 1.f) : pack2(cmul, cmul);
+        const uint64_t sub2 = big ? 0 : pack2(-sub, -sub);
+        auto round_big = [&](uint32_t(&r)[16]) {
+          if (!big) return;
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            r[e] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(r[e]), cmul), sub));
+        };
         // 16 scores: exp2, their sum, the parts
         auto weigh = [&](auto masked, int st, const uint32_t (&r)[16], uint32_t vw) {
           uint64_t x[8];
@@ -639,6 +649,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             tmem_ld16(ts + 32 * i, ra);
             tmem_ld16(ts + 32 * i + 16, rb);
             tmem_ld_wait();
+            round_big(ra);
+            round_big(rb);
             weigh(std::false_type(), 2 * i, ra, 0u);
             weigh(std::false_type(), 2 * i + 1, rb, 0u);
           }
@@ -649,6 +661,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             tmem_ld16(ts + 16 * i, r);
             const uint32_t vw = seen(i >> 1) >> (16 * (i & 1));
             tmem_ld_wait();
+            round_big(r);
             weigh(std::true_type(), i, r, vw);
           }
         }

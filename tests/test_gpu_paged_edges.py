@@ -71,3 +71,37 @@ def test_lengths_that_fall_leave_out_what_lies_behind(sess, cu, kept, scale, dty
             cache[where] = kv[row:row + m].view(m, G, D).to(dtype)
         row += m
     assert torch.equal(key, s["key"]) and torch.equal(value, s["value"])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("size", [2.0 ** 23, 1e8, 1e12])
+@pytest.mark.parametrize("new,past,shared", [([1, 3], [90, 200], 0), ([140, 60], [0, 33], 0),
+                                             ([1, 150], [90, 200], 80)])
+def test_scores_that_leave_one_key(sess, new, past, shared, size, dtype):
+    """Scores so large that a row's weight is all on its largest.  Scores are held to
+    2^-20 of sum |q k| at least; rows whose two largest lie 2^-16 of it apart (near all)
+    give that key's value."""
+    heads, G, D = 8, 2, 64
+    s = ref.make(32, dtype, new, past, heads, G, D, 16, shared)
+    s["q"] *= size
+    want = ref.attention(s, new, past, heads)
+    got = run(sess, s, heads, new, shared_len=shared)
+    assert torch.isfinite(got).all()
+    clear = torch.zeros((sum(new), heads), dtype=torch.bool)
+    row = 0
+    for b, (n, p0) in enumerate(zip(new, past)):
+        pos = torch.arange(n + p0)
+        k = s["key"][s["table"][b].cpu()[pos // 16].long(), pos % 16].double()
+        for i in range(n):
+            q = s["q"][row].double().view(G, heads // G, D)
+            sc = torch.einsum("ghd,tgd->ght", q, k[:p0 + i + 1])
+            size_of = torch.einsum("ghd,tgd->ght", q.abs(), k[:p0 + i + 1].abs()).amax(-1)
+            if p0 + i:
+                top = sc.topk(2, -1).values
+                clear[row] = (top[..., 0] - top[..., 1] > 2.0 ** -16 * size_of).flatten().cpu()
+            else:
+                clear[row] = True
+            row += 1
+    assert clear.float().mean() > 0.99
+    clear = clear.cuda()
+    near(want.view(-1, heads, D)[clear], got.view(-1, heads, D)[clear])
