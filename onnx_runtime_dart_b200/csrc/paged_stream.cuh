@@ -188,13 +188,10 @@ struct StreamPos {
   int lo, hi, nt, nrt;      // its keys, key tiles and row tiles
 };
 
-// Sets the sequence of `s` and returns its length in the list per KV head
-// (0: nothing for this kernel).  The length passes 32 bits where a KV head has more
-// query heads than a tile takes: 128 heads and 131072 tokens over fp32 pages are
-// 1048576 row tiles of 2050 places.
-template <int R, int TK, int EXTRA>
-__host__ __device__ __forceinline__ long long stream_seq(const StreamArgs& p, StreamPos& s, int b,
-                                                         int min_past) {
+// Sets the sequence of `s`; false: nothing for this kernel.
+template <int R, int TK>
+__host__ __device__ __forceinline__ bool stream_seq(const StreamArgs& p, StreamPos& s, int b,
+                                                    int min_past) {
   const PagedAttnArgs& a = p.a;
   s.b = b;
   if (p.prefix) {
@@ -212,10 +209,18 @@ __host__ __device__ __forceinline__ long long stream_seq(const StreamArgs& p, St
   if (rows == 0 || (!p.prefix && rows > p.max_rows)) {
     s.count = 0;
     s.nt = s.nrt = 0;
-    return 0;
+    return false;
   }
   s.nrt = (int)((rows + R - 1) / R);
   s.nt = max(1, (s.hi - s.lo + TK - 1) / TK);
+  return true;
+}
+
+// The sequence's length in the list per KV head.  It passes 32 bits where a KV head has
+// more query heads than a tile takes: 128 heads and 131072 tokens over fp32 pages are
+// 1048576 row tiles of 2050 places.
+template <int EXTRA>
+__host__ __device__ __forceinline__ long long stream_places(const StreamPos& s) {
   return (long long)(s.nt + EXTRA) * s.nrt;
 }
 
@@ -320,12 +325,13 @@ __device__ __forceinline__ void stream_step(const uint4* qs, const unsigned char
   float corr[NR];
 #pragma unroll
   for (int rr = 0; rr < NR; rr++) {
-    float mx = -INFINITY;
+    constexpr bool shifted = std::is_same<T, __half>::value;
+    float mx = shifted ? -INFINITY : m[rr];
 #pragma unroll
     for (int t = 0; t < NT; t++) mx = fmaxf(mx, fmaxf(pr[rr][t][0], pr[rr][t][1]));
     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-    mx = fmaxf(m[rr], row_base<T>(mx));
+    if (shifted) mx = fmaxf(m[rr], row_base<T>(mx));
     const float mb = mx == -INFINITY ? 0.f : mx;
     corr[rr] = ex2(m[rr] - mb);
     m[rr] = mx;
@@ -577,8 +583,9 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     long long base = 0;
     for (int b0 = 0; b0 < nb; b0 += 256) {
       StreamPos t;
-      const long long n =
-          b0 + tid < nb ? stream_seq<R, TK, EXTRA>(p, t, b0 + tid, min_past) * G : 0;
+      const long long n = b0 + tid < nb && stream_seq<R, TK>(p, t, b0 + tid, min_past)
+                              ? stream_places<EXTRA>(t) * G
+                              : 0;
       long long x = n;
       for (int o = 1; o < 32; o <<= 1) {
         const long long y = __shfl_up_sync(~0u, x, o);
@@ -628,7 +635,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
   }
   __syncthreads();
   if ((int)blockIdx.x >= runs || u0 >= u1) return;
-  stream_seq<R, TK, EXTRA>(p, cur, s_b0, min_past);
+  stream_seq<R, TK>(p, cur, s_b0, min_past);
   long long seg_u = s_u0base;  // place of tile 0 of the segment in the list
   {
     const int len = cur.nt + EXTRA;
@@ -658,7 +665,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     if (++s.rt < s.nrt) return;
     s.rt = 0;
     for (int b = s.b + 1; b < nb; b++)
-      if (stream_seq<R, TK, EXTRA>(p, s, b, min_past)) return;
+      if (stream_seq<R, TK>(p, s, b, min_past)) return;
   };
   // the page of lane r's key (r < KW) of a tile, and whether it has one
   auto page_of = [&](const StreamPos& s, int& slot) {

@@ -593,16 +593,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // weights, over the scores
         uint64_t sums[2] = {0, 0};
         // The fused product is not rounded as the maximum's was, which below 2^20 is no
-        // more than 2^-5 apart.  Where the base is larger, scores are rounded like it.
-        const bool big = !CAP && fabsf(m) >= 1048576.f;
-        const uint64_t cmul2 = big ? pack2(1.f, 1.f) : pack2(cmul, cmul);
-        const uint64_t sub2 = big ? 0 : pack2(-sub, -sub);
-        auto round_big = [&](uint32_t(&r)[16]) {
-          if (!big) return;
-#pragma unroll
-          for (int e = 0; e < 16; e++)
-            r[e] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(r[e]), cmul), sub));
-        };
+        // more than 2^-5 apart.  A warp with a larger base rounds its scores like it.
+        const bool big = !CAP && __any_sync(~0u, fabsf(m) >= 1048576.f);
+        const uint64_t cmul2 = pack2(cmul, cmul), sub2 = pack2(-sub, -sub);
         // 16 scores: exp2, their sum, the parts
         auto weigh = [&](auto masked, int st, const uint32_t (&r)[16], uint32_t vw) {
           uint64_t x[8];
@@ -612,6 +605,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (CAP)
               t = make_float2(fmaf(tanhf(t.x * fac), p.t_mul, -sub),
                               fmaf(tanhf(t.y * fac), p.t_mul, -sub));
+            else if (masked && big)
+              t = make_float2(__fsub_rn(__fmul_rn(t.x, cmul), sub),
+                              __fsub_rn(__fmul_rn(t.y, cmul), sub));
             else
               t = unpack2(fma2(pack2(t.x, t.y), cmul2, sub2));
             t.x = ex2(t.x), t.y = ex2(t.y);
@@ -642,15 +638,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             tmem_st8(ts + KB + 8 * st, make_uint4(w2[0], w2[1], w2[2], w2[3]),
                      make_uint4(w2[4], w2[5], w2[6], w2[7]));
         };
-        if (full) {
+        if (full && !big) {
 #pragma unroll 1
           for (int i = 0; i < KB / 32; i++) {
             uint32_t ra[16], rb[16];
             tmem_ld16(ts + 32 * i, ra);
             tmem_ld16(ts + 32 * i + 16, rb);
             tmem_ld_wait();
-            round_big(ra);
-            round_big(rb);
             weigh(std::false_type(), 2 * i, ra, 0u);
             weigh(std::false_type(), 2 * i + 1, rb, 0u);
           }
@@ -661,7 +655,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             tmem_ld16(ts + 16 * i, r);
             const uint32_t vw = seen(i >> 1) >> (16 * (i & 1));
             tmem_ld_wait();
-            round_big(r);
             weigh(std::true_type(), i, r, vw);
           }
         }

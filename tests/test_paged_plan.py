@@ -32,7 +32,7 @@ long long places(int count, int past, int group) {
   p.a.group = group;
   p.max_rows = INT_MAX;
   StreamPos s;
-  return stream_seq<R, TK, EXTRA>(p, s, 0, 0);
+  return stream_seq<R, TK>(p, s, 0, 0) ? stream_places<EXTRA>(s) : 0;
 }
 
 int main(int argc, char** argv) {
