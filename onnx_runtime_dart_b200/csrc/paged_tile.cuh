@@ -153,10 +153,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint32_t* kvalid = reinterpret_cast<uint32_t*>(stats + 256);  // [8][4]
   uint64_t* bars = reinterpret_cast<uint64_t*>(kvalid + 32);
   uint64_t *kfull = bars, *kempty = kfull + NK, *vfull = kempty + NK, *vempty = vfull + NV,
-           *sfull = vempty + NV, *pfull = sfull + 2, *pvfull = pfull + 2, *qfull = pvfull + 2;
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(qfull + 1);
+           *sfull = vempty + NV, *pfull = sfull + 2, *pvfull = pfull + 2, *qfull = pvfull + 2,
+           *done = qfull + 1;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(done + 1);
   int* s_last = reinterpret_cast<int*>(tmem_at + 1);
-  static_assert((2 * 4 + 2 * 4 + 7) * 8 + 8 <= 256, "barriers");
+  static_assert((2 * 4 + 2 * 4 + 8) * 8 + 8 <= 256, "barriers");
 
   const StreamArgs& p = args.s;
   const PagedAttnArgs& a = p.a;
@@ -182,6 +183,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     for (int i = 0; i < NV; i++) mbar_init(vfull + i, rows_tma ? 1 : 3), mbar_init(vempty + i, 1);
     for (int i = 0; i < 2; i++) mbar_init(sfull + i, 1), mbar_init(pfull + i, 128), mbar_init(pvfull + i, 1);
     mbar_init(qfull, 256);
+    mbar_init(done, 1);
     fence_mbarrier_init();
   }
   if (warp == 8) {
@@ -262,6 +264,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         if (!next(cur, seg, k0)) break;
       }
+      // every product has ended before TMEM is given up, also where a wait ran out
+      if (elect_one()) mma_commit(done);
+      __syncwarp();
+      if (!mbar_wait(done, 0)) record_error(c.err, KERR_WAIT_DRAIN);
     } else if (rows_tma) {
       // ---- TMA: warp 9 keys, warp 10 values; lane i the box of tokens i * rows_tma
       if (warp <= 10) {
@@ -519,10 +525,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int k = wg; k < n; k += 2) {
         const int base = cur.lo + (k0 + k) * KB;
         wait(sfull + wg, sc & 1);
-        bool full = base + KB - 1 <= all_hi && base + KB <= cur.hi && base >= first &&
-                    (!a.window || base > all_lo - a.window);
+        // Whether all rows see the whole block (alike for all threads: a barrier below
+        // depends on it), and whether its pages are there too (alike within a warp; where
+        // a wait ran out, one warp may read what another does not).
+        const bool inner = base + KB - 1 <= all_hi && base + KB <= cur.hi && base >= first &&
+                           (!a.window || base > all_lo - a.window);
         const uint32_t* kv = kvalid + ((gb + k) & 7) * 4;
+        bool full = inner;
         for (int i = 0; i < KB / 32; i++) full = full && kv[i] == ~0u;
+        full = __all_sync(~0u, full);
         auto seen = [&](int i) {  // keys of the block's word i that the row sees
           const int b = base + 32 * i, x0 = max(from - b, 0), x1 = min(pos - b, 31);
           return pos < b || x0 > x1 ? 0u : kv[i] & (~0u >> (31 - x1)) & (~0u << x0);
@@ -587,7 +598,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
           odd = (top & 0x80008000u) != 0;
           fence_proxy_async_smem();
-          odd = bar_or(2 + wg, 128, odd);
+          odd = !inner && bar_or(2 + wg, 128, odd);
         }
 
         // weights, over the scores

@@ -105,3 +105,37 @@ def test_scores_that_leave_one_key(sess, new, past, shared, size, dtype):
     assert clear.float().mean() > 0.99
     clear = clear.cuda()
     near(want.view(-1, heads, D)[clear], got.view(-1, heads, D)[clear])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("page", [16, 12])  # TMA boxes, copies of 16 bytes
+@pytest.mark.parametrize("new,past,window", [([140, 90], [900, 700], 0), ([1, 2], [900, 700], 0),
+                                             ([150, 40], [900, 700], 300)])
+def test_missing_pages_inside_what_all_rows_see(sess, new, past, window, page, dtype):
+    """Keys of a page that is not there are left out of blocks that every row sees, and the
+    rows' own keys behind them are not."""
+    heads, G, D = 8, 2, 64
+    s = ref.make(33, dtype, new, past, heads, G, D, page)
+    want = torch.zeros((sum(new), heads, D), dtype=torch.float64, device="cuda")
+    bad = {b: [p // page - 30 + b, p // page - 7, p // page - 12] for b, p in enumerate(past)}
+    row = 0
+    for b, (n, p0) in enumerate(zip(new, past)):
+        pos = torch.arange(n + p0, device="cuda")
+        where = (s["table"][b][pos // page].long(), pos % page)
+        k, v = s["key"][where].double(), s["value"][where].double()
+        gone = torch.isin(pos // page, torch.tensor(bad[b], device="cuda"))
+        for i in range(n):
+            q = s["q"][row].double().view(G, heads // G, D)
+            sc = torch.einsum("ghd,tgd->ght", q, k) / math.sqrt(D)
+            hide = gone | (pos > p0 + i)
+            if window:
+                hide = hide | (pos <= p0 + i - window)
+            weight = torch.softmax(sc.masked_fill(hide, -math.inf), -1)
+            want[row] = torch.einsum("ght,tgd->ghd", weight, v).reshape(heads, D)
+            row += 1
+    for b, pages in bad.items():
+        for p, x in zip(pages, (-3, 2 ** 30, s["key"].shape[0])):
+            s["table"][b, p] = x
+    got = run(sess, s, heads, new, checked=False, local_window_size=window)
+    near(want.flatten(1), got)
+    reported(sess, "page")
