@@ -54,10 +54,17 @@ void CUDART_CB release_hold(void* p) {
   delete h;
 }
 
-// A new zeroed workspace, also while a stream is being captured.
-int new_buf(PagedScratch* w, size_t bytes, PagedScratch::Buf* out) {
+// Allocating and freeing are allowed in its scope while a stream of this thread, this
+// one or another, is being captured.
+struct RelaxedCapture {
   cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  ORTC_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// A new zeroed workspace.
+int new_buf(PagedScratch* w, size_t bytes, PagedScratch::Buf* out) {
+  RelaxedCapture relaxed;
   PagedScratch::Buf b;
   cudaStream_t st = nullptr;
   cudaError_t e = cudaMalloc(&b.p, bytes);
@@ -66,7 +73,6 @@ int new_buf(PagedScratch* w, size_t bytes, PagedScratch::Buf* out) {
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   if (st) cudaStreamDestroy(st);
   if (e != cudaSuccess && b.p) cudaFree(b.p);
-  cudaThreadExchangeStreamCaptureMode(&mode);
   if (e != cudaSuccess) return cuda_fail(e, "paged attention workspace");
   b.bytes = bytes;
   w->all.push_back(b.p);
@@ -87,6 +93,7 @@ int paged_scratch(ort_cuda_session* s, size_t bytes, void** out) {
     PagedScratch::Buf& b = w->streams[s->stream];
     if (bytes > b.bytes) {
       if (b.p) {
+        RelaxedCapture relaxed;
         ORTC_CUDA(cudaStreamSynchronize(s->stream));
         ORTC_CUDA(cudaFree(b.p));
         w->all.erase(std::find(w->all.begin(), w->all.end(), b.p));

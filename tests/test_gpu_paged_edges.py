@@ -139,3 +139,26 @@ def test_missing_pages_inside_what_all_rows_see(sess, new, past, window, page, d
     got = run(sess, s, heads, new, checked=False, local_window_size=window)
     near(want.flatten(1), got)
     reported(sess, "page")
+
+
+def test_workspace_grows_while_another_stream_is_captured(sess):
+    """A call outside the capture, on a stream whose workspace is too small for it, in a
+    thread that captures another stream (in the mode that forbids the most)."""
+    small = ref.make(34, F16, [1], [300], 8, 2, 64, 16)
+    large = ref.make(35, F16, [200, 90], [100, 700], 8, 2, 64, 16)
+    want_small, want_large = run(sess, small, 8, [1]), run(sess, large, 8, [200, 90])
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run(sess, small, 8, [1])
+    out, h = torch.zeros_like(large["q"]), handle(large)
+    got, hs = torch.zeros_like(small["q"]), handle(small)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="global"):
+        sess.paged_attention(hs, small["q"], 8, max_seq=1, out=got)
+        with torch.cuda.stream(side):
+            sess.paged_attention(h, large["q"], 8, max_seq=200, out=out)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want_large) and torch.equal(got, want_small)
+    sess.sync()
