@@ -490,8 +490,9 @@ ORT_CUDA_API int ort_cuda_paged_kv_append(ort_cuda_session* s, const ort_cuda_pa
  * fp32 results whatever the cache's type: products, softmax statistics and
  * sums keep 22 bits or more.  Device pointers only; stream-ordered.  A call
  * uses a workspace of its stream (or of the graph being captured), so calls
- * on different streams may run at the same time; the session must outlive the
- * graphs that were captured with its calls. */
+ * on different streams may run at the same time (two instances of one captured
+ * graph share it and may not); the session must outlive the graphs that were
+ * captured with its calls. */
 ORT_CUDA_API int ort_cuda_paged_attention(ort_cuda_session* s, const ort_cuda_paged_cache* cache,
                                           const float* Q, int64_t q_stride, int64_t num_tokens,
                                           int64_t max_seq, int num_heads, double scale,

@@ -19,9 +19,11 @@ namespace ortc {
 // ---- workspaces ----------------------------------------------------------------
 // A call's workspace belongs to the stream it is launched on, or to the graph
 // being captured on that stream: calls on two streams, and two captured graphs
-// replayed at once, never share one.  A graph's workspace is handed back when
-// the graph and everything instantiated from it are gone (a CUDA user object),
-// and is reused by later captures.  The first kTicketBytes are zero between calls.
+// replayed at once, never share one.  Streams are told apart by their ids: a handle
+// may come again when its stream is destroyed, even with work of it still to run.  A
+// graph's workspace is handed back when the graph and everything instantiated from it
+// are gone (a CUDA user object), and is reused by later captures.  The first
+// kTicketBytes are zero between calls.
 struct PagedScratch {
   struct Buf {
     void* p = nullptr;
@@ -31,9 +33,12 @@ struct PagedScratch {
     std::mutex m;
     std::vector<Buf> idle;
   };
+  struct OfStream : Buf {
+    cudaStream_t handle = nullptr;
+  };
   std::shared_ptr<Pool> pool = std::make_shared<Pool>();
   std::vector<void*> all;
-  std::map<cudaStream_t, Buf> streams;
+  std::map<unsigned long long, OfStream> streams;  // by the stream's id
   unsigned long long capture = 0;  // the capture `captured` belongs to
   std::map<cudaStream_t, Buf> captured;
 };
@@ -80,6 +85,16 @@ int new_buf(PagedScratch* w, size_t bytes, PagedScratch::Buf* out) {
   return ORT_CUDA_OK;
 }
 
+// Frees a workspace.  cudaFree waits for what still runs on it.
+int free_buf(PagedScratch* w, PagedScratch::Buf* b) {
+  if (!b->p) return ORT_CUDA_OK;
+  RelaxedCapture relaxed;
+  ORTC_CUDA(cudaFree(b->p));
+  w->all.erase(std::find(w->all.begin(), w->all.end(), b->p));
+  *b = PagedScratch::Buf();
+  return ORT_CUDA_OK;
+}
+
 int paged_scratch(ort_cuda_session* s, size_t bytes, void** out) {
   *out = nullptr;
   if (bytes == 0) return ORT_CUDA_OK;
@@ -90,16 +105,32 @@ int paged_scratch(ort_cuda_session* s, size_t bytes, void** out) {
   cudaGraph_t graph = nullptr;
   ORTC_CUDA(cudaStreamGetCaptureInfo_v2(s->stream, &status, &id, &graph, nullptr, nullptr));
   if (status == cudaStreamCaptureStatusNone) {
-    PagedScratch::Buf& b = w->streams[s->stream];
+    unsigned long long stream = 0;  // (not to be had while it is captured)
+    ORTC_CUDA(cudaStreamGetId(s->stream, &stream));
+    auto at = w->streams.find(stream);
+    if (at == w->streams.end()) {
+      // another stream of this handle is gone, and its workspace goes too (the handle of
+      // the per-thread stream is one stream for every host thread)
+      for (auto i = w->streams.begin(); i != w->streams.end();)
+        if (i->second.handle == s->stream && s->stream != cudaStreamPerThread) {
+          const int rc = free_buf(w, &i->second);
+          if (rc) return rc;
+          i = w->streams.erase(i);
+        } else {
+          ++i;
+        }
+      at = w->streams.emplace(stream, PagedScratch::OfStream()).first;
+      at->second.handle = s->stream;
+    }
+    PagedScratch::Buf& b = at->second;
     if (bytes > b.bytes) {
       if (b.p) {
         RelaxedCapture relaxed;
         ORTC_CUDA(cudaStreamSynchronize(s->stream));
-        ORTC_CUDA(cudaFree(b.p));
-        w->all.erase(std::find(w->all.begin(), w->all.end(), b.p));
-        b = PagedScratch::Buf();
       }
-      const int rc = new_buf(w, bytes, &b);
+      int rc = free_buf(w, &b);
+      if (rc) return rc;
+      rc = new_buf(w, bytes, &b);
       if (rc) return rc;
     }
     *out = b.p;

@@ -162,3 +162,43 @@ def test_workspace_grows_while_another_stream_is_captured(sess):
     torch.cuda.synchronize()
     assert torch.equal(out, want_large) and torch.equal(got, want_small)
     sess.sync()
+
+
+def test_stream_destroyed_with_work_to_run_and_its_handle_used_again(sess):
+    """Work of a destroyed stream still runs; the next stream may get its handle, and must
+    not get its workspace while that is so."""
+    import ctypes
+    rt = ctypes.CDLL("libcudart.so.12")
+
+    def create():
+        p = ctypes.c_void_p()
+        assert rt.cudaStreamCreateWithFlags(ctypes.byref(p), 1) == 0
+        return p.value
+
+    cases = []
+    for i, (new, past) in enumerate((([1] * 3, [9000] * 3), ([1] * 8, [4000] * 8))):
+        s = ref.make(36 + i, F16, new, past, 8, 2, 128, 16)
+        cases.append((s, handle(s), run(sess, s, 8, new), torch.zeros_like(s["q"])))
+    (s0, h0, want0, out0), (s1, h1, want1, out1) = cases
+    outs = [torch.zeros_like(out1) for _ in range(30)]
+    torch.cuda.synchronize()
+    first, others = create(), []
+    try:
+        sess.set_stream(first)
+        with torch.cuda.stream(torch.cuda.ExternalStream(first)):
+            torch.cuda._sleep(40_000_000)  # some 20 ms
+        sess.paged_attention(h0, s0["q"], 8, max_seq=1, out=out0)
+        assert rt.cudaStreamDestroy(ctypes.c_void_p(first)) == 0
+        while first not in others and len(others) < 16:
+            others.append(create())
+        sess.set_stream(others[-1])
+        for out in outs:
+            sess.paged_attention(h1, s1["q"], 8, max_seq=1, out=out)
+        torch.cuda.synchronize()
+        sess.sync()
+        assert torch.equal(out0, want0)
+        assert all(torch.equal(out, want1) for out in outs)
+    finally:
+        sess.set_stream(None)
+        for p in others:
+            rt.cudaStreamDestroy(ctypes.c_void_p(p))
