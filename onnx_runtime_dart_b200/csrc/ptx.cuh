@@ -21,6 +21,14 @@ enum KernelError : int {
   KERR_PAGED_POSITION = 18,
 };
 
+// The word of the host-mapped error area that a code is written to: waits share the
+// first (one that ran out is reported whatever else is), what does not fit has a word
+// each.
+constexpr int kErrorWords = 4;
+__host__ __device__ constexpr int error_word(int code) {
+  return code < KERR_PAGED_LENGTH ? 0 : code - KERR_PAGED_LENGTH + 1;
+}
+
 // Upper bound of any single wait (ns of %globaltimer).  Every legitimate
 // wait in these kernels is microseconds; the bound only turns a bug into an
 // error status instead of a hung GPU.
@@ -245,7 +253,7 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
 }
 
 __device__ __forceinline__ void record_error(int* err, int code) {
-  if (err) *reinterpret_cast<volatile int*>(err) = code;
+  if (err) reinterpret_cast<volatile int*>(err)[error_word(code)] = code;
 }
 
 }  // namespace ortc

@@ -22,8 +22,8 @@
 #include <vector>
 
 #include "common.cuh"
+#include "kernel_errors.cuh"
 #include "nccl_dl.cuh"
-#include "ptx.cuh"
 
 namespace ortc {
 
@@ -163,32 +163,13 @@ bool replicate_nbits(const ort_cuda_session* s, int64_t bytes) {
   return bytes <= (s->replicate_bytes >= 0 ? s->replicate_bytes : kReplicateBytes);
 }
 
-// A kernel whose bounded wait gave up wrote a code into the host-mapped
-// error word; report it once.
 }  // namespace
 
 int check_kernel_error(ort_cuda_session* s) {
-  volatile int* e = s->err_host;
-  if (!e || *e == 0) return ORT_CUDA_OK;
-  const int code = *e;
-  *e = 0;
-  switch (code) {
-    case KERR_PAGED_LENGTH:
-      return fail(ORT_CUDA_ERR_INVALID_ARG,
-                  "paged KV cache: cu_seqlens and past_lens do not fit num_tokens, max_seq, "
-                  "shared_len or max_pages * page_size; the sequence was left out");
-    case KERR_PAGED_PAGE:
-      return fail(ORT_CUDA_ERR_INVALID_ARG,
-                  "paged KV cache: block_table names a page outside [0, num_pages); its tokens "
-                  "were left out");
-    case KERR_PAGED_POSITION:
-      return fail(ORT_CUDA_ERR_INVALID_ARG,
-                  "paged KV cache: a position is outside the cos/sin caches; its token was left "
-                  "out");
-  }
-  return fail(ORT_CUDA_ERR_TIMEOUT,
-              "a kernel wait exceeded its bound (code " + std::to_string(code) +
-                  "); the kernel stopped and returned");
+  if (!s->err_host) return ORT_CUDA_OK;
+  std::string msg;
+  const int rc = take_kernel_errors(s->err_host, &msg);
+  return rc == ORT_CUDA_OK ? rc : fail(rc, msg);
 }
 
 // Bounded wait on the session stream.  Polls an event so that a collective
@@ -366,7 +347,7 @@ static int open_common(int device, int mode, ort_cuda_session** out) {
     delete s;
     return cuda_fail(e, "cudaHostAlloc(error word)");
   }
-  *s->err_host = 0;
+  std::memset(s->err_host, 0, 64);
   *out = s;
   return ORT_CUDA_OK;
 }

@@ -202,3 +202,14 @@ def test_stream_destroyed_with_work_to_run_and_its_handle_used_again(sess):
         sess.set_stream(None)
         for p in others:
             rt.cudaStreamDestroy(ctypes.c_void_p(p))
+
+
+@pytest.mark.parametrize("new", [[1, 2], [80, 70]])
+def test_lengths_and_pages_are_reported_together(sess, new):
+    s = ref.make(38, F16, new, [300, 400], 8, 2, 64, 16)
+    s["table"][0, 3] = -1
+    s["past"][1] = -1
+    run(sess, s, 8, new, checked=False)
+    with pytest.raises(ValueError, match="cu_seqlens.*block_table"):
+        sess.sync()
+    sess.sync()
