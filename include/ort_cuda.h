@@ -476,10 +476,11 @@ ORT_CUDA_API int ort_cuda_paged_kv_append(ort_cuda_session* s, const ort_cuda_pa
  * keys and values (ort_cuda_paged_kv_append first).  The query at position p
  * of its sequence sees keys j <= p of that sequence and, with window > 0,
  * only j > p - window (window keys, its own among them; <= 0: all).  Scores
- * are scale * q.k (scale <= 0: 1/sqrt(head_size)) and, with softcap > 0,
- * softcap * tanh(score / softcap).  Q [num_tokens, num_heads * head_size] fp32
- * with row stride q_stride; out [num_tokens, num_heads * head_size] fp32,
- * contiguous, apart from Q.  Query head h reads KV head h / (num_heads / kv_num_heads).
+ * are scale * q.k (scale <= 0: 1/sqrt(head_size); 2^-100 to 2^100) and, with
+ * softcap > 0 (2^-20 to 2^20), softcap * tanh(score / softcap).
+ * Q [num_tokens, num_heads * head_size] fp32 with row stride q_stride; out
+ * [num_tokens, num_heads * head_size] fp32, contiguous, apart from Q.  Query
+ * head h reads KV head h / (num_heads / kv_num_heads).
  *   max_seq     bound of the tokens of any one sequence of the call (a
  *               sequence with more is left out and reported)
  *   shared_len  > 0: the first shared_len positions of every sequence hold

@@ -574,6 +574,12 @@ ORT_CUDA_API int ort_cuda_paged_attention(ort_cuda_session* s, const ort_cuda_pa
              "paged attention: shared_len exceeds max_pages * page_size");
   ORTC_CHECK(std::isfinite(scale) && std::isfinite(softcap), ORT_CUDA_ERR_INVALID_ARG,
              "paged attention: scale and softcap must be finite");
+  // Within fp32 with room for their quotient; a cap of 2^20 at most, since weights over
+  // fp16 pages have room for tanhf's last bits times the cap (2^15.4 of 2^15.99).
+  ORTC_CHECK((scale <= 0 || (scale >= 0x1p-100 && scale <= 0x1p100)) &&
+                 (softcap <= 0 || (softcap >= 0x1p-20 && softcap <= 0x1p20)),
+             ORT_CUDA_ERR_INVALID_ARG,
+             "paged attention: scale lies in [2^-100, 2^100], softcap in [2^-20, 2^20]");
   if (num_tokens == 0 || cache->batch == 0) return ORT_CUDA_OK;
   ORTC_CHECK(Q && out, ORT_CUDA_ERR_INVALID_ARG, "NULL argument");
   ORTC_CHECK(num_tokens * num_heads <= INT_MAX, ORT_CUDA_ERR_INVALID_ARG,

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from tests import paged_reference as ref
-from tests.test_gpu_paged import BF16, F16, F32, handle, near, reported, run, sess  # noqa: F401
+from tests.test_gpu_paged import BF16, F16, F32, handle, near, reported, run, sess  # noqa: F401,E501
 
 pytestmark = pytest.mark.gpu
 
@@ -213,3 +213,31 @@ def test_lengths_and_pages_are_reported_together(sess, new):
     with pytest.raises(ValueError, match="cu_seqlens.*block_table"):
         sess.sync()
     sess.sync()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("new,past", [([1, 3], [90, 200]), ([140, 60], [0, 33])])
+@pytest.mark.parametrize("scale,softcap,size", [
+    (None, 2.0 ** 20, 1.0), (None, 2.0 ** 20, 2.0 ** 24), (0.125, 2.0 ** -20, 1.0),
+    (2.0 ** -100, 0.0, 2.0 ** 97), (2.0 ** -100, 30.0, 2.0 ** 97)])
+def test_extreme_scales_and_caps(sess, scale, softcap, size, new, past, dtype):
+    """At the ends of what is taken.  A cap of 2^-20 leaves the mean; scores behind a cap of
+    2^20 are held to its last bits in fp32 (2^-4), so the sharp rows there have to be finite
+    and of a value's size only."""
+    s = ref.make(39, dtype, new, past, 8, 2, 64, 16)
+    s["q"] *= size
+    got = run(sess, s, 8, new, scale=scale, softcap=softcap)
+    want = ref.attention(s, new, past, 8, scale, softcap)
+    if softcap == 2.0 ** 20 and size > 1:
+        assert torch.isfinite(got).all()
+        assert got.abs().max() <= s["value"].float().nan_to_num().abs().max() * (1 + 1e-5)
+    else:
+        near(want, got)
+
+
+def test_scales_and_caps_that_fp32_does_not_hold_are_refused(sess):
+    s = ref.make(15, F16, [2], [5], 8, 2, 64, 16)
+    for kw in (dict(scale=1e300), dict(scale=1e-300), dict(softcap=1e300), dict(softcap=1e-300),
+               dict(softcap=1e7), dict(softcap=1e-7), dict(scale=1e-38), dict(scale=1e38)):
+        with pytest.raises(ValueError, match="lies in"):
+            sess.paged_attention(handle(s), s["q"], 8, **kw)
