@@ -524,6 +524,8 @@ ORT_CUDA_API int ort_cuda_paged_kv_append(ort_cuda_session* s, const ort_cuda_pa
                     num_heads <= INT_MAX / D && q_stride >= num_heads * D),
              ORT_CUDA_ERR_INVALID_ARG,
              "paged append: need num_heads a multiple of kv_num_heads and q_stride >= its row");
+  ORTC_CHECK((Q ? num_heads : 0) * D + 2 * row <= INT_MAX, ORT_CUDA_ERR_INVALID_ARG,
+             "paged append: sizes too large");
   const int64_t rows = std::max<int64_t>(num_tokens - 1, 0), qn = num_heads * D;
   ORTC_CHECK(!Q || num_tokens == 0 ||
                  (Q == Q_out ? q_stride == qn : !overlap(Q_out, (rows + 1) * qn, Q, rows * q_stride + qn)),

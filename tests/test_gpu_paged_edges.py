@@ -241,3 +241,19 @@ def test_scales_and_caps_that_fp32_does_not_hold_are_refused(sess):
                dict(softcap=1e7), dict(softcap=1e-7), dict(scale=1e-38), dict(scale=1e38)):
         with pytest.raises(ValueError, match="lies in"):
             sess.paged_attention(handle(s), s["q"], 8, **kw)
+
+
+def test_append_of_a_token_that_32_bits_do_not_count_is_refused(sess):
+    """The features of a token's q, k and v rows together pass 2^31 (checked without tokens:
+    nothing is launched)."""
+    import ctypes
+    from onnx_runtime_dart_b200 import _lib
+    G, D, some = 1 << 24, 64, torch.zeros(4, device="cuda").data_ptr()
+    c = _lib.PagedCacheStruct(some, some, some, some, some, 1, 1, 1, 1, D, G, _lib.CACHE_F16)
+    for heads, rc in ((0, _lib.ERR_INVALID_ARG), (G, _lib.ERR_INVALID_ARG), (None, 0)):
+        kv = 1 << 23 if heads is None else G
+        c.kv_num_heads = kv
+        q = some if heads else 0
+        assert _lib.load().ort_cuda_paged_kv_append(
+            sess.handle, ctypes.addressof(c), q, (heads or 0) * D, some, kv * D, some, kv * D, 0,
+            heads or 0, 0, 0, 0, 0, q, 0) == rc
