@@ -458,12 +458,14 @@ typedef struct ort_cuda_paged_cache {
  * rows k_stride and v_stride floats apart (slices of a fused projection's
  * output need no copy), Q [num_tokens, num_heads * head_size] with row stride
  * q_stride, or NULL with Q_out NULL; Q_out is contiguous and may be Q itself
- * when q_stride is its row length (else it may not overlap Q, K or V).  cos/sin caches [max_pos, rotary_half] as
- * for ort_cuda_group_query_attention (ORT_CUDA_ROTARY_INTERLEAVED for (2i, 2i + 1)
- * pairs; a position >= max_pos is not rotated but left out, and reported as
- * above), or both NULL: no rotation.  The rows of one call must be distinct
- * (no page listed twice within the written range).  head_size a multiple of 8
- * up to 128.  Device pointers only; stream-ordered. */
+ * when q_stride is its row length (else it may not overlap Q, nor ever K, V or
+ * the pages).  The key and value pages are apart.  cos/sin caches
+ * [max_pos, rotary_half] as for ort_cuda_group_query_attention
+ * (ORT_CUDA_ROTARY_INTERLEAVED for (2i, 2i + 1) pairs; a position >= max_pos is
+ * not rotated but left out, and reported as above), or both NULL: no rotation.
+ * The rows of one call must be distinct (no page listed twice within the
+ * written range).  head_size a multiple of 8 up to 128.  Device pointers only;
+ * stream-ordered. */
 ORT_CUDA_API int ort_cuda_paged_kv_append(ort_cuda_session* s, const ort_cuda_paged_cache* cache,
                                           const float* Q, int64_t q_stride, const float* K,
                                           int64_t k_stride, const float* V, int64_t v_stride,
@@ -479,8 +481,8 @@ ORT_CUDA_API int ort_cuda_paged_kv_append(ort_cuda_session* s, const ort_cuda_pa
  * are scale * q.k (scale <= 0: 1/sqrt(head_size); 2^-100 to 2^100) and, with
  * softcap > 0 (2^-20 to 2^20), softcap * tanh(score / softcap).
  * Q [num_tokens, num_heads * head_size] fp32 with row stride q_stride; out
- * [num_tokens, num_heads * head_size] fp32, contiguous, apart from Q.  Query
- * head h reads KV head h / (num_heads / kv_num_heads).
+ * [num_tokens, num_heads * head_size] fp32, contiguous, apart from Q and the
+ * pages.  Query head h reads KV head h / (num_heads / kv_num_heads).
  *   max_seq     bound of the tokens of any one sequence of the call (a
  *               sequence with more is left out and reported)
  *   shared_len  > 0: the first shared_len positions of every sequence hold

@@ -463,6 +463,15 @@ bool overlap(const float* a, int64_t an, const float* b, int64_t bn) {
   return a && b && a < b + bn && b < a + an;
 }
 
+// Whether a range of floats lies in the key or value pages.
+bool in_pages(const ort_cuda_paged_cache* c, const float* a, int64_t an) {
+  const int64_t bytes = c->num_pages * c->page_size * c->kv_num_heads * c->head_size *
+                        (c->type == ORT_CUDA_CACHE_F32 ? 4 : 2);
+  const int64_t n = (bytes + 3) / 4;
+  return overlap(a, an, static_cast<const float*>(c->key), n) ||
+         overlap(a, an, static_cast<const float*>(c->value), n);
+}
+
 // Checks what the host can see of a cache and fills the kernels' view.
 int paged_view(ort_cuda_session* s, const ort_cuda_paged_cache* c, int64_t num_tokens, int flags,
                PagedView* v) {
@@ -535,6 +544,8 @@ ORT_CUDA_API int ort_cuda_paged_kv_append(ort_cuda_session* s, const ort_cuda_pa
                  (!overlap(Q_out, (rows + 1) * qn, K, rows * k_stride + row) &&
                   !overlap(Q_out, (rows + 1) * qn, V, rows * v_stride + row)),
              ORT_CUDA_ERR_INVALID_ARG, "paged append: Q_out overlaps K or V");
+  ORTC_CHECK(!Q || num_tokens == 0 || !in_pages(cache, Q_out, (rows + 1) * qn),
+             ORT_CUDA_ERR_INVALID_ARG, "paged append: Q_out overlaps the pages");
   ORTC_CHECK(k_stride >= row && v_stride >= row, ORT_CUDA_ERR_INVALID_ARG,
              "paged append: k_stride and v_stride must be at least a row");
   ORTC_CHECK((cos_cache == nullptr) == (sin_cache == nullptr), ORT_CUDA_ERR_INVALID_ARG,
@@ -544,6 +555,8 @@ ORT_CUDA_API int ort_cuda_paged_kv_append(ort_cuda_session* s, const ort_cuda_pa
              "paged append: rotary needs cos/sin caches of rotary_half <= head_size / 2 values");
   if (num_tokens == 0 || cache->batch == 0) return ORT_CUDA_OK;
   ORTC_CHECK(K && V, ORT_CUDA_ERR_INVALID_ARG, "NULL argument");
+  ORTC_CHECK(cache->key != cache->value, ORT_CUDA_ERR_INVALID_ARG,
+             "paged append: key and value are the same pages");
   a.q = Q, a.q_out = Q_out, a.q_stride = q_stride, a.heads = Q ? num_heads : 0;
   a.k = K, a.k_stride = k_stride, a.v = V, a.v_stride = v_stride;
   if (cos_cache) {
@@ -588,6 +601,8 @@ ORT_CUDA_API int ort_cuda_paged_attention(ort_cuda_session* s, const ort_cuda_pa
              "paged attention: sizes too large");
   ORTC_CHECK(!overlap(out, num_tokens * num_heads * D, Q, (num_tokens - 1) * q_stride + num_heads * D),
              ORT_CUDA_ERR_INVALID_ARG, "paged attention: out overlaps Q");
+  ORTC_CHECK(!in_pages(cache, out, num_tokens * num_heads * D), ORT_CUDA_ERR_INVALID_ARG,
+             "paged attention: out overlaps the pages");
   a.q = Q, a.q_stride = q_stride, a.out = out;
   a.heads = num_heads, a.group = num_heads / cache->kv_num_heads;
   a.max_seq = (int)std::min<int64_t>(max_seq, num_tokens);

@@ -257,3 +257,19 @@ def test_append_of_a_token_that_32_bits_do_not_count_is_refused(sess):
         assert _lib.load().ort_cuda_paged_kv_append(
             sess.handle, ctypes.addressof(c), q, (heads or 0) * D, some, kv * D, some, kv * D, 0,
             heads or 0, 0, 0, 0, 0, q, 0) == rc
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_outputs_in_the_pages_are_refused(sess, dtype):
+    s = ref.make(40, dtype, [2], [5], 8, 2, 64, 16, garbage=False)
+    h, kv = handle(s), torch.zeros((2, 128), device="cuda")
+    for pages in (s["key"], s["value"]):
+        out = pages.view(torch.uint8).flatten()[-4096:].view(torch.float32).view(2, 512)
+        with pytest.raises(ValueError, match="overlaps the pages"):
+            sess.paged_attention(h, s["q"], 8, out=out)
+        with pytest.raises(ValueError, match="overlaps the pages"):
+            sess.paged_kv_append(h, kv, kv, q=s["q"], num_heads=8, q_out=out)
+    same = {**s, "value": s["key"]}
+    with pytest.raises(ValueError, match="same pages"):
+        sess.paged_kv_append(handle(same), kv, kv)
+    near(ref.attention(same, [2], [5], 8), run(sess, same, 8, [2]))  # reading them is fine
