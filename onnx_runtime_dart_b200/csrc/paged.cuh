@@ -23,8 +23,8 @@ struct PagedView {
 };
 
 // Sequence b of a call: its first token, its token count and its past; no
-// tokens when its lengths do not fit (see fits).  Callers pass no sequence behind the
-// first one whose lengths fall (paged_falls): those before it share no token.
+// tokens when its lengths do not fit (see fits), a count of -1 when they fall.  Callers
+// pass no sequence behind the first whose lengths fall: those before it share no token.
 struct PagedSeq {
   int row0, count, past;
 };
@@ -44,12 +44,9 @@ __host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedView& v, int b
 #ifdef __CUDA_ARCH__
     record_error(v.err, KERR_PAGED_LENGTH);
 #endif
-    s.count = 0;
+    s.count = c1 < c0 ? -1 : 0;
   }
   return s;
-}
-__device__ __forceinline__ bool paged_falls(const PagedView& v, int b) {
-  return v.cu[b + 1] < v.cu[b];
 }
 
 // The sequence that token t belongs to: the first that ends behind t, `batch`
@@ -59,8 +56,9 @@ __device__ __forceinline__ int paged_find(const PagedView& v, int t) {
   const int lane = threadIdx.x & 31;
   for (int b0 = 0; b0 < v.batch; b0 += 32) {
     const bool in = b0 + lane < v.batch;
-    const unsigned m = __ballot_sync(0xffffffffu, in && v.cu[b0 + lane + 1] > t);
-    const unsigned f = __ballot_sync(0xffffffffu, in && paged_falls(v, b0 + lane));
+    const int c0 = in ? v.cu[b0 + lane] : 0, c1 = in ? v.cu[b0 + lane + 1] : 0;
+    const unsigned m = __ballot_sync(0xffffffffu, in && c1 > t);
+    const unsigned f = __ballot_sync(0xffffffffu, c1 < c0);
     if (f && (!m || __ffs(f) < __ffs(m))) break;
     if (m) return b0 + __ffs(m) - 1;
   }

@@ -20,7 +20,8 @@ struct TilePos {
   int base, ramp;
 };
 
-// Sets the sequence of `s`; its number of row tiles (0: not this kernel's).
+// Sets the sequence of `s`; its number of row tiles (0: not this kernel's; count -1: its
+// lengths fall).
 __device__ __forceinline__ int tile_seq(const StreamArgs& p, TilePos& s, int b, int min_past,
                                         int TT, int align) {
   const PagedAttnArgs& a = p.a;
@@ -111,6 +112,7 @@ struct TileRun {
       long long base = 0;
       for (int b0 = 0; b0 < nb; b0 += nt) {
         TilePos t;
+        t.count = 0;
         long long n = 0;
         if (b0 + tid < nb) {
           const int nrt = tile_seq(p, t, b0 + tid, min_past, TT, align);
@@ -122,7 +124,7 @@ struct TileRun {
           if (lane >= o) x += y;
         }
         if (lane == 31) s_scan[warp] = x;
-        const bool falls = !p.prefix && b0 + tid < nb && paged_falls(c, b0 + tid);
+        const bool falls = t.count < 0;
         if (__syncthreads_or(falls)) {  // the list again, without what lies behind
           if (falls) atomicMin(s_falls, b0 + tid);
           __syncthreads();

@@ -188,7 +188,7 @@ struct StreamPos {
   int lo, hi, nt, nrt;      // its keys, key tiles and row tiles
 };
 
-// Sets the sequence of `s`; false: nothing for this kernel.
+// Sets the sequence of `s`; false: nothing for this kernel (count -1: its lengths fall).
 template <int R, int TK>
 __host__ __device__ __forceinline__ bool stream_seq(const StreamArgs& p, StreamPos& s, int b,
                                                     int min_past) {
@@ -206,8 +206,7 @@ __host__ __device__ __forceinline__ bool stream_seq(const StreamArgs& p, StreamP
     s.hi = q.past + q.count;
   }
   const int64_t rows = (int64_t)s.count * a.group;
-  if (rows == 0 || (!p.prefix && rows > p.max_rows)) {
-    s.count = 0;
+  if (rows <= 0 || (!p.prefix && rows > p.max_rows)) {
     s.nt = s.nrt = 0;
     return false;
   }
@@ -583,6 +582,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     long long base = 0;
     for (int b0 = 0; b0 < nb; b0 += 256) {
       StreamPos t;
+      t.count = 0;
       const long long n = b0 + tid < nb && stream_seq<R, TK>(p, t, b0 + tid, min_past)
                               ? stream_places<EXTRA>(t) * G
                               : 0;
@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
         if (lane >= o) x += y;
       }
       if (lane == 31) s_scan[w] = x;
-      const bool falls = !p.prefix && b0 + tid < nb && paged_falls(c, b0 + tid);
+      const bool falls = t.count < 0;
       if (__syncthreads_or(falls)) {  // the list again, without what lies behind
         if (falls) atomicMin(&s_falls, b0 + tid);
         __syncthreads();
