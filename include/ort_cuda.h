@@ -454,7 +454,8 @@ typedef struct ort_cuda_paged_cache {
 /* Appends this call's keys and values to the cache, with RoPE of the keys
  * (and, when Q is given, of the queries) on the way: key row = R(position) .
  * K, value row = V, each rounded once to the cache's type; Q_out = R(position)
- * . Q in fp32.  K and V are [num_tokens, kv_num_heads * head_size] fp32 with
+ * . Q in fp32 (a value beyond the 16-bit type's range becomes an infinity).
+ * K and V are [num_tokens, kv_num_heads * head_size] fp32 with
  * rows k_stride and v_stride floats apart (slices of a fused projection's
  * output need no copy), Q [num_tokens, num_heads * head_size] with row stride
  * q_stride, or NULL with Q_out NULL; Q_out is contiguous and may be Q itself
@@ -490,12 +491,19 @@ ORT_CUDA_API int ort_cuda_paged_kv_append(ort_cuda_session* s, const ort_cuda_pa
  *               block table (whether or not its sequence has tokens in this
  *               call), once for the whole batch; every past_lens[b] of a
  *               sequence with tokens must be at least shared_len
- * fp32 results whatever the cache's type: products, softmax statistics and
- * sums keep 22 bits or more.  Device pointers only; stream-ordered.  A call
- * uses a workspace of its stream (or of the graph being captured), so calls
- * on different streams may run at the same time (two instances of one captured
- * graph share it and may not); the session must outlive the graphs that were
- * captured with its calls. */
+ * fp32 results whatever the cache's type: softmax statistics and sums are fp32,
+ * products are held to 2^-20 (fp32 pages), 2^-22 (fp16) or 2^-24 (bf16) of
+ * theirs, features of a query over fp16 pages to 2^-38 of the row's largest.
+ *
+ * What a row does not see has no part in it, finite or not.  What it sees is to
+ * be finite: a value that is not makes its feature infinite or NaN in the rows
+ * that see it, and no other; a key that is not leaves the rows that see it
+ * unspecified, and a query's feature that is not its row.
+ *
+ * Device pointers only; stream-ordered.  A call uses a workspace of its stream
+ * (or of the graph being captured), so calls on different streams may run at the
+ * same time (two instances of one captured graph share it and may not); the
+ * session must outlive the graphs that were captured with its calls. */
 ORT_CUDA_API int ort_cuda_paged_attention(ort_cuda_session* s, const ort_cuda_paged_cache* cache,
                                           const float* Q, int64_t q_stride, int64_t num_tokens,
                                           int64_t max_seq, int num_heads, double scale,

@@ -742,9 +742,11 @@ class CudaSession:
         cache that already holds their keys (ort_cuda_paged_attention): causal,
         optionally over the last ``local_window_size`` keys, scores optionally
         capped by ``softcap * tanh(score / softcap)``.  ``max_seq`` bounds the
-        tokens of any one sequence (default: the tokens of the call);
+        tokens of any one sequence (default: the tokens of the call, which plans
+        a batch of single tokens as if they were prompts: pass 1 there);
         ``shared_len``: that many first positions are the same in every
-        sequence and are read once, through the block table's first row."""
+        sequence and are read once, through the block table's first row.  What
+        a row sees is to be finite; what it does not see may hold anything."""
         on = self._paged_stream(cache)
         if on is not None:
             with on:

@@ -273,3 +273,99 @@ def test_outputs_in_the_pages_are_refused(sess, dtype):
     with pytest.raises(ValueError, match="same pages"):
         sess.paged_kv_append(handle(same), kv, kv)
     near(ref.attention(same, [2], [5], 8), run(sess, same, 8, [2]))  # reading them is fine
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("new,past", [([1, 3], [600, 300]), ([140, 90], [600, 300])])
+@pytest.mark.parametrize("plant", [math.inf, -math.inf, math.nan])
+def test_values_a_row_sees_that_are_not_finite(sess, new, past, plant, dtype):
+    """They make the feature they stand in not finite in the rows that see them, deep inside
+    the sequence and at the border of the mask, and touch no other feature."""
+    heads, G, D = 8, 2, 64
+    s = ref.make(41, dtype, new, past, heads, G, D, 16)
+    want = ref.attention(s, new, past, heads).view(-1, heads, D)
+    seen = torch.zeros_like(want, dtype=torch.bool)
+    row = 0
+    for b, (n, p0) in enumerate(zip(new, past)):
+        for j, d in ((130 + b, 3), (p0, 17), (p0 + n - 1, 40)):
+            s["value"][int(s["table"][b, j // 16]), j % 16, :, d] = plant
+            seen[row + max(0, j - p0):row + n, :, d] = True
+        row += n
+    got = run(sess, s, heads, new).view(-1, heads, D)
+    assert not torch.isfinite(got[seen]).any()
+    near(want[~seen], got[~seen])
+
+
+def test_query_rows_that_are_not_finite(sess):
+    """They stay in their row."""
+    for dtype in (F32, F16, BF16):
+        for new, past in (([1, 3], [600, 300]), ([140, 90], [600, 300])):
+            s = ref.make(42, dtype, new, past, 8, 2, 64, 16)
+            want = ref.attention(s, new, past, 8)
+            s["q"][0], s["q"][2, 100] = math.nan, math.inf
+            got = run(sess, s, 8, new)
+            keep = torch.ones_like(got, dtype=torch.bool)
+            keep[0] = keep[2, 64:128] = False
+            near(want[keep], got[keep])
+            assert got[0].isnan().all() and not torch.isfinite(got[2, 64:128]).any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("lead", [0, 1])  # 16-byte pieces, and the kernel for any alignment
+def test_append_rounds_once(sess, dtype, interleaved, lead):
+    """Keys whose rotation lies next to the middle of two 16-bit numbers, where fp32 holds
+    the middle only: the nearest of the two all the same.  And keys drawn at random."""
+    import numpy as np
+    n, G, D, half = 64, 2, 128, 64
+    bits = 11 if dtype == F16 else 8
+    g = torch.Generator().manual_seed(43)
+    r = torch.randint(2 ** (bits - 1), 2 ** bits, (n // 2, G * D), generator=g).double() + 0.5
+    middle = r * 2.0 ** -(bits - 1) * (torch.randint(0, 2, r.shape, generator=g) * 2 - 1)
+    k = torch.cat([middle, torch.randn((n // 2, G * D), generator=g).double()]).float()
+    assert torch.equal(k[:n // 2].double(), middle)
+    ang = torch.rand((n, half), generator=g, dtype=torch.float64) * 6.3
+    cos, sin = ang.cos().float(), ang.sin().float()
+    cos[:n // 2], sin[:n // 2] = 1.0, 2.0 ** -30
+    s = ref.make(44, dtype, [n], [0], 2, G, D, 16)
+    fused = torch.zeros((n, G * D + 4 * lead), device="cuda")
+    rows = fused[:, lead:lead + G * D] if lead else fused
+    rows.copy_(k)
+    sess.paged_kv_append(handle(s), rows, rows, cos_cache=cos.cuda(), sin_cache=sin.cuda(),
+                         rotary_interleaved=interleaved)
+    sess.sync()
+    want = ref.rotate(k.view(n, G, D), cos, sin, interleaved)  # exact in the rows of middles
+    pos = torch.arange(n)
+    have = s["key"][s["table"][0].cpu()[pos // 16].long(), pos % 16].cpu()
+    word = have.view(torch.int16)
+    off = (have.double() - want).abs()
+    for step in (-1, 1):  # the neighbours
+        other = (word + step).view(dtype).double()
+        away = (other - want).abs()
+        assert (off[:n // 2] < away[:n // 2]).all()
+        assert (off[n // 2:] <= away[n // 2:] * (1 + 1e-9)).all()
+    assert np.isfinite(have.double().numpy()).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("new,past", [([1, 1, 1], [200, 40, 9]), ([90, 1, 33], [20, 300, 0])])
+@pytest.mark.parametrize("attrs", [dict(local_window_size=1), dict(local_window_size=37),
+                                   dict(softcap=3.0), dict(scale=0.5),
+                                   dict(scale=0.05, softcap=20.0, local_window_size=64)])
+def test_dispatch_hands_on_the_attributes(sess, new, past, attrs, dtype):
+    """A window of w keys has the query's own among them: w = 1 gives the key's own value."""
+    heads, G, D, n = 8, 2, 64, sum(new)
+    s = ref.make(45, dtype, new, past, heads, G, D, 16)
+    k, v = (torch.randn((n, G * D), device="cuda") for _ in range(2))
+    out, key, value = sess.dispatch(
+        dict(op_type="PagedAttention", inputs=["q", "k", "v", "kc", "vc", "cu", "past", "bt"],
+             attrs=dict(num_heads=heads, kv_num_heads=G, **attrs)),
+        dict(q=s["q"], k=k, v=v, kc=s["key"], vc=s["value"], cu=s["cu"], past=s["past"],
+             bt=s["table"]))
+    sess.sync()
+    want = ref.attention(s, new, past, heads, attrs.get("scale"), attrs.get("softcap", 0.0),
+                         attrs.get("local_window_size", 0))
+    near(want, out)
+    if attrs == dict(local_window_size=1):
+        own = v.to(dtype).double().view(n, G, 1, D).expand(n, G, heads // G, D).reshape(n, -1)
+        near(own, out)
