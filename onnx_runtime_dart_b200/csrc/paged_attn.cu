@@ -11,15 +11,22 @@ namespace {
 
 size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Query rows of a sequence and KV head up to which the stream kernel takes it.  The
-// tiles win from 33 to 64 rows where their segments fill the device (16-bit pages, 8
-// sequences of 8 KV heads over 2000 to 4000 keys, 64 rows: 58 us against 84, 32 rows: 53
-// against 49) and lose where few do (1 sequence, 64 rows: 36 against 22); over fp32
-// pages the stream wins to 64 rows either way (276 against 211, 68 against 38; 128 rows:
-// 324 against 408).
-// A shared prefix is one sequence.
+// Query rows of a sequence and KV head up to which the stream kernel takes it.  From 33
+// to 64 rows over 16-bit pages the tiles win where their segments fill the device, and
+// lose where few do.  Tiles and stream, us, 40 and 64 rows over 2000 to 4000 keys of
+// heads of 128:
+//   segments   fp16, 40        64            bf16, 40        64
+//    8         39.3, 22.7      41.2, 22.8    43.2, 24.4      43.4, 25.8
+//   16         37.6, 26.6      39.2, 29.5    39.2, 28.9      41.2, 33.0
+//   24         40.7, 33.0      41.2, 39.1    44.1, 37.1      45.3, 45.3
+//   32         42.6, 39.2      43.3, 47.3    47.3, 45.3      47.9, 55.4
+//   48         51.4, 57.5      52.4, 69.9    60.2, 66.8      61.5, 82.3
+//   64         59.7, 70.3      61.0, 89.3    71.6, 82.5      72.5, 105
+// With 32 rows the stream is ahead at 64 segments too (53, 49); over fp32 pages it wins
+// to 64 rows either way (276, 211; one sequence 68, 38; 128 rows: 324, 408).  A shared
+// prefix is one sequence.
 int stream_limit(const PagedAttnArgs& a, int sequences) {
-  const bool many = (int64_t)sequences * a.c.kv_heads > 16;
+  const bool many = (int64_t)sequences * a.c.kv_heads > 24;
   return a.c.type != ORT_CUDA_CACHE_F32 && many ? 32 : 64;
 }
 
@@ -29,7 +36,10 @@ int stream_rows(int64_t rows) { return rows <= 8 ? 8 : 16; }
 int padded_head(int D) { return D <= 64 ? 64 : 128; }
 
 // Whether tiles of 128 rows may be used (csrc/paged_tile.cuh for 16-bit pages,
-// csrc/paged_rows.cuh for fp32): two tokens' heads at least fit one.
+// csrc/paged_rows.cuh for fp32): two tokens' heads at least fit one.  More heads on a KV
+// head go to the stream at any length, where every tile of 16 rows reads all keys of its
+// sequence: a prompt of 2048 tokens, one KV head of 64, takes 179 us with 64 query heads
+// and 1431 with 71 (fp16; bf16 195, 1564; fp32 880, 3068).
 bool tile_ok(const PagedAttnArgs& a) { return a.group <= 64; }
 
 template <typename K>
