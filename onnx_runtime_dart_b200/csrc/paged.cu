@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(128, 8) append_kernel(const __grid_constant__ 
 }
 
 template <typename T>
-int launch_append_type(AppendArgs& a, cudaStream_t st) {
+int launch_append_type(AppendArgs& a, int sm_count, cudaStream_t st) {
   const PagedView& c = a.c;
   auto ok = [](const void* p, int64_t stride) {
     return ((uintptr_t)p & 15) == 0 && stride % 4 == 0;
@@ -435,8 +435,8 @@ int launch_append_type(AppendArgs& a, cudaStream_t st) {
   }
   const int pieces = (a.heads + 2 * c.kv_heads) * (c.D / 8);
   a.piece_div.set((uint32_t)(c.D / 8));
-  // one piece a thread until the CTAs fill the device, then three
-  const int it = (int64_t)c.num_tokens * pieces > 148 * 2048 ? 3 : 1;
+  // one piece a thread until there are 2048 threads a SM, then three
+  const int it = (int64_t)c.num_tokens * pieces > (int64_t)sm_count * 2048 ? 3 : 1;
   a.parts = (pieces + 128 * it - 1) / (128 * it);
   ORTC_CHECK((int64_t)c.num_tokens * a.parts <= INT_MAX, ORT_CUDA_ERR_INVALID_ARG,
              "paged append: sizes too large");
@@ -449,11 +449,11 @@ int launch_append_type(AppendArgs& a, cudaStream_t st) {
   return ORT_CUDA_OK;
 }
 
-int launch_append(AppendArgs& a, cudaStream_t st, int64_t* launches) {
+int launch_append(AppendArgs& a, int sm_count, cudaStream_t st, int64_t* launches) {
   a.page_div.set((uint32_t)a.c.page_size);
-  const int rc = a.c.type == ORT_CUDA_CACHE_F32   ? launch_append_type<float>(a, st)
-                 : a.c.type == ORT_CUDA_CACHE_F16 ? launch_append_type<__half>(a, st)
-                                                  : launch_append_type<__nv_bfloat16>(a, st);
+  const int rc = a.c.type == ORT_CUDA_CACHE_F32   ? launch_append_type<float>(a, sm_count, st)
+                 : a.c.type == ORT_CUDA_CACHE_F16 ? launch_append_type<__half>(a, sm_count, st)
+                                                  : launch_append_type<__nv_bfloat16>(a, sm_count, st);
   if (rc == ORT_CUDA_OK) (*launches)++;
   return rc;
 }
@@ -565,7 +565,7 @@ ORT_CUDA_API int ort_cuda_paged_kv_append(ort_cuda_session* s, const ort_cuda_pa
   }
   DeviceGuard guard(s->device);
   OpTimer timer(s, "PagedKVAppend");
-  return launch_append(a, s->stream, &s->launches);
+  return launch_append(a, s->sm_count, s->stream, &s->launches);
 } catch (const std::exception& e) {
   return fail(ORT_CUDA_ERR_OOM, std::string("paged append: ") + e.what());
 }
