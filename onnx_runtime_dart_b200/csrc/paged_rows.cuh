@@ -5,10 +5,10 @@
 // both sides split in two, fp32 softmax and sums); here the eight warps share the
 // keys, 32 at a time through a ring of shared memory with one barrier a block, where
 // there they share the rows.  Each warp leaves out the steps whose keys none of its rows
-// sees (the causal border, the window).  Bound by the tensor cores' tf32 rate through
-// mma.sync, three products for each; what TMEM would hold as fp32 operands in two parts
-// leaves no room for a second key block beside the accumulators.  1000 + 300 tokens of
-// 32 heads of 64: 174 us, 29 TFLOP/s; 2048 tokens of heads of 128: 865 us, 40 TFLOP/s.
+// sees (the causal border, the window).  Bound by the latency of eight warps, two a
+// scheduler at 230 registers and more (tensor pipe 34 %, issue slots 40 %); each of them
+// splits every key and value into its two tf32 parts for itself.  1000 + 300 tokens of 32
+// heads of 64: 177 us, 29 TFLOP/s; 2048 tokens of heads of 128: 877 us, 39 TFLOP/s.
 #pragma once
 
 #include "paged_segments.cuh"

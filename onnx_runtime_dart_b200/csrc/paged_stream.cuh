@@ -23,9 +23,11 @@
 // rows, a row's hi and lo parts are rows r and r + 8 of one MMA, so the split
 // costs nothing.
 //
-// Bound by memory: 64 sequences of 100 to 8191 keys, fp16, 81 us, 5.9 TB/s (0.90 of
-// the copy); one of 131000 keys 94 us, 5.7 TB/s; bf16 with capped scores and 8 rows
-// 4.2 TB/s, by the products and tanh of two warps a scheduler.
+// Bound by memory over fp16 pages: 64 sequences of 100 to 8191 keys 84 us, 5.7 TB/s
+// (0.87 of the copy); one of 131000 keys 98 us, 5.5 TB/s.  bf16 (100 us) and fp32 pages
+// (203 us) take more steps a key with two warps a scheduler, and are bound by their
+// latency at 4.8 and 4.7 TB/s, 8 rows with capped scores at 4.1 (tensor pipe 26 %, issue
+// slots 38 %).
 //
 // Operand layouts avoid shuffles and transposes: the feature order of q.k is
 // free, so a lane's 16-byte chunk of a key row serves as its B operand of two
