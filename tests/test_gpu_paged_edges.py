@@ -369,3 +369,70 @@ def test_dispatch_hands_on_the_attributes(sess, new, past, attrs, dtype):
     if attrs == dict(local_window_size=1):
         own = v.to(dtype).double().view(n, G, 1, D).expand(n, G, heads // G, D).reshape(n, -1)
         near(own, out)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("head", [8, 24, 48, 104])
+@pytest.mark.parametrize("heads,kv_heads", [(3, 3), (4, 1)])
+def test_small_and_odd_heads_on_whole_pages(sess, head, heads, kv_heads, dtype):
+    """Heads narrower than a box of a page, prompts and single tokens."""
+    new, past = [150, 1], [20, 300]
+    s = ref.make(46, dtype, new, past, heads, kv_heads, head, 16)
+    near(ref.attention(s, new, past, heads), run(sess, s, heads, new))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("window", [2 ** 31 - 2, 2 ** 31 - 1, 2 ** 40])
+def test_windows_longer_than_any_sequence(sess, window, dtype):
+    for new, past, shared in (([150, 1], [20, 300], 0), ([150, 1], [20, 300], 17), ([1], [9], 0)):
+        s = ref.make(47, dtype, new, past, 8, 2, 64, 16, shared)
+        near(ref.attention(s, new, past, 8),
+             run(sess, s, 8, new, local_window_size=window, shared_len=shared))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_output_at_an_odd_address(sess, dtype):
+    for new, past, shared in (([150, 1], [20, 300], 0), ([90, 2], [20, 300], 17), ([1], [9], 0)):
+        s = ref.make(48, dtype, new, past, 8, 2, 64, 16, shared)
+        n = s["q"].numel()
+        out = torch.full((n + 2,), 7.0, device="cuda")
+        run(sess, s, 8, new, shared_len=shared, out=out[1:-1].view(-1, 512))
+        near(ref.attention(s, new, past, 8), out[1:-1].view(-1, 512))
+        assert out[0] == 7.0 and out[-1] == 7.0
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("shared", [0, 16])
+def test_call_whose_sequences_are_all_empty(sess, shared, dtype):
+    """A padded step without a token in it: nothing is written, nothing reported."""
+    s = ref.make(49, dtype, [0, 0, 0], [40, 20, 16], 8, 2, 64, 16, shared)
+    for n in (1, 200):
+        q = torch.full((n, 512), math.nan, device="cuda")
+        out = torch.full_like(q, 7.0)
+        run(sess, {**s, "q": q}, 8, [n], out=out, shared_len=shared)
+        assert (out == 7.0).all()
+
+
+def test_captured_step_follows_a_batch_that_falls_apart_and_recovers(sess):
+    """Replays of one captured call over lengths that fit, fall, and fit again."""
+    new, past, heads = [70, 1, 40], [100, 300, 5], 8
+    s = ref.make(50, F16, new, past, heads, 2, 64, 16)
+    want = run(sess, s, heads, new)
+    good = s["cu"].clone()
+    out, h = torch.zeros_like(s["q"]), handle(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        sess.paged_attention(h, s["q"], heads, max_seq=70, out=out)
+    for _ in range(3):
+        out.fill_(7.0)
+        s["cu"].copy_(good)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        sess.sync()
+        out.fill_(7.0)
+        s["cu"][2] = 3
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[:70], want[:70]) and (out[70:] == 7.0).all()
+        reported(sess, "cu_seqlens")
