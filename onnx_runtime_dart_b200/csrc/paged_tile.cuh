@@ -13,7 +13,7 @@
 // other), an MMA warp, and loaders: TMA boxes of as many tokens as a power of
 // two divides the page size, or, where that is below 8, cp.async in pieces of
 // 16 bytes by three warps (a 2048-token prompt on pages of 16, 24, 17 tokens:
-// 137, 152, 322 us).  A warpgroup's thread owns one query row: it reads the
+// 140, 152, 335 us).  A warpgroup's thread owns one query row: it reads the
 // row's scores from TMEM, writes the weights back over them as the A operand of p.v, and adds each
 // block's product, which comes in TMEM columns of its own, to its fp32 output in
 // registers (so sums over many blocks are rounded, where the tensor cores cut
@@ -26,8 +26,8 @@
 // bound is 1/2 (1/3) of the dense rate.
 //
 // Bound by the softmax warpgroups and by what lies between two segments: a
-// 4096-token prompt of 32 heads of 128 over fp16 pages takes 335 us, 410 TFLOP/s of
-// useful products (tensor pipe 42 %); a mixed bf16 step with capped scores 131.
+// 4096-token prompt of 32 heads of 128 over fp16 pages takes 340 us, 404 TFLOP/s of
+// useful products (tensor pipe 42 %); a mixed bf16 step with capped scores 129.
 //
 // TMEM columns: scores / weights of the two warpgroups (KB, or KB + KB / 2
 // where three parts need more than the scores), then their p.v (DP each).
