@@ -21,6 +21,7 @@ namespace ortc {
 // being captured on that stream: calls on two streams, and two captured graphs
 // replayed at once, never share one.  Streams are told apart by their ids: a handle
 // may come again when its stream is destroyed, even with work of it still to run.  A
+// stream's workspace is kept until the session closes or its handle comes again.  A
 // graph's workspace is handed back when the graph and everything instantiated from it
 // are gone (a CUDA user object), and is reused by later captures.  The first
 // kTicketBytes are zero between calls.

@@ -436,3 +436,27 @@ def test_captured_step_follows_a_batch_that_falls_apart_and_recovers(sess):
         torch.cuda.synchronize()
         assert torch.equal(out[:70], want[:70]) and (out[70:] == 7.0).all()
         reported(sess, "cu_seqlens")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("new,past,shared,window", [
+    ([1, 2], [40, 90], 0, 0), ([130, 70], [40, 90], 0, 30), ([130, 3], [40, 90], 33, 0),
+    ([1, 2], [40, 90], 33, 60)])
+def test_tokens_before_the_first_sequence_are_padding(sess, new, past, shared, window, dtype):
+    heads, G, D, lead = 8, 2, 64, 9
+    s = ref.make(51, dtype, new, past, heads, G, D, 16, shared)
+    want = ref.attention(s, new, past, heads, window=window)
+    q = torch.cat([torch.full((lead, heads * D), math.nan, device="cuda"), s["q"]])
+    t = {**s, "q": q, "cu": s["cu"] + lead}
+    out = torch.full_like(q, 7.0)
+    run(sess, t, heads, new, out=out, shared_len=shared, local_window_size=window)
+    near(want, out[lead:])
+    assert (out[:lead] == 7.0).all()
+    kv = torch.randn((len(q), G * D), device="cuda")
+    kv[:lead] = math.nan
+    before = s["key"].isnan().sum()
+    sess.paged_kv_append(handle(t), kv, kv)
+    sess.sync()
+    assert s["key"].isnan().sum() == before
+    page = int(s["table"][0, past[0] // 16])
+    assert torch.equal(s["key"][page, past[0] % 16].flatten(), kv[lead].to(dtype))
